@@ -112,7 +112,8 @@ int tllm_stream_wait_event(tllm_stream_t stream, void *event);
 /* Device-side error word of the current device (bit set: 1 = a bounded
  * wait ran out, 2 = a device-side length exceeded its bound, 4 = a token id
  * was out of range, 8 = dynamic shared memory misaligned, 16 = a projection
- * launch with an invalid pipeline layout). Waits for the library stream
+ * launch with an invalid pipeline layout, 32 = a page, sequence, position or
+ * beam index of the paged cache was out of range). Waits for the library stream
  * first; reset != 0 clears the word. Kernels report through it instead of
  * trapping. */
 int tllm_device_error(int *code, int reset);
@@ -230,6 +231,188 @@ int tllm_gqa_rows_hint(const float *q, long q_row_stride, long q_head_stride,
                        int head_dim, int cache_batch, int max_seq, int max_len,
                        float sm_scale, void *partial, size_t partial_bytes,
                        int32_t *counters, long keys_hint, tllm_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged KV cache                                                            */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * K and V of one layer in pages of page_size token slots, and the page tables
+ * of its sequences. Token j of sequence s is slot j % page_size of page
+ * table[s * table_stride + j / page_size]; slot t of head h of page p starts
+ * at element p * page_stride + h * head_stride + t * slot_stride of k_pages
+ * and v_pages (its head_dim values are contiguous), so pages of
+ * (n_kv_head, page_size, head_dim) and of (page_size, n_kv_head, head_dim)
+ * are both described. Table entries of tokens that no call reads or writes
+ * may hold anything; an entry that is needed and outside [0, n_pages) makes
+ * its tokens invisible (reads) or skipped (writes) and sets bit 32 of the
+ * device error word. No counterpart in the reference, whose cache is one
+ * preallocated block per sequence (smollm2_triton/model.py:219-225).
+ */
+typedef struct {
+  void *k_pages;
+  void *v_pages;
+  int kv_dtype;        /* F32 or BF16 */
+  int n_pages;
+  int page_size;       /* token slots of a page, >= 1 */
+  int n_kv_head;
+  int head_dim;
+  int n_seq;           /* rows of the table */
+  int table_cols;      /* pages a sequence may have */
+  int reserved;        /* 0 */
+  long page_stride;    /* elements */
+  long head_stride;
+  long slot_stride;
+  long table_stride;   /* entries between table rows */
+  const int32_t *table;
+} tllm_paged_kv;
+
+/*
+ * Attention of one token per row over a paged cache. Row r, head h attends
+ * the keys j of sequence row_seq[r] (NULL: sequence r) with
+ *   j < row_len[r]  and  (window == 0 or j < sinks or j >= row_len[r] - window)
+ * (a sliding window of the last `window` tokens plus the first `sinks`):
+ *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j)
+ * and a row without a visible key gives zeros. Pages outside the window and
+ * the sinks are not read, so they may have been freed. q, out, their strides
+ * and formats as for tllm_gqa_rows; q 16-byte aligned with strides of whole
+ * 16 bytes. max_len (0: the table's capacity) bounds row_len on the host and
+ * keys_hint (0: unknown) is the sum of row_len as far as the caller knows it;
+ * both only size the split of each row's keys over the GPU: results are
+ * right for any value. row_len above the table's capacity is clamped (bit 2 of the
+ * device error word). bf16 and fp32 caches; head_dim up to 512 whose rows
+ * are whole 16-byte units. Scratch: partial (tllm_paged_attention_workspace;
+ * fewer bytes give fewer, longer splits) and counters, zero-filled once and
+ * zero again after every call; a call that overlaps another on the GPU needs
+ * its own. No counterpart in the reference (its decode attention over the
+ * preallocated cache: triton_llm/kernels/attention_gqa.py:149-269).
+ */
+int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_head,
+                                   int head_dim, size_t *partial_bytes,
+                                   size_t *counter_bytes);
+int tllm_paged_attention(const tllm_paged_kv *kv, const float *q,
+                         long q_row_stride, long q_head_stride,
+                         const int32_t *row_seq, const int32_t *row_len,
+                         void *out, int out_dtype, long out_plane_rows,
+                         long out_row_stride, long out_head_stride, int rows,
+                         int n_head, int max_len, long keys_hint, int window,
+                         int sinks, float sm_scale, void *partial,
+                         size_t partial_bytes, int32_t *counters,
+                         size_t counter_bytes, tllm_stream_t stream);
+
+/*
+ * New tokens into a paged cache, with rotary positions. Row r of q
+ * (n_head heads), k and v (n_kv_head heads each) is token row_pos[r] of
+ * sequence row_seq[r] (NULL: sequence r). The first rotary_dim values of every
+ * q and k head are rotated by the angles of row row_pos[r] of the tables
+ * cos_t / sin_t (n_pos, rotary_dim / 2); pair i is (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) with interleaved != 0:
+ *   x' = x cos - y sin,  y' = y cos + x sin
+ * and the other values pass. k and v are rounded to the cache's type into
+ * their slots; q goes to q_out (fp32, may be q itself). q NULL: k and v only.
+ * cos_t NULL: no rotation. src_dtype (F32 or BF16) is the type of q, k and v.
+ * row_src (NULL: r) is the source row of q, k and v for row r. blocked != 0:
+ * the sources hold each head as blocks of 8 values (8b..8b+7, D/2+8b..D/2+8b+7),
+ * the row order of the QKV projection (tllm_linear op QKV); outputs are in
+ * plain order. lens_out (may be NULL): raised to row_pos + 1 at the row's
+ * sequence where it is lower (rows may come in any order).
+ * Strides in elements. A row whose position is outside the table's capacity
+ * or n_pos, or whose sequence or page is out of range, is skipped and sets
+ * bit 32 of the device error word. Two rows must not name the same token.
+ * Replaces, for pages, triton_llm/kernels/rope.py:153-222 and the cache write
+ * of smollm2_triton/model.py:296-308.
+ */
+typedef struct {
+  const void *q;          /* NULL: none */
+  const void *k;
+  const void *v;
+  float *q_out;
+  const int32_t *row_src;
+  const int32_t *row_seq;
+  const int32_t *row_pos;
+  int32_t *lens_out;
+  const float *cos_t;     /* NULL: no rotation */
+  const float *sin_t;
+  long q_row_stride, q_head_stride;
+  long k_row_stride, k_head_stride;
+  long v_row_stride, v_head_stride;
+  long q_out_row_stride, q_out_head_stride;
+  int src_dtype;
+  int rows;
+  int n_head;
+  int rotary_dim;
+  int n_pos;
+  int interleaved;
+  int blocked;
+  int reserved;           /* 0 */
+} tllm_paged_rows;
+int tllm_paged_append(const tllm_paged_kv *kv, const tllm_paged_rows *rows,
+                      tllm_stream_t stream);
+
+/*
+ * Page copies over the planes of an arena (K and V of every layer), for
+ * forking and compacting sequences: for every copy i and plane p
+ *   the first fill[i] slots (NULL: page_size) of each of `heads` runs of page
+ *   dst[i] = those of page src[i].
+ * Slot t of run h of page g of plane p is row_bytes bytes at byte
+ * p * plane_stride + g * page_stride + h * run_stride + t * row_bytes. src,
+ * dst and fill are on the device. A copy with src == dst or a negative src or
+ * dst does nothing; one outside [0, n_pages) or with fill outside
+ * [0, page_size] is skipped and sets bit 32 of the device error word. No page
+ * may be the dst of two copies, nor the dst of one and the src of another.
+ * No counterpart in the reference.
+ */
+int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
+                   int n_pages, int heads, long run_stride, int page_size,
+                   int row_bytes, const int32_t *src, const int32_t *dst,
+                   const int32_t *fill, int n_copies, tllm_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Beam search                                                               */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * One selection step of beam search for `groups` requests of `beams` beams
+ * each (rows g * beams + b of logits (rows, vocab) f32, row stride ld, 0: vocab):
+ *   candidate (b, t) = scores[g][b] + (logits[b][t] - logsumexp(logits[b]))
+ * and the k best of each group's beams * vocab candidates, best first, equal
+ * ones by the lower beam, then the lower token: out_scores, out_parents
+ * (beam within the group) and out_tokens, all (groups, k). A beam with
+ * done[row] != 0 (done may be NULL) has one candidate, (pad_token,
+ * scores[row]). NaN candidates, and all of a beam whose score is +inf, count
+ * as -inf. 1 <= k <= 64, k <= vocab,
+ * beams <= 32. Scratch: tllm_beam_workspace bytes, zero-filled once; a call
+ * that overlaps another on the GPU needs its own. The reference selects
+ * greedily or by sampling (smollm2_triton/model.py:566-584).
+ */
+int tllm_beam_workspace(int groups, int beams, int vocab, int k, size_t *bytes);
+int tllm_beam_select(const float *logits, long ld, const float *scores,
+                     const int32_t *done, int pad_token, int groups, int beams,
+                     int vocab, int k, float *out_scores, int32_t *out_parents,
+                     int32_t *out_tokens, void *workspace, size_t workspace_bytes,
+                     tllm_stream_t stream);
+
+/*
+ * Page tables after a selection step: beam i of group g continues beam
+ * parents[g][i]. lens[row] tokens are cached for each row before the step
+ * (equal within a group: its first row's is used); c = lens / page_size and
+ * f = lens % page_size are the column of the partly filled page and its
+ * tokens. For every row
+ *   table_out[row][j] = table_in[parent][j]          for j < c
+ *   table_out[row][j] = table_in[row][j]             for j > c, or j == c and f == 0
+ * and for f > 0 the page of column c, which every row of table_in owns alone,
+ * stays with its beam's first child (lowest i); the other children get the
+ * pages of the beams without a child, in order, and copy_src / copy_dst /
+ * copy_fill[row] name the page copy (tllm_page_copy) that fills theirs
+ * (src == dst for a first child; -1, -1, 0 where f == 0). table_out may be
+ * table_in. Parents or lengths out of range leave their group's tables as
+ * they were, name no copies and set bit 32 of the device error word.
+ */
+int tllm_beam_reorder(const int32_t *parents, const int32_t *lens,
+                      const int32_t *table_in, int32_t *table_out, int groups,
+                      int beams, int table_cols, int page_size,
+                      int32_t *copy_src, int32_t *copy_dst, int32_t *copy_fill,
+                      tllm_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Projections (GEMM with fused epilogues)                                   */

@@ -56,6 +56,7 @@ enum DeviceError : int {
   DEV_ERR_TOKEN_RANGE = 4,    // a token id outside [0, vocab)
   DEV_ERR_SMEM_ALIGN = 8,     // dynamic shared memory not 1024-byte aligned
   DEV_ERR_LAYOUT = 16,        // a launch whose ring / issuer layout is invalid
+  DEV_ERR_PAGE = 32,          // a page, sequence, position or beam index out of range
 };
 int *device_error_ptr();
 

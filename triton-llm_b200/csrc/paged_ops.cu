@@ -1,0 +1,248 @@
+// Writing and moving the pages of a paged KV cache, for sm_100a: new tokens
+// with rotary positions (tllm_paged_append) and page copies over the planes of
+// an arena (tllm_page_copy).
+#include "paged.cuh"
+
+namespace tllm {
+namespace {
+
+// --------------------------------------------------------------------------
+// Append
+// --------------------------------------------------------------------------
+struct AppendParams {
+  PagedView kv;
+  tllm_paged_rows in;
+  int *err;
+};
+
+template <typename S>
+__device__ __forceinline__ float load_src(const S *p) {
+  if constexpr (sizeof(S) == 4)
+    return *p;
+  else
+    return bf16_bits_to_f32(*p);
+}
+
+// Position of value d of a head in the source.
+__device__ __forceinline__ int source_dim(int d, int D, int blocked) {
+  if (!blocked) return d;
+  const int half = D >> 1;
+  return d < half ? (d >> 3) * 16 + (d & 7) : ((d - half) >> 3) * 16 + 8 + ((d - half) & 7);
+}
+
+// Row `row` of the call: cache row index, position, page, slot; false (and an
+// error bit) where an index is out of range.
+struct AppendRow {
+  int seq, pos, page, slot;
+  size_t src;
+};
+__device__ __forceinline__ bool append_row(const AppendParams &p, int row, AppendRow *r) {
+  r->seq = p.in.row_seq ? p.in.row_seq[row] : row;
+  r->pos = p.in.row_pos[row];
+  r->src = p.in.row_src ? p.in.row_src[row] : row;
+  bool ok = r->seq >= 0 && r->seq < p.kv.n_seq && r->pos >= 0 &&
+            r->pos < p.kv.table_cols * p.kv.page_size &&
+            (!p.in.cos_t || r->pos < p.in.n_pos);
+  if (ok) {
+    const int col = p.kv.column(r->pos);
+    r->slot = r->pos - col * p.kv.page_size;
+    r->page = p.kv.table[(size_t)r->seq * p.kv.table_stride + col];
+    ok = r->page >= 0 && r->page < p.kv.n_pages;
+  }
+  if (!ok && threadIdx.x == 0) atomicOr(p.err, DEV_ERR_PAGE);
+  return ok;
+}
+
+// Any head_dim, rotary part and alignment: one thread per rotated pair or
+// passed value.
+template <typename S, typename T>
+__global__ void append_kernel(const __grid_constant__ AppendParams p) {
+  griddep_launch();
+  griddep_wait();
+  const int row = blockIdx.x;
+  AppendRow r;
+  if (!append_row(p, row, &r)) return;
+  if (threadIdx.x == 0 && p.in.lens_out) atomicMax(p.in.lens_out + r.seq, r.pos + 1);
+  const int D = p.kv.head_dim, H = p.in.q ? p.in.n_head : 0, K = p.kv.n_kv;
+  const int rot = p.in.cos_t ? p.in.rotary_dim : 0, pairs = rot >> 1;
+  const int per = D - pairs;
+  for (int i = threadIdx.x; i < (H + 2 * K) * per; i += blockDim.x) {
+    const int head = i / per, u = i - head * per;
+    const bool is_v = head >= H + K;
+    const S *src;
+    float *qo = nullptr;
+    T *to = nullptr;
+    if (head < H) {
+      src = static_cast<const S *>(p.in.q) + r.src * p.in.q_row_stride +
+            (size_t)head * p.in.q_head_stride;
+      qo = p.in.q_out + (size_t)row * p.in.q_out_row_stride +
+           (size_t)head * p.in.q_out_head_stride;
+    } else if (!is_v) {
+      src = static_cast<const S *>(p.in.k) + r.src * p.in.k_row_stride +
+            (size_t)(head - H) * p.in.k_head_stride;
+      to = static_cast<T *>(p.kv.k) + p.kv.offset(r.page, head - H, r.slot);
+    } else {
+      src = static_cast<const S *>(p.in.v) + r.src * p.in.v_row_stride +
+            (size_t)(head - H - K) * p.in.v_head_stride;
+      to = static_cast<T *>(p.kv.v) + p.kv.offset(r.page, head - H - K, r.slot);
+    }
+    auto put = [&](int d, float v) {
+      if (qo)
+        qo[d] = v;
+      else if constexpr (sizeof(T) == 4)
+        to[d] = v;
+      else
+        to[d] = f32_to_bf16_bits(v);
+    };
+    if (u < pairs) {
+      const int a = p.in.interleaved ? 2 * u : u;
+      const int b = p.in.interleaved ? 2 * u + 1 : u + pairs;
+      const float x = load_src(src + source_dim(a, D, p.in.blocked));
+      const float y = load_src(src + source_dim(b, D, p.in.blocked));
+      float c = 1.f, s = 0.f;
+      if (!is_v) {
+        c = p.in.cos_t[(size_t)r.pos * pairs + u];
+        s = p.in.sin_t[(size_t)r.pos * pairs + u];
+      }
+      put(a, is_v ? x : x * c - y * s);
+      put(b, is_v ? y : y * c + x * s);
+    } else {
+      const int d = u + pairs;
+      put(d, load_src(src + source_dim(d, D, p.in.blocked)));
+    }
+  }
+}
+
+template <typename S, typename T>
+int launch_append(const AppendParams &p, cudaStream_t st) {
+  const int D = p.kv.head_dim, rot = p.in.cos_t ? p.in.rotary_dim : 0;
+  const long items = ((p.in.q ? p.in.n_head : 0) + 2L * p.kv.n_kv) * (D - rot / 2);
+  const int threads = items >= 512 ? 512 : (int)((items + 31) / 32 * 32);
+  TLLM_CUDA(launch_pdl(append_kernel<S, T>, dim3(p.in.rows), dim3(threads), 0, st, p));
+  return TLLM_OK;
+}
+
+// --------------------------------------------------------------------------
+// Page copies
+// --------------------------------------------------------------------------
+struct CopyParams {
+  char *arena;
+  const int *src, *dst, *fill;
+  long plane_stride, page_stride, run_stride;
+  int n_pages, heads, page_size, row_bytes;
+  int *err;
+};
+
+// One CTA per (copy, plane); units of type U.
+template <typename U>
+__global__ void page_copy_kernel(const CopyParams p) {
+  griddep_launch();
+  griddep_wait();
+  const int i = blockIdx.x;
+  const int src = p.src[i], dst = p.dst[i];
+  if (src < 0 || dst < 0 || src == dst) return;
+  const int fill = p.fill ? p.fill[i] : p.page_size;
+  if (src >= p.n_pages || dst >= p.n_pages || fill < 0 || fill > p.page_size) {
+    if (threadIdx.x == 0) atomicOr(p.err, DEV_ERR_PAGE);
+    return;
+  }
+  char *plane = p.arena + (size_t)blockIdx.y * p.plane_stride;
+  const char *from = plane + (size_t)src * p.page_stride;
+  char *to = plane + (size_t)dst * p.page_stride;
+  const unsigned per = (unsigned)((size_t)fill * p.row_bytes / sizeof(U));
+  for (int h = 0; h < p.heads; ++h) {
+    const U *f = reinterpret_cast<const U *>(from + (size_t)h * p.run_stride);
+    U *t = reinterpret_cast<U *>(to + (size_t)h * p.run_stride);
+#pragma unroll 4
+    for (unsigned u = threadIdx.x; u < per; u += blockDim.x) t[u] = f[u];
+  }
+}
+
+}  // namespace
+}  // namespace tllm
+
+using namespace tllm;
+
+extern "C" int tllm_paged_append(const tllm_paged_kv *kv, const tllm_paged_rows *in,
+                                 tllm_stream_t stream) {
+  TLLM_INJECT("launch");
+  AppendParams p;
+  int rc = paged_view(kv, &p.kv);
+  if (rc) return rc;
+  TLLM_CHECK_ARG(in, "rows is NULL");
+  const int D = kv->head_dim;
+  TLLM_CHECK_ARG(in->rows >= 0, "rows (%d) must be >= 0", in->rows);
+  TLLM_CHECK_ARG(in->src_dtype == TLLM_F32 || in->src_dtype == TLLM_BF16,
+                 "src_dtype must be F32 or BF16");
+  TLLM_CHECK_ARG(!in->q || in->n_head > 0, "n_head (%d) must be > 0", in->n_head);
+  if (in->rows == 0) return TLLM_OK;
+  TLLM_CHECK_ARG(in->k && in->v && in->row_pos, "NULL tensor pointer");
+  TLLM_CHECK_ARG(!in->q || in->q_out, "q without q_out");
+  TLLM_CHECK_ARG(in->row_seq || in->rows <= kv->n_seq,
+                 "%d rows for a table of %d sequences (pass row_seq)", in->rows, kv->n_seq);
+  TLLM_CHECK_ARG(!in->cos_t == !in->sin_t, "cos_t and sin_t go together");
+  if (in->cos_t)
+    TLLM_CHECK_ARG(in->rotary_dim >= 2 && in->rotary_dim % 2 == 0 && in->rotary_dim <= D &&
+                       in->n_pos > 0,
+                   "rotary_dim (%d) must be even, within head_dim (%d), and n_pos (%d) > 0",
+                   in->rotary_dim, D, in->n_pos);
+  TLLM_CHECK_ARG(!in->blocked || D % 16 == 0, "blocked heads need head_dim %% 16 == 0");
+  TLLM_CHECK_ARG(in->q_row_stride >= 0 && in->q_head_stride >= 0 && in->k_row_stride >= 0 &&
+                     in->k_head_stride >= 0 && in->v_row_stride >= 0 &&
+                     in->v_head_stride >= 0 && in->q_out_row_stride >= 0 &&
+                     in->q_out_head_stride >= 0,
+                 "negative stride");
+  TLLM_CHECK_ARG((const void *)in->q_out != in->q || !in->q ||
+                     (!in->blocked && !in->row_src && in->src_dtype == TLLM_F32 &&
+                      in->q_row_stride == in->q_out_row_stride &&
+                      in->q_head_stride == in->q_out_head_stride),
+                 "q in place needs fp32 rows in plain order with the same strides");
+  p.in = *in;
+  p.err = device_error_ptr();
+  TLLM_CHECK_ARG(p.err, "device error word unavailable");
+  cudaStream_t st = resolve(stream);
+  const bool t32 = kv->kv_dtype == TLLM_F32;
+  if (in->src_dtype == TLLM_F32)
+    return t32 ? launch_append<float, float>(p, st) : launch_append<float, uint16_t>(p, st);
+  return t32 ? launch_append<uint16_t, float>(p, st) : launch_append<uint16_t, uint16_t>(p, st);
+}
+
+extern "C" int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
+                              int n_pages, int heads, long run_stride, int page_size,
+                              int row_bytes, const int32_t *src, const int32_t *dst,
+                              const int32_t *fill, int n_copies, tllm_stream_t stream) {
+  TLLM_INJECT("launch");
+  TLLM_CHECK_ARG(planes >= 0 && planes <= 65535 && n_pages >= 0 && heads >= 0 &&
+                     page_size >= 1 && row_bytes >= 1 && n_copies >= 0,
+                 "invalid arena: %d planes, %d pages of %d runs of %d slots of %d bytes, %d copies",
+                 planes, n_pages, heads, page_size, row_bytes, n_copies);
+  TLLM_CHECK_ARG((long)page_size * row_bytes < (1L << 31), "a run of a page must be below 2 GiB");
+  TLLM_CHECK_ARG(plane_stride >= 0 && page_stride >= 0 && run_stride >= 0, "negative stride");
+  if (planes == 0 || heads == 0 || n_copies == 0) return TLLM_OK;
+  TLLM_CHECK_ARG(arena && src && dst, "NULL pointer");
+  CopyParams p;
+  p.arena = static_cast<char *>(arena);
+  p.src = src;
+  p.dst = dst;
+  p.fill = fill;
+  p.plane_stride = plane_stride;
+  p.page_stride = page_stride;
+  p.run_stride = run_stride;
+  p.n_pages = n_pages;
+  p.heads = heads;
+  p.page_size = page_size;
+  p.row_bytes = row_bytes;
+  p.err = device_error_ptr();
+  TLLM_CHECK_ARG(p.err, "device error word unavailable");
+  cudaStream_t st = resolve(stream);
+  const unsigned long bits = (unsigned long)(uintptr_t)arena | plane_stride | page_stride |
+                             run_stride | row_bytes;
+  const dim3 grid(n_copies, planes);
+  if (bits % 16 == 0)
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint4>, grid, dim3(256), 0, st, p));
+  else if (bits % 4 == 0)
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint32_t>, grid, dim3(256), 0, st, p));
+  else
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint8_t>, grid, dim3(256), 0, st, p));
+  return TLLM_OK;
+}

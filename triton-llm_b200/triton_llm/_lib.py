@@ -95,6 +95,17 @@ SIGNATURES: dict[str, list] = {
                       _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _vp],
     "tllm_gqa_rows_hint": [_vp, _l, _l, _vp, _vp, _i, _vp, _vp, _vp, _i, _l, _l, _l,
                            _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _l, _vp],
+    # paged cache
+    "tllm_paged_attention_workspace": [_i, _i, _i, _i, _psz, _psz],
+    "tllm_paged_attention": [_vp, _vp, _l, _l, _vp, _vp, _vp, _i, _l, _l, _l, _i, _i, _i,
+                             _l, _i, _i, _f, _vp, _sz, _vp, _sz, _vp],
+    "tllm_paged_append": [_vp, _vp, _vp],
+    "tllm_page_copy": [_vp, _l, _i, _l, _i, _i, _l, _i, _i, _vp, _vp, _vp, _i, _vp],
+    # beam search
+    "tllm_beam_workspace": [_i, _i, _i, _i, _psz],
+    "tllm_beam_select": [_vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz,
+                         _vp],
+    "tllm_beam_reorder": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp],
     # projections
     "tllm_linear_workspace": [_i, _i, _i, _psz, _psz],
     "tllm_linear_plan": [_i, _i, _i, _i, _pi],
@@ -147,6 +158,28 @@ class NormFold(ctypes.Structure):
     _fields_ = [("next_norm_w", _vp), ("fx", _vp), ("fx_dtype", _i),
                 ("fx_plane_rows", _i), ("ss_out", _vp), ("ss_in", _vp),
                 ("ss_parts", _i), ("ss_cols", _i), ("eps", _f), ("ss_ld", _i)]
+
+
+class PagedKVStruct(ctypes.Structure):
+    """tllm_paged_kv (include/tllm.h): one layer's pages and page tables."""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("kv_dtype", _i), ("n_pages", _i),
+                ("page_size", _i), ("n_kv_head", _i), ("head_dim", _i), ("n_seq", _i),
+                ("table_cols", _i), ("reserved", _i), ("page_stride", _l),
+                ("head_stride", _l), ("slot_stride", _l), ("table_stride", _l),
+                ("table", _vp)]
+
+
+class PagedRowsStruct(ctypes.Structure):
+    """tllm_paged_rows (include/tllm.h): the new tokens of an append."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("row_src", _vp),
+                ("row_seq", _vp), ("row_pos", _vp), ("lens_out", _vp), ("cos_t", _vp),
+                ("sin_t", _vp), ("q_row_stride", _l), ("q_head_stride", _l),
+                ("k_row_stride", _l), ("k_head_stride", _l), ("v_row_stride", _l),
+                ("v_head_stride", _l), ("q_out_row_stride", _l), ("q_out_head_stride", _l),
+                ("src_dtype", _i), ("rows", _i), ("n_head", _i), ("rotary_dim", _i),
+                ("n_pos", _i), ("interleaved", _i), ("blocked", _i), ("reserved", _i)]
+
+
 EL_SWIGLU, EL_ADD, EL_GELU = 0, 1, 2
 
 _lib = None

@@ -9,11 +9,14 @@ from .add import add
 from .attention import attention
 from .attention_gqa import attention_gqa, gqa_decode, DecodeWorkspace
 from .attention_prefill import gqa_rows, gqa_prefill, prefill_blocks
+from .beam import BeamWorkspace, beam_reorder, beam_select
 from .embedding import embedding, embedding_dev
 from .gelu import gelu
 from .gemm import gemm
 from .layernorm import layer_norm, layer_norm_dev
 from .linear import Linear, LinearWorkspace, linear
+from .paged import (PagedKV, PagedWorkspace, page_copy, paged_append, paged_attention,
+                    paged_write)
 from .rms_norm import rms_norm
 from .rope import precompute_cos_sin, precompute_cos_sin_device, apply_rope
 from .softmax import softmax
@@ -44,4 +47,14 @@ __all__ = [
     "Linear",
     "LinearWorkspace",
     "linear",
+    # paged cache and beam search
+    "PagedKV",
+    "PagedWorkspace",
+    "paged_attention",
+    "paged_append",
+    "paged_write",
+    "page_copy",
+    "BeamWorkspace",
+    "beam_select",
+    "beam_reorder",
 ]
