@@ -18,6 +18,11 @@
 #include "paged.cuh"
 
 namespace tllm {
+
+// tma.cu
+int make_map(CUtensorMap *m, const void *base, int dtype, int rank, const long *dims,
+             const long *strides_bytes, const int *box, bool swizzle128);
+
 namespace {
 
 constexpr int kMaxSplits = 256;
@@ -47,17 +52,29 @@ struct AttnParams {
 struct RowSpan {
   int seq, len;
   int s, a;              // keys [0, s) and [a, len) are visible
-  int n;                 // s + len - a
-  int n_splits, begin, end;
+  int n_splits, begin, end;   // on the axis of the kernel's keys
 };
 
-__device__ __forceinline__ RowSpan row_span(const AttnParams &p, int row, int split) {
+// Splits of the planned size over n keys; longer ones where the host's bound
+// on the length was too small.
+__device__ __forceinline__ void split_row(const AttnParams &p, RowSpan &x, int split, int n) {
+  int chunk = p.chunk;
+  if ((long)chunk * p.max_splits < n) {
+    chunk = (n + p.max_splits - 1) / p.max_splits;
+    chunk = (chunk + p.tile - 1) / p.tile * p.tile;
+  }
+  x.n_splits = n > 0 ? (n + chunk - 1) / chunk : 1;
+  x.begin = split * chunk;
+  x.end = min(x.begin + chunk, n);
+}
+
+__device__ __forceinline__ RowSpan row_keys(const AttnParams &p, int row, int split) {
   RowSpan x;
   x.seq = p.row_seq ? p.row_seq[row] : row;
   x.len = p.row_len[row];
-  const long cap = (long)p.kv.table_cols * p.kv.page_size;
+  const int cap = p.kv.table_cols * p.kv.page_size;
   if (x.len > cap) {
-    x.len = (int)cap;
+    x.len = cap;
     if (threadIdx.x == 0 && split == 0) atomicOr(p.err, DEV_ERR_LEN_CLAMPED);
   }
   if (x.seq < 0 || x.seq >= p.kv.n_seq) {
@@ -67,17 +84,6 @@ __device__ __forceinline__ RowSpan row_span(const AttnParams &p, int row, int sp
   if (x.len < 0) x.len = 0;
   x.s = p.window > 0 ? min(p.sinks, x.len) : 0;
   x.a = p.window > 0 ? max(x.len - p.window, x.s) : 0;
-  x.n = x.s + x.len - x.a;
-  // splits of the planned size; longer ones where the host's bound on the
-  // length was too small
-  int chunk = p.chunk;
-  if ((long)chunk * p.max_splits < x.n) {
-    chunk = (x.n + p.max_splits - 1) / p.max_splits;
-    chunk = (chunk + p.tile - 1) / p.tile * p.tile;
-  }
-  x.n_splits = x.n > 0 ? (x.n + chunk - 1) / chunk : 1;
-  x.begin = split * chunk;
-  x.end = min(x.begin + chunk, x.n);
   return x;
 }
 
@@ -209,7 +215,8 @@ __global__ void __launch_bounds__(kGenWarps * 32)
   extern __shared__ __align__(16) float smem_f[];
   __shared__ int s_flag;
   const int row = blockIdx.z, y = blockIdx.y, split = blockIdx.x;
-  const RowSpan x = row_span(p, row, split);
+  RowSpan x = row_keys(p, row, split);
+  split_row(p, x, split, x.s + x.len - x.a);   // the visible keys, in order
   if (split >= x.n_splits) return;
   const int kvh = y / p.n_gsub;
   const int gofs = (y - kvh * p.n_gsub) * p.g_tile;
@@ -374,8 +381,419 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 }
 
 // --------------------------------------------------------------------------
+// bf16 pages of 8, 16, 32, .. slots, head_dim 64 or 128: TMA and tensor cores.
+//
+// A producer warp streams KT-key tiles of K and V (128-byte swizzle) from the
+// pages into a ring of kStages shared-memory stages; each of NCW = KT / 16
+// consumer warps owns 16 keys of every tile and computes with mma.sync
+// m16n8k16, keys as the 16 rows and query heads as the 8 columns:
+//   S^T (16 keys x 8 heads) = K_w Q^T,   O^T (D x 8 heads) += V_w^T P^T.
+// q and p are fp32 and go in as three bf16 terms each (8 + 8 + 8 bits, exact),
+// so the products are exact and sums are fp32, as in the plain formula: two
+// terms leave 2.5e-6 of each value, which the result then shows. A tile's
+// O^T is added to the running one by ordinary fp32 additions: the tensor
+// core's own additions round towards zero, and a chain of them over a long
+// row loses 1e-5 (measured over 20011 keys). The work is bound by HBM: at head_dim 128 a tile is 32 KB, 1400 cycles of an SM's share
+// of 6.4 TB/s.
+//
+// The tiles run over the row's pages: with a window, the pages of the first
+// tokens and then those from the window's first page on (all pages where the
+// two meet); keys between are masked.
+// --------------------------------------------------------------------------
+constexpr int kStages = 3;
+
+template <int D>
+struct Tile {
+  static constexpr int KT = D == 128 ? 64 : 128;   // keys
+  static constexpr int SUB = D / 64;               // 128-byte columns
+  static constexpr int SUB_BYTES = KT * 128;
+  static constexpr int BYTES = SUB * SUB_BYTES;    // K or V of a tile: 16 KB
+  static constexpr int NCW = KT / 16;
+  static constexpr int THREADS = (NCW + 1) * 32;
+  static constexpr size_t SMEM = 2 * (size_t)kStages * BYTES + 2 * kStages * 8 + kStages * 4;
+};
+
+// 4-D tiled TMA load, completion on bar.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint64_t *bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(c0),
+      "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Transpose of the 8 x 8 bf16 matrix in the accumulator fragment layout.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// (x0, x1) as three bf16 pairs of their sign whose sum is x (cut off, not
+// rounded, so 8 + 8 + 8 bits hold all 24). The lower terms of an x != 0 are
+// kept from zero by 2e-38, far below any product that counts: an infinite k
+// or v then gives x * inf, and not the NaN of 0 * inf.
+__device__ __forceinline__ void split3(float x0, float x1, uint32_t (&t)[3]) {
+  const float e0 = copysignf(x0 == 0.f ? 0.f : 2e-38f, x0);
+  const float e1 = copysignf(x1 == 0.f ? 0.f : 2e-38f, x1);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    t[i] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    x0 = (x0 - bf16lo(t[i])) + e0;
+    x1 = (x1 - bf16hi(t[i])) + e1;
+  }
+}
+// The same for weights, which are not negative (one that is 0 where V is
+// infinite gives infinity instead of NaN).
+__device__ __forceinline__ void split3_weight(float x0, float x1, uint32_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    t[i] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    x0 = (x0 - bf16lo(t[i])) + 2e-38f;
+    x1 = (x1 - bf16hi(t[i])) + 2e-38f;
+  }
+}
+
+// The pages of a row as one axis: sink pages, then the window's.
+struct PageSpan {
+  int sink_pages, first;   // pages [0, sink_pages) and [first, ..)
+  __device__ __forceinline__ int column(int vp) const {
+    return vp < sink_pages ? vp : vp - sink_pages + first;
+  }
+};
+__device__ __forceinline__ PageSpan page_span(const AttnParams &p, RowSpan &x, int split) {
+  const int P = p.kv.page_size;
+  PageSpan g;
+  g.first = p.kv.column(x.a);
+  g.sink_pages = p.kv.column(x.s + P - 1);
+  if (g.sink_pages >= g.first) g.sink_pages = g.first = 0;
+  split_row(p, x, split, g.sink_pages * P + x.len - g.first * P);
+  return g;
+}
+
+template <int D, int QB>
+__global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
+    paged_mma_kernel(const AttnParams p, const __grid_constant__ CUtensorMap mk,
+                     const __grid_constant__ CUtensorMap mv, const int slots_first) {
+  griddep_launch();
+  using T = Tile<D>;
+  constexpr int KT = T::KT, NCW = T::NCW;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + 2 * kStages * T::BYTES);
+  uint64_t *empty = full + kStages;
+  uint32_t *s_bad = reinterpret_cast<uint32_t *>(empty + kStages);   // bad pages of a stage
+  __shared__ int s_flag, s_issued;
+  const int row = blockIdx.z, y = blockIdx.y, split = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023) {
+    griddep_wait();
+    if (tid == 0) atomicOr(p.err, DEV_ERR_SMEM_ALIGN);
+    return;
+  }
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], NCW);
+    }
+    fence_mbar_init();
+    s_flag = 0;
+    s_issued = 0;
+  }
+  __syncthreads();
+  griddep_wait();
+  RowSpan x = row_keys(p, row, split);
+  const PageSpan g = page_span(p, x, split);
+  if (split >= x.n_splits) return;
+  const int kvh = y / p.n_gsub, gofs = (y - kvh * p.n_gsub) * p.g_tile;
+  const int G = min(p.g_tile, p.group - gofs), head0 = kvh * p.group + gofs;
+  const int P = p.kv.page_size;
+  const int ntiles = x.end > x.begin ? (x.end - x.begin + KT - 1) / KT : 0;
+  bool failed = false;
+
+  if (warp == NCW) {
+    // ---- producer: lane (kv, sub, page of the tile) issues its loads
+    const int box = min(P, KT), pt = KT / box;          // slots of a load, pages of a tile
+    const int j = lane % pt, sub = lane / pt % T::SUB, is_v = lane / pt / T::SUB;
+    const bool mine = is_v < 2;
+    const int *table = p.kv.table + (size_t)x.seq * p.kv.table_stride;
+    // page of tile t for this lane: -1 past the end, -2 out of range
+    auto entry = [&](int t) {
+      const int u = x.begin + t * KT + j * box;
+      if (t >= ntiles || u >= x.end) return -1;
+      const int page = table[g.column(p.kv.column(u))];
+      return page >= 0 && page < p.kv.n_pages ? page : -2;
+    };
+    int next0 = entry(0), next1 = entry(1);
+    for (int t = 0; t < ntiles; ++t) {
+      const int s = t % kStages, page = next0;
+      next0 = next1;
+      next1 = entry(t + 2);
+      const uint32_t good = __ballot_sync(~0u, mine && page >= 0);
+      const uint32_t bad = __ballot_sync(~0u, lane < pt && page == -2);
+      if (t >= kStages && !mbar_wait_bounded(&empty[s], (t / kStages - 1) & 1)) failed = true;
+      if (__any_sync(~0u, failed)) {
+        failed = true;
+        break;
+      }
+      if (lane == 0) {
+        s_bad[s] = bad;
+        s_issued = t + 1;
+        mbar_expect_tx(&full[s], __popc(good) * box * 128);
+        if (bad) atomicOr(p.err, DEV_ERR_PAGE);
+      }
+      __syncwarp();
+      if (mine && page >= 0) {
+        const int u = x.begin + t * KT + j * box;
+        const int slot = u - p.kv.column(u) * P;
+        const uint32_t dst = smem_u32(smem) + (is_v ? kStages * T::BYTES : 0) + s * T::BYTES +
+                             sub * T::SUB_BYTES + j * box * 128;
+        tma_load_4d(dst, is_v ? &mv : &mk, &full[s], sub * 64, slots_first ? kvh : slot,
+                    slots_first ? slot : kvh, page);
+      }
+    }
+  }
+
+  // ---- consumers. Fragments: rows (keys, or dims of O^T) r0 and r0 + 8,
+  // columns (heads) cq and cq + 1 of every block of 8.
+  const int r0 = lane >> 2, cq = (lane & 3) * 2;
+  float o[QB][D / 16][4], m_r[QB][2], l_r[QB][2];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    m_r[qb][0] = m_r[qb][1] = -INFINITY;
+    l_r[qb][0] = l_r[qb][1] = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[qb][mb][e] = 0.f;
+  }
+  if (warp < NCW) {
+    uint32_t qf[QB][D / 16][2][3];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          float2 v = make_float2(0.f, 0.f);
+          if (qb * 8 + r0 < G)
+            v = *reinterpret_cast<const float2 *>(p.q + (size_t)row * p.q_sr +
+                                                  (size_t)(head0 + qb * 8 + r0) * p.q_sh +
+                                                  kk * 16 + cq + 8 * f);
+          split3(v.x * p.qscale, v.y * p.qscale, qf[qb][kk][f]);
+        }
+    // ldmatrix rows: K as the A operand, V^T by the transposing load
+    const int a_key = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), a_dim = (lane >> 4) * 8;
+    const int t_key = warp * 16 + (lane >> 4) * 8 + (lane & 7), t_dim = ((lane >> 3) & 1) * 8;
+    const int sink_keys = g.sink_pages * P;
+
+    for (int t = 0; t < ntiles; ++t) {
+      const int s = t % kStages;
+      if (!__all_sync(~0u, mbar_wait_bounded(&full[s], (t / kStages) & 1))) {
+        failed = true;
+        break;
+      }
+      const uint32_t kt = smem_u32(smem) + s * T::BYTES;
+      const uint32_t vt = kt + kStages * T::BYTES;
+      const int u0 = x.begin + t * KT + warp * 16;   // this warp's first key
+      const uint32_t bad = s_bad[s];
+      // position of key u0 + i, and whether the row sees it
+      auto sees = [&](int i) {
+        const int u = u0 + i;
+        if (u >= x.end || (bad && (bad >> ((warp * 16 + i) / min(P, KT)) & 1))) return false;
+        const int pos = u < sink_keys ? u : u - sink_keys + g.first * P;
+        return pos < x.s || pos >= x.a;
+      };
+      const int pos0 = u0 < sink_keys ? 0 : u0 - sink_keys + g.first * P;
+      const bool whole = !bad && u0 + 16 <= x.end && pos0 >= x.a;
+
+      float sc[QB][3][4];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[qb][i][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const int dim = kk * 16 + a_dim;
+        uint32_t ka[4];
+        ldsm_x4(kt + (dim >> 6) * T::SUB_BYTES + a_key * 128 +
+                    ((((dim & 63) >> 3) ^ (a_key & 7)) << 4),
+                ka[0], ka[1], ka[2], ka[3]);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+          for (int i = 0; i < 3; ++i)   // (three independent sums)
+            mma_bf16(sc[qb][i], ka, qf[qb][kk][0][i], qf[qb][kk][1][i]);
+      }
+      uint32_t pb[QB][2][3];
+      bool see0 = true, see1 = true;
+      if (!whole) {
+        see0 = sees(r0);
+        see1 = sees(r0 + 8);
+      }
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = sc[qb][0][e] + (sc[qb][1][e] + sc[qb][2][e]);
+          if (!(e < 2 ? see0 : see1)) w[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(w[c], w[c + 2]);
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+          const float mn = fmaxf(m_r[qb][c], mx);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          if (mn != m_r[qb][c]) {
+            const float alpha = fast_exp2(m_r[qb][c] - base);   // 0 while m is -inf
+            l_r[qb][c] *= alpha;
+#pragma unroll
+            for (int mb = 0; mb < D / 16; ++mb) {
+              o[qb][mb][c] *= alpha;
+              o[qb][mb][c + 2] *= alpha;
+            }
+            m_r[qb][c] = mn;
+          }
+          w[c] = fast_exp2(w[c] - base);
+          w[c + 2] = fast_exp2(w[c + 2] - base);
+          l_r[qb][c] += w[c] + w[c + 2];
+        }
+        uint32_t t0[3], t1[3];
+        split3_weight(w[0], w[1], t0);   // key r0
+        split3_weight(w[2], w[3], t1);   // key r0 + 8
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          pb[qb][0][i] = transpose8(t0[i]);
+          pb[qb][1][i] = transpose8(t1[i]);
+        }
+      }
+      if (!whole) {
+        // V of keys that the row does not see may be anything, NaN too, and
+        // 0 * NaN is no 0: clear it
+        for (int i = lane; i < 16 * T::SUB * 8; i += 32) {
+          const int key = i / (T::SUB * 8), c = i % (T::SUB * 8);
+          if (!sees(key))
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             vt + (c >> 3) * T::SUB_BYTES + (warp * 16 + key) * 128 +
+                             ((c & 7) << 4)),
+                         "r"(0)
+                         : "memory");
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) {
+        const int dim = mb * 16 + t_dim;
+        uint32_t va[4];
+        ldsm_x4_t(vt + (dim >> 6) * T::SUB_BYTES + t_key * 128 +
+                      ((((dim & 63) >> 3) ^ (t_key & 7)) << 4),
+                  va[0], va[1], va[2], va[3]);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 2; i >= 0; --i) mma_bf16(d, va, pb[qb][0][i], pb[qb][1][i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[qb][mb][e] += d[e];
+        }
+      }
+      if (!whole) fence_proxy_async();   // generic writes before the next TMA
+      __syncwarp();
+      if (lane == 0) arrive(&empty[s]);
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l_r[qb][c] += __shfl_xor_sync(~0u, l_r[qb][c], d);
+  }
+  if (failed) {
+    atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+    s_flag = 1;
+  }
+  __syncthreads();
+  if (s_flag) {
+    // let the copies in flight land (bounded) before the CTA exits
+    if (tid == 0)
+      for (int t = max(0, s_issued - kStages); t < s_issued; ++t)
+        mbar_wait_bounded(&full[t % kStages], (t / kStages) & 1, 1u << 12);
+    return;
+  }
+  float *w_acc = reinterpret_cast<float *>(smem);
+  float *w_m = w_acc + NCW * G * D, *w_l = w_m + NCW * G;
+  if (warp < NCW) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int h = qb * 8 + cq + c;
+        if (h >= G) continue;
+#pragma unroll
+        for (int mb = 0; mb < D / 16; ++mb) {
+          w_acc[(warp * G + h) * D + mb * 16 + r0] = o[qb][mb][c];
+          w_acc[(warp * G + h) * D + mb * 16 + r0 + 8] = o[qb][mb][c + 2];
+        }
+        if (r0 == 0) {
+          w_m[warp * G + h] = m_r[qb][c];
+          w_l[warp * G + h] = l_r[qb][c];
+        }
+      }
+  }
+  __syncthreads();
+  finish_split<NCW, T::THREADS>(p, x, row, y, head0, G, D, split, w_acc, &s_flag);
+}
+
+// --------------------------------------------------------------------------
 // Host side
 // --------------------------------------------------------------------------
+template <int D, int QB>
+int launch_mma(const AttnParams &p, const CUtensorMap &mk, const CUtensorMap &mv,
+               bool slots_first, dim3 grid, cudaStream_t st) {
+  auto kern = paged_mma_kernel<D, QB>;
+  static bool configured[64] = {};
+  int dev = 0;
+  TLLM_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    TLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)Tile<D>::SMEM));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  TLLM_CUDA(launch_pdl(kern, grid, dim3(Tile<D>::THREADS), Tile<D>::SMEM, st, p, mk, mv,
+                       (int)slots_first));
+  return TLLM_OK;
+}
+
+// Tensor map of K or V pages with boxes of 64 values x `rows` slots of one
+// head and page; the axes are in the order of their strides.
+int page_map(CUtensorMap *m, const void *base, const tllm_paged_kv *kv, int rows,
+             bool slots_first) {
+  const long slot = kv->slot_stride * 2;
+  const long head = kv->n_kv_head > 1 ? kv->head_stride * 2 : slot * kv->page_size;
+  const long page = kv->n_pages > 1 ? kv->page_stride * 2
+                                    : (slot > head ? slot : head) * kv->page_size;
+  const long dims[4] = {kv->head_dim, slots_first ? kv->n_kv_head : kv->page_size,
+                        slots_first ? kv->page_size : kv->n_kv_head, kv->n_pages};
+  const long strides[3] = {slots_first ? head : slot, slots_first ? slot : head, page};
+  const int box[4] = {64, slots_first ? 1 : rows, slots_first ? rows : 1, 1};
+  return make_map(m, base, TLLM_BF16, 4, dims, strides, box, true);
+}
+
+// The tensor-core kernel takes bf16 pages of a power of two >= 8 slots (a TMA
+// box of 8 rows is one swizzle atom, and pages divide tiles or tiles pages),
+// head_dim 64 or 128, and distinct heads and pages (strides > 0).
+bool mma_takes(const tllm_paged_kv *kv, const PagedView &w) {
+  return kv->kv_dtype == TLLM_BF16 && (kv->head_dim == 64 || kv->head_dim == 128) &&
+         w.page_shift >= 3 && kv->n_pages > 0 && (kv->n_kv_head == 1 || kv->head_stride > 0) &&
+         (kv->n_pages == 1 || kv->page_stride > 0);
+}
+
 template <typename T, int G, int NV>
 int launch_rows(const AttnParams &p, int lpr, dim3 grid, cudaStream_t st) {
   const int D = p.kv.head_dim;
@@ -491,7 +909,7 @@ extern "C" int tllm_paged_attention(
   AttnParams p;
   int rc = paged_view(kv, &p.kv);
   if (rc) return rc;
-  const int D = kv->head_dim, n_kv = kv->n_kv_head;
+  const int D = kv->head_dim, n_kv = kv->n_kv_head, P = kv->page_size;
   TLLM_CHECK_ARG(rows >= 0 && n_head > 0, "invalid rows %d / n_head %d", rows, n_head);
   TLLM_CHECK_ARG(n_head % n_kv == 0, "n_head (%d) must be divisible by n_kv_head (%d)",
                  n_head, n_kv);
@@ -520,17 +938,19 @@ extern "C" int tllm_paged_attention(
   TLLM_CHECK_ARG(((uintptr_t)out & (out_dtype == TLLM_F32 ? 3 : 1)) == 0, "out misaligned");
 
   const int group = n_head / n_kv;
+  const bool mma = mma_takes(kv, p.kv);
   const int units = D / vec;
   int lpr = 1;
   while (lpr < units && lpr < 32) lpr <<= 1;
   int nv = (units + lpr - 1) / lpr;
   if (nv == 3) nv = 4;
-  const int g_max = nv * vec <= 8 ? 8 : 4;
+  const int g_max = mma ? 16 : nv * vec <= 8 ? 8 : 4;
   const int n_gsub = (group + g_max - 1) / g_max;
   const int g_even = (group + n_gsub - 1) / n_gsub;
-  const int g_tile = g_even <= 2 ? g_even : g_even <= 4 ? 4 : 8;
+  const int g_tile = mma ? g_even : g_even <= 2 ? g_even : g_even <= 4 ? 4 : 8;
   const int n_y = n_kv * n_gsub;
-  const int tile = kGenWarps * (nv == 1 ? 4 : 2) * (32 / lpr);
+  const int tile = mma ? (D == 128 ? Tile<128>::KT : Tile<64>::KT)
+                       : kGenWarps * (nv == 1 ? 4 : 2) * (32 / lpr);
   TLLM_CHECK_ARG(n_y <= 65535 && rows <= 65535, "grid too large: %d rows, %d head groups",
                  rows, n_y);
 
@@ -542,7 +962,12 @@ extern "C" int tllm_paged_attention(
     if (most > seen) most = seen;
     if (keys > seen * rows) keys = seen * rows;
   }
-  int chunk = plan_chunk(tile, rows, n_y, keys, most, 4L * sm_count());
+  if (mma && window > 0) {
+    // whole pages, and tiles that start before the window
+    most += 2 * (P > tile ? P : tile);
+    if (most > cap) most = cap;
+  }
+  int chunk = plan_chunk(tile, rows, n_y, keys, most, (mma ? 2L : 4L) * sm_count());
   long splits = most > 0 ? (most + chunk - 1) / chunk : 1;
   const size_t one = (size_t)rows * n_y * g_tile * (D + 2) * sizeof(float);
   if (splits > 1 && one * splits > partial_bytes) {
@@ -589,6 +1014,18 @@ extern "C" int tllm_paged_attention(
   p.qscale = sm_scale * kLog2e;
   const dim3 grid((unsigned)splits, n_y, rows);
   cudaStream_t st = resolve(stream);
+  if (mma) {
+    const bool slots_first = n_kv > 1 && kv->head_stride < kv->slot_stride;
+    CUtensorMap mk, mv;
+    rc = page_map(&mk, kv->k_pages, kv, P < tile ? P : tile, slots_first);
+    if (!rc) rc = page_map(&mv, kv->v_pages, kv, P < tile ? P : tile, slots_first);
+    if (rc) return rc;
+    if (D == 64)
+      return g_tile <= 8 ? launch_mma<64, 1>(p, mk, mv, slots_first, grid, st)
+                         : launch_mma<64, 2>(p, mk, mv, slots_first, grid, st);
+    return g_tile <= 8 ? launch_mma<128, 1>(p, mk, mv, slots_first, grid, st)
+                       : launch_mma<128, 2>(p, mk, mv, slots_first, grid, st);
+  }
   return kv->kv_dtype == TLLM_BF16
              ? launch_rows_t<__nv_bfloat16>(p, lpr, nv, grid, st)
              : launch_rows_t<float>(p, lpr, nv, grid, st);
