@@ -42,7 +42,7 @@ struct AttnParams {
   float *part_ml;        // (rows, n_y, max_splits, G, 2)
   int *counters;         // (rows, n_y)
   int *err;
-  int group, n_gsub, g_tile, n_y;   // heads per KV head, sub-groups, heads per CTA
+  int rows, group, n_gsub, g_tile, n_y;   // heads per KV head, sub-groups, heads per CTA
   int chunk, max_splits, tile;
   int window, sinks;
   float qscale;          // sm_scale * log2(e)
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 // bf16 pages of 8, 16, 32, .. slots, head_dim 64 or 128: TMA and tensor cores.
 //
 // A producer warp streams KT-key tiles of K and V (128-byte swizzle) from the
-// pages into a ring of kStages shared-memory stages; each of NCW = KT / 16
-// consumer warps owns 16 keys of every tile and computes with mma.sync
+// pages into a ring of kStages shared-memory stages; each of four consumer
+// warps owns KB blocks of 16 keys of every tile and computes with mma.sync
 // m16n8k16, keys as the 16 rows and query heads as the 8 columns:
 //   S^T (16 keys x 8 heads) = K_w Q^T,   O^T (D x 8 heads) += V_w^T P^T.
 // q and p are fp32 and go in as three bf16 terms each (8 + 8 + 8 bits, exact),
@@ -401,6 +401,10 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 // two meet); keys between are masked.
 // --------------------------------------------------------------------------
 constexpr int kStages = 3;
+constexpr int kRowBlock = 512;   // rows that share one axis (and one grid row)
+constexpr int kMaxPerSm = 2;     // CTAs that the shared memory lets an SM hold
+constexpr int kMinTiles = 2;     // least tiles of a share
+constexpr int kJoinTiles = 4;    // tiles that a CTA reads in the time of a join
 
 template <int D>
 struct Tile {
@@ -408,9 +412,10 @@ struct Tile {
   static constexpr int SUB = D / 64;               // 128-byte columns
   static constexpr int SUB_BYTES = KT * 128;
   static constexpr int BYTES = SUB * SUB_BYTES;    // K or V of a tile: 16 KB
-  static constexpr int NCW = KT / 16;
+  static constexpr int NCW = 4;                    // consumer warps
+  static constexpr int KB = KT / NCW / 16;         // 16-key blocks of a warp
   static constexpr int THREADS = (NCW + 1) * 32;
-  static constexpr size_t SMEM = 2 * (size_t)kStages * BYTES + 2 * kStages * 8 + kStages * 4;
+  static constexpr size_t SMEM = 2 * (size_t)kStages * BYTES + 2 * kStages * 8;
 };
 
 // 4-D tiled TMA load, completion on bar.
@@ -456,36 +461,129 @@ __device__ __forceinline__ void split3_weight(float x0, float x1, uint32_t (&t)[
   }
 }
 
-// The pages of a row as one axis: sink pages, then the window's.
+// The pages of a row as one axis: sink pages, then the window's. n counts its
+// slots up to the row's end.
 struct PageSpan {
   int sink_pages, first;   // pages [0, sink_pages) and [first, ..)
+  int n;
   __device__ __forceinline__ int column(int vp) const {
     return vp < sink_pages ? vp : vp - sink_pages + first;
   }
 };
-__device__ __forceinline__ PageSpan page_span(const AttnParams &p, RowSpan &x, int split) {
+__device__ __forceinline__ PageSpan page_span(const AttnParams &p, int len, int *s, int *a) {
   const int P = p.kv.page_size;
+  *s = p.window > 0 ? min(p.sinks, len) : 0;
+  *a = p.window > 0 ? max(len - p.window, *s) : 0;
   PageSpan g;
-  g.first = p.kv.column(x.a);
-  g.sink_pages = p.kv.column(x.s + P - 1);
+  g.first = p.kv.column(*a);
+  g.sink_pages = p.kv.column(*s + P - 1);
   if (g.sink_pages >= g.first) g.sink_pages = g.first = 0;
-  split_row(p, x, split, g.sink_pages * P + x.len - g.first * P);
+  g.n = g.sink_pages * P + len - g.first * P;
   return g;
+}
+
+// The tiles of all (row, head group) pairs, in that order, as one axis cut
+// into equal shares, one for each CTA. A pair is a segment of the axis; a
+// share holds the end of one, some whole ones and the start of another.
+struct Segment {
+  int row, y;      // row of this block of rows, head group
+  int nt, t0, t1;  // tiles of the pair, and those of this share
+};
+
+__device__ __forceinline__ void bar_consumers(int threads) {
+  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+}
+
+// The n parts of one pair joined by NCW consumer warps: part 0 lies in slot
+// base + 1 of the partials, part i > 0 in slot base + 2 i. (Not inlined: its
+// registers would take away from those of the tile loop.)
+template <int D, int NCW>
+__device__ __noinline__ void join_parts(const AttnParams &p, size_t base, int n, int G,
+                                        float *sw, size_t out_row) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __threadfence();
+  // Loads are issued in batches of kJoin whose count does not depend on
+  // n, the first of them beside those of the statistics: a join of up to
+  // kJoin parts waits for one round trip to L2.
+  constexpr int kJoin = 8;
+  const float4 *acc4 = reinterpret_cast<const float4 *>(p.part_acc);
+  const size_t step = (size_t)p.g_tile * (D / 4);
+  auto load = [&](float4 (&v)[kJoin], int k0, int i) {
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      const int c = min(k0 + k, n - 1);
+      v[k] = __ldcg(acc4 + (base + 2 * c + (c == 0)) * step + i);
+    }
+  };
+  float4 v[kJoin];
+  if (tid < G * (D / 4)) load(v, 0, tid);
+  // sw: [G][n] weights of the parts
+  for (int h = warp; h < G; h += NCW) {
+    auto stats = [&](int i) {
+      return i < n ? __ldcg(reinterpret_cast<const float2 *>(p.part_ml) +
+                            (base + 2 * i + (i == 0)) * p.g_tile + h)
+                   : make_float2(-INFINITY, 0.f);
+    };
+    const float2 ml0 = stats(lane), ml1 = stats(lane + 32);
+    float mx = fmaxf(ml0.x, ml1.x), den = 0.f;
+    for (int i = lane + 64; i < n; i += 32) mx = fmaxf(mx, stats(i).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
+    auto weigh = [&](int i, float2 ml) {
+      if (i >= n) return;
+      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
+      sw[h * n + i] = f;
+      den = fmaf(ml.y, f, den);
+    };
+    weigh(lane, ml0);
+    weigh(lane + 32, ml1);
+    for (int i = lane + 64; i < n; i += 32) weigh(i, stats(i));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) den += __shfl_xor_sync(~0u, den, d);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) sw[h * n + i] *= inv;
+  }
+  bar_consumers(NCW * 32);
+  for (int i = tid; i < G * (D / 4); i += NCW * 32) {
+    const int h = i / (D / 4);
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < n; k0 += kJoin) {
+      if (i != tid || k0 > 0) load(v, k0, i);
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k) {
+        if (k0 + k >= n) continue;
+        const float f = sw[h * n + k0 + k];
+        r.x = fmaf(f, v[k].x, r.x);
+        r.y = fmaf(f, v[k].y, r.y);
+        r.z = fmaf(f, v[k].z, r.z);
+        r.w = fmaf(f, v[k].w, r.w);
+      }
+    }
+    const size_t at = out_row + (size_t)h * p.o_sh + (i - h * (D / 4)) * 4;
+    store_out(p, at, r.x);
+    store_out(p, at + 1, r.y);
+    store_out(p, at + 2, r.z);
+    store_out(p, at + 3, r.w);
+  }
 }
 
 template <int D, int QB>
 __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
-    paged_mma_kernel(const AttnParams p, const __grid_constant__ CUtensorMap mk,
+    paged_mma_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const int slots_first) {
   griddep_launch();
   using T = Tile<D>;
-  constexpr int KT = T::KT, NCW = T::NCW;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int KT = T::KT, NCW = T::NCW, KB = T::KB;
+  extern __shared__ __align__(1024) uint8_t smem[];   // stages of (K, V)
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + 2 * kStages * T::BYTES);
   uint64_t *empty = full + kStages;
-  uint32_t *s_bad = reinterpret_cast<uint32_t *>(empty + kStages);   // bad pages of a stage
-  __shared__ int s_flag, s_issued;
-  const int row = blockIdx.z, y = blockIdx.y, split = blockIdx.x;
+  __shared__ uint32_t s_bad[kStages];                 // bad pages of a stage's tile
+  __shared__ int s_cum[kRowBlock + 1], s_len[kRowBlock];
+  __shared__ int s_warp[2][NCW + 1], s_last;
+  __shared__ volatile int s_fail;
+  __shared__ float s_m[NCW][16], s_l[NCW][16];
+  const int row0 = blockIdx.y * kRowBlock, nrows = min(kRowBlock, p.rows - row0);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(smem) & 1023) {
     griddep_wait();
@@ -498,82 +596,202 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
       mbar_init(&empty[s], NCW);
     }
     fence_mbar_init();
-    s_flag = 0;
-    s_issued = 0;
+    s_fail = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
+  griddep_wait();
+
+  // ---- tiles of every row, summed up (a row without keys has one, empty)
+  const int per = (nrows + T::THREADS - 1) / T::THREADS;
+  int sum = 0, most = 0;
+  for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
+    int len = p.row_len[row0 + i];
+    const int cap = p.kv.table_cols * p.kv.page_size;
+    if (len > cap) {
+      len = cap;
+      if (blockIdx.x == 0) atomicOr(p.err, DEV_ERR_LEN_CLAMPED);
+    }
+    const int seq = p.row_seq ? p.row_seq[row0 + i] : row0 + i;
+    if (seq < 0 || seq >= p.kv.n_seq) {
+      len = 0;
+      if (blockIdx.x == 0) atomicOr(p.err, DEV_ERR_PAGE);
+    }
+    if (len < 0) len = 0;
+    int xs, xa;
+    const int nt = max(1, (page_span(p, len, &xs, &xa).n + KT - 1) / KT);
+    s_len[i] = len;
+    s_cum[i] = nt;
+    sum += nt;
+    most = max(most, nt);
+  }
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, scan, o);
+    if (lane >= o) scan += v;
+    most = max(most, __shfl_xor_sync(~0u, most, o));
+  }
+  if (lane == 31) {
+    s_warp[0][warp] = scan;
+    s_warp[1][warp] = most;
   }
   __syncthreads();
-  griddep_wait();
-  RowSpan x = row_keys(p, row, split);
-  const PageSpan g = page_span(p, x, split);
-  if (split >= x.n_splits) return;
-  const int kvh = y / p.n_gsub, gofs = (y - kvh * p.n_gsub) * p.g_tile;
-  const int G = min(p.g_tile, p.group - gofs), head0 = kvh * p.group + gofs;
-  const int P = p.kv.page_size;
-  const int ntiles = x.end > x.begin ? (x.end - x.begin + KT - 1) / KT : 0;
-  bool failed = false;
+  int before = scan - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w <= NCW; ++w) {
+    if (w < warp) before += s_warp[0][w];
+    total += s_warp[0][w];
+    most = max(most, s_warp[1][w]);
+  }
+  for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
+    const int nt = s_cum[i];
+    s_cum[i] = before;
+    before += nt;
+  }
+  if (tid == 0) s_cum[nrows] = total;
+  __syncthreads();
+
+  // ---- this CTA's share [w0, w1) of the axis. Where every pair can have a
+  // CTA of its own and sharing would save less than kJoinTiles, pairs stay
+  // whole: joining the parts costs about as much.
+  const int ncta = gridDim.x;
+  const long work = (long)total * p.n_y;
+  int share = (int)((work + ncta - 1) / ncta);
+  if (share < kMinTiles) share = kMinTiles;
+  const bool whole_pairs = (long)nrows * p.n_y <= ncta && most <= share + kJoinTiles;
+  long w0 = (long)blockIdx.x * share;
+  const long w1 = min(w0 + share, work);
+  Segment first;
+  if (whole_pairs) {
+    if (blockIdx.x >= nrows * p.n_y) return;
+    first.row = blockIdx.x / p.n_y;
+    first.y = blockIdx.x - first.row * p.n_y;
+    first.nt = s_cum[first.row + 1] - s_cum[first.row];
+    first.t0 = 0;
+    first.t1 = first.nt;
+  } else {
+    if (w0 >= work) return;
+    int lo = 0, hi = nrows;   // s_cum[lo] * n_y <= w0 < s_cum[hi] * n_y
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((long)s_cum[mid] * p.n_y <= w0) lo = mid; else hi = mid;
+    }
+    first.row = lo;
+    first.nt = s_cum[lo + 1] - s_cum[lo];
+    const int rem = (int)(w0 - (long)s_cum[lo] * p.n_y);
+    first.y = rem / first.nt;
+    first.t0 = rem - first.y * first.nt;
+    first.t1 = (int)min((long)first.nt, first.t0 + w1 - w0);
+  }
+  // the segment after g, w = position of its first tile on the axis
+  auto advance = [&](Segment &g, long &w) {
+    w += g.t1 - g.t0;
+    if (whole_pairs || w >= w1) return false;
+    if (++g.y == p.n_y) {
+      g.y = 0;
+      ++g.row;
+      g.nt = s_cum[g.row + 1] - s_cum[g.row];
+    }
+    g.t0 = 0;
+    g.t1 = (int)min((long)g.nt, w1 - w);
+    return true;
+  };
+  const int P = p.kv.page_size, box = min(P, KT);   // slots of one load
 
   if (warp == NCW) {
     // ---- producer: lane (kv, sub, page of the tile) issues its loads
-    const int box = min(P, KT), pt = KT / box;          // slots of a load, pages of a tile
+    const int pt = KT / box;
     const int j = lane % pt, sub = lane / pt % T::SUB, is_v = lane / pt / T::SUB;
     const bool mine = is_v < 2;
-    const int *table = p.kv.table + (size_t)x.seq * p.kv.table_stride;
-    // page of tile t for this lane: -1 past the end, -2 out of range
-    auto entry = [&](int t) {
-      const int u = x.begin + t * KT + j * box;
-      if (t >= ntiles || u >= x.end) return -1;
-      const int page = table[g.column(p.kv.column(u))];
-      return page >= 0 && page < p.kv.n_pages ? page : -2;
-    };
-    int next0 = entry(0), next1 = entry(1);
-    for (int t = 0; t < ntiles; ++t) {
-      const int s = t % kStages, page = next0;
-      next0 = next1;
-      next1 = entry(t + 2);
-      const uint32_t good = __ballot_sync(~0u, mine && page >= 0);
-      const uint32_t bad = __ballot_sync(~0u, lane < pt && page == -2);
-      if (t >= kStages && !mbar_wait_bounded(&empty[s], (t / kStages - 1) & 1)) failed = true;
-      if (__any_sync(~0u, failed)) {
-        failed = true;
-        break;
+    const uint32_t dst0 = smem_u32(smem) + (is_v ? T::BYTES : 0) + sub * T::SUB_BYTES +
+                          j * box * 128;
+    Segment g = first;
+    int it = 0;        // tiles issued
+    bool more = true, failed = false;
+    while (more && !failed) {
+      int xs, xa;
+      const PageSpan ps = page_span(p, s_len[g.row], &xs, &xa);
+      const int seq = p.row_seq ? p.row_seq[row0 + g.row] : row0 + g.row;
+      const int *table = p.kv.table + (size_t)seq * p.kv.table_stride;
+      const int kvh = g.y / p.n_gsub;
+      // page of tile t for this lane: -1 past the end, -2 out of range
+      auto entry = [&](int t) {
+        const int u = t * KT + j * box;
+        if (t >= g.t1 || u >= ps.n) return -1;
+        const int page = table[ps.column(p.kv.column(u))];
+        return page >= 0 && page < p.kv.n_pages ? page : -2;
+      };
+      int next0 = entry(g.t0), next1 = entry(g.t0 + 1);
+      for (int t = g.t0; t < g.t1; ++t, ++it) {
+        const int s = it % kStages, page = next0;
+        next0 = next1;
+        next1 = entry(t + 2);
+        const uint32_t good = __ballot_sync(~0u, mine && page >= 0);
+        const uint32_t bad = __ballot_sync(~0u, lane < pt && page == -2);
+        if (it >= kStages && (s_fail || !mbar_wait_bounded(&empty[s], (it / kStages - 1) & 1)))
+          failed = true;
+        if (__any_sync(~0u, failed)) {
+          failed = true;
+          break;
+        }
+        if (lane == 0) {
+          s_bad[s] = bad;
+          mbar_expect_tx(&full[s], __popc(good) * box * 128);
+          if (bad) atomicOr(p.err, DEV_ERR_PAGE);
+        }
+        __syncwarp();
+        if (mine && page >= 0) {
+          const int u = t * KT + j * box;
+          const int slot = u - p.kv.column(u) * P;
+          tma_load_4d(dst0 + s * 2 * T::BYTES, is_v ? &mv : &mk, &full[s], sub * 64,
+                      slots_first ? kvh : slot, slots_first ? slot : kvh, page);
+        }
       }
+      more = advance(g, w0);
+    }
+    if (failed) {
+      // let the copies in flight land (bounded) before the CTA exits
       if (lane == 0) {
-        s_bad[s] = bad;
-        s_issued = t + 1;
-        mbar_expect_tx(&full[s], __popc(good) * box * 128);
-        if (bad) atomicOr(p.err, DEV_ERR_PAGE);
+        atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+        s_fail = 1;
+        for (int t = max(0, it - kStages); t < it; ++t)
+          mbar_wait_bounded(&full[t % kStages], (t / kStages) & 1, 1u << 12);
       }
       __syncwarp();
-      if (mine && page >= 0) {
-        const int u = x.begin + t * KT + j * box;
-        const int slot = u - p.kv.column(u) * P;
-        const uint32_t dst = smem_u32(smem) + (is_v ? kStages * T::BYTES : 0) + s * T::BYTES +
-                             sub * T::SUB_BYTES + j * box * 128;
-        tma_load_4d(dst, is_v ? &mv : &mk, &full[s], sub * 64, slots_first ? kvh : slot,
-                    slots_first ? slot : kvh, page);
-      }
     }
+    return;
   }
 
   // ---- consumers. Fragments: rows (keys, or dims of O^T) r0 and r0 + 8,
-  // columns (heads) cq and cq + 1 of every block of 8.
+  // columns (heads) cq and cq + 1 of every block of 8. A wait that runs out
+  // sets s_fail and an error bit; the CTA then goes through its segments
+  // without waiting, so that barriers and tickets stay in step.
   const int r0 = lane >> 2, cq = (lane & 3) * 2;
-  float o[QB][D / 16][4], m_r[QB][2], l_r[QB][2];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    m_r[qb][0] = m_r[qb][1] = -INFINITY;
-    l_r[qb][0] = l_r[qb][1] = 0.f;
-#pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[qb][mb][e] = 0.f;
-  }
-  if (warp < NCW) {
+  // ldmatrix rows: K as the A operand, V^T by the transposing load
+  const int key0 = warp * KB * 16;   // this warp's first key of a tile
+  const int a_key = key0 + ((lane >> 3) & 1) * 8 + (lane & 7), a_dim = (lane >> 4) * 8;
+  const int t_key = key0 + (lane >> 4) * 8 + (lane & 7), t_dim = ((lane >> 3) & 1) * 8;
+  Segment g = first;
+  int it = 0;
+  bool more = true;
+  while (more) {
+    const int row = row0 + g.row;
+    int xs, xa;
+    const PageSpan ps = page_span(p, s_len[g.row], &xs, &xa);
+    const int kvh = g.y / p.n_gsub, gofs = (g.y - kvh * p.n_gsub) * p.g_tile;
+    const int G = min(p.g_tile, p.group - gofs), head0 = kvh * p.group + gofs;
+    const int sink_keys = ps.sink_pages * P;
+    float o[QB][D / 16][4], m_r[QB][2], l_r[QB][2];
     uint32_t qf[QB][D / 16][2][3];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+    for (int qb = 0; qb < QB; ++qb) {
+      m_r[qb][0] = m_r[qb][1] = -INFINITY;
+      l_r[qb][0] = l_r[qb][1] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
+      for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[qb][kk][e] = 0.f;
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           float2 v = make_float2(0.f, 0.f);
@@ -583,68 +801,77 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
                                                   kk * 16 + cq + 8 * f);
           split3(v.x * p.qscale, v.y * p.qscale, qf[qb][kk][f]);
         }
-    // ldmatrix rows: K as the A operand, V^T by the transposing load
-    const int a_key = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), a_dim = (lane >> 4) * 8;
-    const int t_key = warp * 16 + (lane >> 4) * 8 + (lane & 7), t_dim = ((lane >> 3) & 1) * 8;
-    const int sink_keys = g.sink_pages * P;
-
-    for (int t = 0; t < ntiles; ++t) {
-      const int s = t % kStages;
-      if (!__all_sync(~0u, mbar_wait_bounded(&full[s], (t / kStages) & 1))) {
-        failed = true;
-        break;
       }
-      const uint32_t kt = smem_u32(smem) + s * T::BYTES;
-      const uint32_t vt = kt + kStages * T::BYTES;
-      const int u0 = x.begin + t * KT + warp * 16;   // this warp's first key
+    }
+
+    for (int t = g.t0; t < g.t1; ++t, ++it) {
+      const int s = it % kStages;
+      const bool ok = !s_fail && mbar_wait_bounded(&full[s], (it / kStages) & 1);
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0 && !s_fail) atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+        s_fail = 1;
+        continue;
+      }
+      const uint32_t kt = smem_u32(smem) + s * 2 * T::BYTES;
+      const uint32_t vt = kt + T::BYTES;
+      const int u0 = t * KT + key0;
       const uint32_t bad = s_bad[s];
-      // position of key u0 + i, and whether the row sees it
+      // whether the row sees key u0 + i
       auto sees = [&](int i) {
         const int u = u0 + i;
-        if (u >= x.end || (bad && (bad >> ((warp * 16 + i) / min(P, KT)) & 1))) return false;
-        const int pos = u < sink_keys ? u : u - sink_keys + g.first * P;
-        return pos < x.s || pos >= x.a;
+        if (u >= ps.n || (bad && (bad >> ((key0 + i) / box) & 1))) return false;
+        const int pos = u < sink_keys ? u : u - sink_keys + ps.first * P;
+        return pos < xs || pos >= xa;
       };
-      const int pos0 = u0 < sink_keys ? 0 : u0 - sink_keys + g.first * P;
-      const bool whole = !bad && u0 + 16 <= x.end && pos0 >= x.a;
+      const int pos0 = u0 < sink_keys ? 0 : u0 - sink_keys + ps.first * P;
+      const bool whole = !bad && u0 + KB * 16 <= ps.n && pos0 >= xa;
 
-      float sc[QB][3][4];
+      float sc[QB][KB][3][4];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[qb][i][e] = 0.f;
+          for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[qb][kb][i][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const int dim = kk * 16 + a_dim;
-        uint32_t ka[4];
-        ldsm_x4(kt + (dim >> 6) * T::SUB_BYTES + a_key * 128 +
-                    ((((dim & 63) >> 3) ^ (a_key & 7)) << 4),
-                ka[0], ka[1], ka[2], ka[3]);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t ka[4];
+          ldsm_x4(kt + (dim >> 6) * T::SUB_BYTES + (a_key + kb * 16) * 128 +
+                      ((((dim & 63) >> 3) ^ (a_key & 7)) << 4),
+                  ka[0], ka[1], ka[2], ka[3]);
 #pragma unroll
-          for (int i = 0; i < 3; ++i)   // (three independent sums)
-            mma_bf16(sc[qb][i], ka, qf[qb][kk][0][i], qf[qb][kk][1][i]);
+          for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+            for (int i = 0; i < 3; ++i)   // (independent sums)
+              mma_bf16(sc[qb][kb][i], ka, qf[qb][kk][0][i], qf[qb][kk][1][i]);
+        }
       }
-      uint32_t pb[QB][2][3];
-      bool see0 = true, see1 = true;
-      if (!whole) {
-        see0 = sees(r0);
-        see1 = sees(r0 + 8);
-      }
+      uint32_t pb[QB][KB][2][3];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        float w[4];
+        float w[KB][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = sc[qb][0][e] + (sc[qb][1][e] + sc[qb][2][e]);
-          if (!(e < 2 ? see0 : see1)) w[e] = -INFINITY;
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[kb][e] = sc[qb][kb][0][e] + (sc[qb][kb][1][e] + sc[qb][kb][2][e]);
+        if (!whole) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            if (!sees(kb * 16 + r0)) w[kb][0] = w[kb][1] = -INFINITY;
+            if (!sees(kb * 16 + r0 + 8)) w[kb][2] = w[kb][3] = -INFINITY;
+          }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(w[c], w[c + 2]);
+          float mx = fmaxf(w[0][c], w[0][c + 2]);
+#pragma unroll
+          for (int kb = 1; kb < KB; ++kb) mx = fmaxf(mx, fmaxf(w[kb][c], w[kb][c + 2]));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
@@ -660,27 +887,33 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
             }
             m_r[qb][c] = mn;
           }
-          w[c] = fast_exp2(w[c] - base);
-          w[c + 2] = fast_exp2(w[c + 2] - base);
-          l_r[qb][c] += w[c] + w[c + 2];
-        }
-        uint32_t t0[3], t1[3];
-        split3_weight(w[0], w[1], t0);   // key r0
-        split3_weight(w[2], w[3], t1);   // key r0 + 8
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          pb[qb][0][i] = transpose8(t0[i]);
-          pb[qb][1][i] = transpose8(t1[i]);
+          for (int kb = 0; kb < KB; ++kb) {
+            w[kb][c] = fast_exp2(w[kb][c] - base);
+            w[kb][c + 2] = fast_exp2(w[kb][c + 2] - base);
+            l_r[qb][c] += w[kb][c] + w[kb][c + 2];
+          }
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t t0[3], t1[3];
+          split3_weight(w[kb][0], w[kb][1], t0);   // key r0
+          split3_weight(w[kb][2], w[kb][3], t1);   // key r0 + 8
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            pb[qb][kb][0][i] = transpose8(t0[i]);
+            pb[qb][kb][1][i] = transpose8(t1[i]);
+          }
         }
       }
       if (!whole) {
         // V of keys that the row does not see may be anything, NaN too, and
         // 0 * NaN is no 0: clear it
-        for (int i = lane; i < 16 * T::SUB * 8; i += 32) {
+        for (int i = lane; i < KB * 16 * T::SUB * 8; i += 32) {
           const int key = i / (T::SUB * 8), c = i % (T::SUB * 8);
           if (!sees(key))
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             vt + (c >> 3) * T::SUB_BYTES + (warp * 16 + key) * 128 +
+                             vt + (c >> 3) * T::SUB_BYTES + (key0 + key) * 128 +
                              ((c & 7) << 4)),
                          "r"(0)
                          : "memory");
@@ -690,49 +923,43 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) {
         const int dim = mb * 16 + t_dim;
-        uint32_t va[4];
-        ldsm_x4_t(vt + (dim >> 6) * T::SUB_BYTES + t_key * 128 +
-                      ((((dim & 63) >> 3) ^ (t_key & 7)) << 4),
-                  va[0], va[1], va[2], va[3]);
+        uint32_t va[KB][4];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          ldsm_x4_t(vt + (dim >> 6) * T::SUB_BYTES + (t_key + kb * 16) * 128 +
+                        ((((dim & 63) >> 3) ^ (t_key & 7)) << 4),
+                    va[kb][0], va[kb][1], va[kb][2], va[kb][3]);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
           float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 2; i >= 0; --i) mma_bf16(d, va, pb[qb][0][i], pb[qb][1][i]);
+          for (int i = 2; i >= 0; --i)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+              mma_bf16(d, va[kb], pb[qb][kb][0][i], pb[qb][kb][1][i]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[qb][mb][e] += d[e];
         }
       }
-      if (!whole) fence_proxy_async();   // generic writes before the next TMA
-      __syncwarp();
-      if (lane == 0) arrive(&empty[s]);
+      if (t + 1 < g.t1) {   // (the segment's last stage is held for the join)
+        if (!whole) fence_proxy_async();   // generic writes before the next TMA
+        __syncwarp();
+        if (lane == 0) arrive(&empty[s]);
+      }
     }
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l_r[qb][c] += __shfl_xor_sync(~0u, l_r[qb][c], d);
-  }
-  if (failed) {
-    atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
-    s_flag = 1;
-  }
-  __syncthreads();
-  if (s_flag) {
-    // let the copies in flight land (bounded) before the CTA exits
-    if (tid == 0)
-      for (int t = max(0, s_issued - kStages); t < s_issued; ++t)
-        mbar_wait_bounded(&full[t % kStages], (t / kStages) & 1, 1u << 12);
-    return;
-  }
-  float *w_acc = reinterpret_cast<float *>(smem);
-  float *w_m = w_acc + NCW * G * D, *w_l = w_m + NCW * G;
-  if (warp < NCW) {
+
+    // ---- join the warps through the last stage's 32 KB, which the producer
+    // gets back afterwards; it loads the next segment's tiles meanwhile
+    const int held = (it - 1) % kStages;
+    float *w_acc = reinterpret_cast<float *>(smem + held * 2 * T::BYTES);   // [NCW][G][D]
+    bar_consumers(NCW * 32);   // all have read the stage
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        float l = l_r[qb][c];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(~0u, l, d);
         const int h = qb * 8 + cq + c;
         if (h >= G) continue;
 #pragma unroll
@@ -741,32 +968,90 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
           w_acc[(warp * G + h) * D + mb * 16 + r0 + 8] = o[qb][mb][c + 2];
         }
         if (r0 == 0) {
-          w_m[warp * G + h] = m_r[qb][c];
-          w_l[warp * G + h] = l_r[qb][c];
+          s_m[warp][h] = m_r[qb][c];
+          s_l[warp][h] = l;
         }
       }
+    bar_consumers(NCW * 32);
+    const bool part = g.t0 > 0 || g.t1 < g.nt;
+    const size_t out_row = (size_t)row * p.o_sr + (size_t)head0 * p.o_sh;
+    const long begin = w0 - g.t0;   // of the pair on the axis
+    const size_t cta = (size_t)blockIdx.y * ncta + blockIdx.x;
+    float *mine = p.part_acc + (cta * 2 + (g.t0 == 0)) * p.g_tile * D;
+    float *mine_ml = p.part_ml + (cta * 2 + (g.t0 == 0)) * p.g_tile * 2;
+    for (int i = tid; i < G * D; i += NCW * 32) {
+      const int h = i / D;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NCW; ++w) mx = fmaxf(mx, s_m[w][h]);
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < NCW; ++w) {
+        const float m = s_m[w][h];
+        // (a warp without a visible key has m = -inf and sums of zero)
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
+        num = fmaf(w_acc[w * G * D + i], f, num);
+        den = fmaf(s_l[w][h], f, den);
+      }
+      if (!part) {
+        store_out(p, out_row + (size_t)h * p.o_sh + (i - h * D), den == 0.f ? 0.f : num / den);
+      } else {
+        mine[i] = num;
+        if (i == h * D) {
+          mine_ml[h * 2] = mx;
+          mine_ml[h * 2 + 1] = den;
+        }
+      }
+    }
+    if (part) {
+      // parts of a pair lie in the second slot of the CTA that starts it and
+      // the first slots of those after it; the last one to finish joins them
+      const int c0 = (int)(begin / share), c1 = (int)((begin + g.nt - 1) / share);
+      const int n = c1 - c0 + 1;
+      __threadfence();
+      bar_consumers(NCW * 32);
+      if (tid == 0) {
+        int *ctr = p.counters + (size_t)blockIdx.y * ncta + c0;
+        s_last = atomicAdd(ctr, 1) == n - 1;
+        if (s_last) *ctr = 0;   // all other parts took their ticket
+      }
+      bar_consumers(NCW * 32);
+      if (s_last) {
+        const size_t base = ((size_t)blockIdx.y * ncta + c0) * 2;
+        join_parts<D, NCW>(p, base, n, G, w_acc, out_row);
+      }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) arrive(&empty[held]);
+    more = advance(g, w0);
   }
-  __syncthreads();
-  finish_split<NCW, T::THREADS>(p, x, row, y, head0, G, D, split, w_acc, &s_flag);
 }
 
 // --------------------------------------------------------------------------
 // Host side
 // --------------------------------------------------------------------------
+using MmaKern = void (*)(const AttnParams, const CUtensorMap, const CUtensorMap, const int);
+
+// The kernel for D and heads per CTA, and its CTAs per SM (looked up once per
+// device).
 template <int D, int QB>
-int launch_mma(const AttnParams &p, const CUtensorMap &mk, const CUtensorMap &mv,
-               bool slots_first, dim3 grid, cudaStream_t st) {
-  auto kern = paged_mma_kernel<D, QB>;
-  static bool configured[64] = {};
+int mma_setup(MmaKern *kern, int *per_sm) {
+  static int occupancy[64] = {};
   int dev = 0;
   TLLM_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    TLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  TLLM_CHECK_ARG(dev >= 0 && dev < 64, "device index %d out of range", dev);
+  *kern = paged_mma_kernel<D, QB>;
+  if (!occupancy[dev]) {
+    TLLM_CUDA(cudaFuncSetAttribute(*kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)Tile<D>::SMEM));
-    if (dev >= 0 && dev < 64) configured[dev] = true;
+    int n = 0;
+    TLLM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, *kern, Tile<D>::THREADS,
+                                                            Tile<D>::SMEM));
+    TLLM_CHECK_ARG(n > 0, "the kernel does not fit the device");
+    occupancy[dev] = n;
   }
-  TLLM_CUDA(launch_pdl(kern, grid, dim3(Tile<D>::THREADS), Tile<D>::SMEM, st, p, mk, mv,
-                       (int)slots_first));
+  *per_sm = occupancy[dev];
   return TLLM_OK;
 }
 
@@ -888,13 +1173,20 @@ extern "C" int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_hea
   TLLM_CHECK_ARG(rows >= 0 && n_head > 0 && n_kv_head > 0 && head_dim > 0, "invalid shape");
   TLLM_CHECK_ARG(n_head % n_kv_head == 0, "n_head (%d) must be divisible by n_kv_head (%d)",
                  n_head, n_kv_head);
-  // splits per row that fill the GPU a few times over, and at least 8
+  // One token per row and split (heads of a KV head padded to a tile of 1, 2, 4
+  // or 8): splits that fill the GPU a few times over, at least 8. Or two parts
+  // of up to 16 heads per CTA and block of rows of the tensor-core kernel.
   long splits = 8192 / ((long)(rows > 0 ? rows : 1) * n_kv_head);
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 8) splits = 8;
-  // (heads of a KV head may be padded to the next tile of 1, 2, 4 or 8)
-  *partial_bytes = (size_t)rows * n_head * 2 * splits * (head_dim + 2) * sizeof(float);
-  *counter_bytes = (size_t)rows * n_head * sizeof(int32_t);
+  const size_t row = (head_dim + 2) * sizeof(float);
+  const size_t ctas = (size_t)(rows + kRowBlock - 1) / kRowBlock * kMaxPerSm * sm_count();
+  const int group = n_head / n_kv_head;
+  const size_t a = (size_t)rows * n_head * 2 * splits * row;
+  const size_t b = ctas * 2 * (group < 16 ? group : 16) * row;
+  *partial_bytes = a > b ? a : b;
+  const size_t c = (size_t)rows * n_head;
+  *counter_bytes = (c > ctas ? c : ctas) * sizeof(int32_t);
   return TLLM_OK;
 }
 
@@ -967,21 +1259,47 @@ extern "C" int tllm_paged_attention(
     most += 2 * (P > tile ? P : tile);
     if (most > cap) most = cap;
   }
-  int chunk = plan_chunk(tile, rows, n_y, keys, most, (mma ? 2L : 4L) * sm_count());
-  long splits = most > 0 ? (most + chunk - 1) / chunk : 1;
-  const size_t one = (size_t)rows * n_y * g_tile * (D + 2) * sizeof(float);
-  if (splits > 1 && one * splits > partial_bytes) {
-    splits = partial_bytes / one;
-    if (splits < 1) splits = 1;
-    const long per = (most + splits - 1) / splits;
-    chunk = (int)((per + tile - 1) / tile * tile);
+  // tensor-core kernel: CTAs that share a block of rows, as many as are
+  // resident at once and have work; others: splits of a row
+  int chunk = 0;
+  long splits = 1, ctas = 1;
+  const long blocks = (rows + kRowBlock - 1) / kRowBlock;
+  MmaKern kern = nullptr;
+  size_t one, count;
+  if (mma) {
+    int per_sm = 0;
+    if (D == 64)
+      rc = g_tile <= 8 ? mma_setup<64, 1>(&kern, &per_sm) : mma_setup<64, 2>(&kern, &per_sm);
+    else
+      rc = g_tile <= 8 ? mma_setup<128, 1>(&kern, &per_sm) : mma_setup<128, 2>(&kern, &per_sm);
+    if (rc) return rc;
+    const long pairs = (long)(rows < kRowBlock ? rows : kRowBlock) * n_y;
+    const long tiles = pairs * ((most + tile - 1) / tile);
+    ctas = (tiles + kMinTiles - 1) / kMinTiles;
+    if (ctas < pairs) ctas = pairs;
+    if (ctas > (long)per_sm * sm_count()) ctas = (long)per_sm * sm_count();
+    one = (size_t)blocks * 2 * g_tile * (D + 2) * sizeof(float);
+    if (ctas > 1 && one * ctas > partial_bytes) ctas = partial_bytes / one;
+    if (ctas < 1) ctas = 1;
+    count = ctas > 1 ? blocks * ctas : 0;
+  } else {
+    chunk = plan_chunk(tile, rows, n_y, keys, most, 4L * sm_count());
+    splits = most > 0 ? (most + chunk - 1) / chunk : 1;
+    one = (size_t)rows * n_y * g_tile * (D + 2) * sizeof(float);
+    if (splits > 1 && one * splits > partial_bytes) {
+      splits = partial_bytes / one;
+      if (splits < 1) splits = 1;
+      const long per = (most + splits - 1) / splits;
+      chunk = (int)((per + tile - 1) / tile * tile);
+    }
+    count = splits > 1 ? (size_t)rows * n_y : 0;
   }
-  if (splits > 1) {
+  if (count > 0) {
     TLLM_CHECK_ARG(partial && counters, "several splits need the partial and counter buffers");
     TLLM_CHECK_ARG(((uintptr_t)partial & 15) == 0, "partial misaligned");
-    TLLM_CHECK_ARG(counter_bytes >= (size_t)rows * n_y * sizeof(int32_t),
+    TLLM_CHECK_ARG(counter_bytes >= count * sizeof(int32_t),
                    "counters hold %zu bytes, %zu needed", counter_bytes,
-                   (size_t)rows * n_y * sizeof(int32_t));
+                   count * sizeof(int32_t));
   }
 
   if (sm_scale <= 0.f) sm_scale = 1.0f / sqrtf((float)D);
@@ -998,10 +1316,12 @@ extern "C" int tllm_paged_attention(
   p.o_sr = out_row_stride;
   p.o_sh = out_head_stride;
   p.part_acc = static_cast<float *>(partial);
-  p.part_ml = p.part_acc ? p.part_acc + (size_t)rows * n_y * splits * g_tile * D : nullptr;
+  const size_t slots = mma ? (size_t)blocks * ctas * 2 : (size_t)rows * n_y * splits;
+  p.part_ml = p.part_acc ? p.part_acc + slots * g_tile * D : nullptr;
   p.counters = counters;
   p.err = device_error_ptr();
   TLLM_CHECK_ARG(p.err, "device error word unavailable");
+  p.rows = rows;
   p.group = group;
   p.n_gsub = n_gsub;
   p.g_tile = g_tile;
@@ -1012,7 +1332,6 @@ extern "C" int tllm_paged_attention(
   p.window = window;
   p.sinks = sinks;
   p.qscale = sm_scale * kLog2e;
-  const dim3 grid((unsigned)splits, n_y, rows);
   cudaStream_t st = resolve(stream);
   if (mma) {
     const bool slots_first = n_kv > 1 && kv->head_stride < kv->slot_stride;
@@ -1020,12 +1339,13 @@ extern "C" int tllm_paged_attention(
     rc = page_map(&mk, kv->k_pages, kv, P < tile ? P : tile, slots_first);
     if (!rc) rc = page_map(&mv, kv->v_pages, kv, P < tile ? P : tile, slots_first);
     if (rc) return rc;
-    if (D == 64)
-      return g_tile <= 8 ? launch_mma<64, 1>(p, mk, mv, slots_first, grid, st)
-                         : launch_mma<64, 2>(p, mk, mv, slots_first, grid, st);
-    return g_tile <= 8 ? launch_mma<128, 1>(p, mk, mv, slots_first, grid, st)
-                       : launch_mma<128, 2>(p, mk, mv, slots_first, grid, st);
+    TLLM_CUDA(launch_pdl(kern, dim3((unsigned)ctas, (unsigned)blocks),
+                         dim3(D == 64 ? Tile<64>::THREADS : Tile<128>::THREADS),
+                         D == 64 ? Tile<64>::SMEM : Tile<128>::SMEM, st, p, mk, mv,
+                         (int)slots_first));
+    return TLLM_OK;
   }
+  const dim3 grid((unsigned)splits, n_y, rows);
   return kv->kv_dtype == TLLM_BF16
              ? launch_rows_t<__nv_bfloat16>(p, lpr, nv, grid, st)
              : launch_rows_t<float>(p, lpr, nv, grid, st);
