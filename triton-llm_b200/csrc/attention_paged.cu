@@ -1267,17 +1267,11 @@ extern "C" int tllm_paged_attention(
   MmaKern kern = nullptr;
   size_t one, count;
   if (mma) {
-    int per_sm = 0;
-    if (D == 64)
-      rc = g_tile <= 8 ? mma_setup<64, 1>(&kern, &per_sm) : mma_setup<64, 2>(&kern, &per_sm);
-    else
-      rc = g_tile <= 8 ? mma_setup<128, 1>(&kern, &per_sm) : mma_setup<128, 2>(&kern, &per_sm);
-    if (rc) return rc;
     const long pairs = (long)(rows < kRowBlock ? rows : kRowBlock) * n_y;
     const long tiles = pairs * ((most + tile - 1) / tile);
     ctas = (tiles + kMinTiles - 1) / kMinTiles;
     if (ctas < pairs) ctas = pairs;
-    if (ctas > (long)per_sm * sm_count()) ctas = (long)per_sm * sm_count();
+    if (ctas > (long)kMaxPerSm * sm_count()) ctas = (long)kMaxPerSm * sm_count();
     one = (size_t)blocks * 2 * g_tile * (D + 2) * sizeof(float);
     if (ctas > 1 && one * ctas > partial_bytes) ctas = partial_bytes / one;
     if (ctas < 1) ctas = 1;
@@ -1300,6 +1294,16 @@ extern "C" int tllm_paged_attention(
     TLLM_CHECK_ARG(counter_bytes >= count * sizeof(int32_t),
                    "counters hold %zu bytes, %zu needed", counter_bytes,
                    count * sizeof(int32_t));
+  }
+
+  if (mma) {
+    int per_sm = 0;
+    if (D == 64)
+      rc = g_tile <= 8 ? mma_setup<64, 1>(&kern, &per_sm) : mma_setup<64, 2>(&kern, &per_sm);
+    else
+      rc = g_tile <= 8 ? mma_setup<128, 1>(&kern, &per_sm) : mma_setup<128, 2>(&kern, &per_sm);
+    if (rc) return rc;
+    if (ctas > (long)per_sm * sm_count()) ctas = (long)per_sm * sm_count();
   }
 
   if (sm_scale <= 0.f) sm_scale = 1.0f / sqrtf((float)D);
