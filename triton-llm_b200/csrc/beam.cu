@@ -6,7 +6,13 @@
 // L_b = max + log sum exp(x_bt - max). Within a beam the order is that of its
 // logits, so a CTA that reads a chunk of one row needs to keep only the
 // chunk's max, its sum of exponentials and its k largest logits; the last CTA
-// of a group to finish joins them.
+// of a group to finish joins them. Each logit is read once.
+//
+// The k largest of a CTA's values: the k-th largest of any set of at least k
+// of them is a bound that the k largest reach. With the threads' own maxima as
+// that set the bound leaves few values over, which go to shared memory and are
+// ranked by counting. Values carry their index in a 64-bit code, so all are
+// distinct and ties are in order.
 #include <cmath>
 
 #include "mma_sync.cuh"
@@ -18,8 +24,10 @@ namespace {
 constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kBeamWarps = 8;
-constexpr int kPerLane = 16;
-constexpr int kChunk = kBeamWarps * 32 * kPerLane;   // logits of one CTA
+constexpr int kBeamThreads = kBeamWarps * 32;
+constexpr int kPerLane = 16;                          // logits of a thread
+constexpr int kChunk = kBeamThreads * kPerLane;       // logits of a CTA
+constexpr int kBatch = 8;                             // listed candidates of a thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxRows = 65535;
 // the groups' tickets lie at the front of the workspace whatever its shape, so
@@ -40,15 +48,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor_sync(~0u, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-
 struct BeamParams {
   const float *logits;
   long ld;
@@ -62,50 +61,105 @@ struct BeamParams {
   uint64_t *lists;      // (rows, chunks, k)
 };
 
-// The k largest of n keys in shared memory, in order, into out[0..k); called
-// by one warp. n >= k. Destroys keys.
-__device__ void warp_select(uint64_t *keys, int n, int k, uint64_t *out) {
-  const int lane = threadIdx.x & 31;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    int at = -1;
-    for (int i = lane; i < n; i += 32)
-      if (keys[i] > best) {
-        best = keys[i];
-        at = i;
-      }
-    const uint64_t top = warp_max(best);
-    if (lane == 0) out[j] = top;
-    if (at >= 0 && best == top) keys[at] = 0;
-    __syncwarp();
+// A bound that at least k keys of the CTA reach, from every thread's largest
+// key `best`: the k-th largest of a warp's 32 (the best of the eight warps'),
+// or for k > 32 the least of the warps' ceil(k / 8)-th largest.
+__device__ __forceinline__ uint64_t key_bound(uint64_t best, int k, uint64_t *s_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // bitonic sort of the warp's keys, largest first
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const uint64_t other = __shfl_xor_sync(~0u, best, d);
+      const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
+      best = (other > best) == larger ? other : best;
+    }
+  const int nth = k <= 32 ? k : (k + kBeamWarps - 1) / kBeamWarps;
+  best = __shfl_sync(~0u, best, nth - 1);
+  if (lane == 0) s_warp[warp] = best;
+  __syncthreads();
+  uint64_t bound = s_warp[0];
+#pragma unroll
+  for (int w = 1; w < kBeamWarps; ++w)
+    bound = (s_warp[w] > bound) == (k <= 32) ? s_warp[w] : bound;
+  return bound;
+}
+
+__device__ __forceinline__ void keep(uint64_t key, uint64_t *list, int *n) {
+  list[atomicAdd(n, 1)] = key;
+}
+
+// Calls put(rank, key) for the k largest of the n keys of a list in shared
+// memory; all threads, after a barrier.
+template <typename F>
+__device__ __forceinline__ void rank_keys(const uint64_t *list, int n, int k, F put) {
+  for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+    const uint64_t key = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < k) put(rank, key);
   }
 }
 
-__global__ void __launch_bounds__(kBeamWarps * 32) beam_select_kernel(const BeamParams p) {
+template <bool kVec>
+__global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamParams p) {
   griddep_launch();
   griddep_wait();
-  extern __shared__ __align__(16) uint64_t smem_k[];
+  extern __shared__ __align__(16) uint64_t s_list[];
+  __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
-  __shared__ int s_last;
+  __shared__ int s_n, s_last;
   __shared__ float s_base[kMaxBeams], s_lse[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = p.k;
+  if (tid == 0) s_n = 0;
 
   if (!(p.done && p.done[row])) {
     const float *x = p.logits + (size_t)row * p.ld;
-    const int first = chunk * kChunk + warp * 32 * kPerLane + lane;
+    const int t0 = chunk * kChunk;
+    // value i of this thread: token t0 + index(i), ascending in i
+    auto index = [&](int i) {
+      return kVec ? (i >> 2) * 4 * kBeamThreads + 4 * tid + (i & 3) : i * kBeamThreads + tid;
+    };
+    const int left = p.vocab - t0;
     float v[kPerLane];
     bool nan = false;
+    if constexpr (kVec) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int t = first + i * 32;
-      v[i] = t < p.vocab ? __ldcs(x + t) : -INFINITY;
-      nan |= v[i] != v[i];
+      for (int i = 0; i < kPerLane; i += 4) {
+        const int at = index(i);
+        float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at + 3 < left) {
+          f = __ldcs(reinterpret_cast<const float4 *>(x + t0 + at));
+        } else {
+          if (at < left) f.x = x[t0 + at];
+          if (at + 1 < left) f.y = x[t0 + at + 1];
+          if (at + 2 < left) f.z = x[t0 + at + 2];
+        }
+        v[i] = f.x;
+        v[i + 1] = f.y;
+        v[i + 2] = f.z;
+        v[i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i)
+        v[i] = index(i) < left ? __ldcs(x + t0 + index(i)) : -INFINITY;
     }
     float m = -INFINITY;
+    int at = 0;      // the first largest
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) m = fmaxf(m, v[i]);
+    for (int i = 0; i < kPerLane; ++i) {
+      nan |= v[i] != v[i];
+      if (v[i] > m) {
+        m = v[i];
+        at = index(i);
+      }
+    }
+    if (m == -INFINITY) at = index(0);
+    const uint64_t best = at < left ? rank_key(m, (uint32_t)(t0 + at)) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     if (__any_sync(~0u, nan)) m = NAN;
@@ -119,39 +173,29 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_select_kernel(const Beam
       s_m[warp] = m;
       s_s[warp] = s;
     }
-    // this warp's k largest
-    uint32_t taken = 0;
-    for (int j = 0; j < k; ++j) {
-      uint64_t best = 0;
-      int at = -1;
+    const uint64_t bound = key_bound(best, k, s_warp);
+    const float least = bound ? key_value(bound) : -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int t = first + i * 32;
-        const uint64_t key = rank_key(v[i], (uint32_t)t);
-        if (t < p.vocab && !(taken >> i & 1) && key > best) {
-          best = key;
-          at = i;
-        }
+    for (int i = 0; i < kPerLane; ++i)
+      if (v[i] >= least && index(i) < left) {
+        const uint64_t key = rank_key(v[i], (uint32_t)(t0 + index(i)));
+        if (key >= bound) keep(key, s_list, &s_n);
       }
-      const uint64_t top = warp_max(best);
-      if (at >= 0 && best == top) taken |= 1u << at;
-      if (lane == 0) smem_k[warp * k + j] = top;
-    }
     __syncthreads();
-    if (warp == 0) {
-      warp_select(smem_k, kBeamWarps * k, k,
-                  p.lists + ((size_t)row * p.chunks + chunk) * k);
-      if (lane == 0) {
-        float mm = -INFINITY, ss = 0.f;
-        bool bad = false;
-        for (int w = 0; w < kBeamWarps; ++w) {
-          bad |= s_m[w] != s_m[w];
-          mm = fmaxf(mm, s_m[w]);
-        }
-        for (int w = 0; w < kBeamWarps; ++w)
-          if (s_m[w] != -INFINITY) ss += s_s[w] * fast_exp2((s_m[w] - mm) * kLog2e);
-        p.stats[(size_t)row * p.chunks + chunk] = make_float2(bad ? NAN : mm, ss);
+    uint64_t *list = p.lists + ((size_t)row * p.chunks + chunk) * k;
+    const int n = s_n;
+    rank_keys(s_list, n, k, [&](int rank, uint64_t key) { list[rank] = key; });
+    for (int i = n + tid; i < k; i += kBeamThreads) list[i] = 0;   // a short last chunk
+    if (tid == 0) {
+      float mm = -INFINITY, ss = 0.f;
+      bool bad = false;
+      for (int w = 0; w < kBeamWarps; ++w) {
+        bad |= s_m[w] != s_m[w];
+        mm = fmaxf(mm, s_m[w]);
       }
+      for (int w = 0; w < kBeamWarps; ++w)
+        if (s_m[w] != -INFINITY) ss += s_s[w] * fast_exp2((s_m[w] - mm) * kLog2e);
+      p.stats[(size_t)row * p.chunks + chunk] = make_float2(bad ? NAN : mm, ss);
     }
   }
   __threadfence();
@@ -160,27 +204,32 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_select_kernel(const Beam
     int *ctr = p.counters + group;
     s_last = atomicAdd(ctr, 1) == p.chunks * p.beams - 1;
     if (s_last) *ctr = 0;
+    s_n = 0;
   }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
 
-  // ---- the last CTA of the group: rows' logsumexp, then the k best
+  // ---- the last CTA of the group: the rows' logsumexp, then the k best
   for (int b = warp; b < p.beams; b += kBeamWarps) {
     const int r = group * p.beams + b;
     float mm = -INFINITY, ss = 0.f;
     if (!(p.done && p.done[r])) {
-      bool bad = false;
-      for (int c = lane; c < p.chunks; c += 32) {
-        const float m = __ldcg(&p.stats[(size_t)r * p.chunks + c]).x;
+      const float2 *stats = p.stats + (size_t)r * p.chunks;
+      const float2 own = lane < p.chunks ? __ldcg(stats + lane) : make_float2(-INFINITY, 0.f);
+      bool bad = own.x != own.x;
+      mm = own.x;
+      for (int c = lane + 32; c < p.chunks; c += 32) {
+        const float m = __ldcg(stats + c).x;
         bad |= m != m;
         mm = fmaxf(mm, m);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
       if (__any_sync(~0u, bad)) mm = NAN;
-      for (int c = lane; c < p.chunks; c += 32) {
-        const float2 st = __ldcg(&p.stats[(size_t)r * p.chunks + c]);
+      if (own.x != -INFINITY) ss = own.y * expf(own.x - mm);
+      for (int c = lane + 32; c < p.chunks; c += 32) {
+        const float2 st = __ldcg(stats + c);
         if (st.x != -INFINITY) ss += st.y * expf(st.x - mm);
       }
 #pragma unroll
@@ -192,59 +241,74 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_select_kernel(const Beam
     }
   }
   __syncthreads();
+  // candidates in batches of kBatch per thread beside the best of those before
   const int per = p.chunks * k, n = p.beams * per;
-  uint64_t mine[1];
-  (void)mine;
-  // candidates are visited k times; each round takes the best one left,
-  // which is the best below the last one taken (keys are distinct)
-  uint64_t last = ~0ull;
-  uint64_t *s_best = smem_k;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    for (int i = tid; i < n; i += kBeamWarps * 32) {
-      const int b = i / per, c = i - b * per;
-      const int r = group * p.beams + b;
-      const float base = s_base[b];
-      float score;
-      uint32_t token;
-      if (p.done && p.done[r]) {
-        if (c >= k) continue;
-        // the pad token first, then others at -inf in order
-        token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
-        score = c == 0 ? base : -INFINITY;
-      } else {
-        const float lse = s_lse[b];
-        const bool dead = !(fabsf(lse) < INFINITY) || !(fabsf(base) < INFINITY);
-        if (dead) {
-          if (c >= k) continue;
-          token = c;
-          score = -INFINITY;
-        } else {
-          const uint64_t key = __ldcg(&p.lists[(size_t)r * per + c]);
-          if (key == 0) continue;
-          token = key_index(key);
-          score = base + (key_value(key) - lse);
-        }
-      }
-      if (!(score == score)) score = -INFINITY;
-      const uint64_t key = rank_key(score, (uint32_t)b * p.vocab + token);
-      if (key < last && key > best) best = key;
-    }
-    best = warp_max(best);
-    __syncthreads();
-    if (lane == 0) s_best[warp] = best;
-    __syncthreads();
-    best = 0;
+  int kept = 0;
+  for (int i0 = 0; i0 < n; i0 += kBatch * kBeamThreads) {
+    uint64_t key[kBatch], best = tid < kept ? s_top[tid] : 0;
+    const uint64_t old = best;
+    // (the loads of a batch are in flight together)
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) best = s_best[w] > best ? s_best[w] : best;
-    last = best;
-    if (tid == 0) {
-      const uint32_t index = key_index(best);
-      p.out_scores[(size_t)group * k + j] = key_value(best);
-      p.out_parents[(size_t)group * k + j] = index / p.vocab;
-      p.out_tokens[(size_t)group * k + j] = index % p.vocab;
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kBeamThreads + tid;
+      key[j] = i < n ? __ldcg(&p.lists[(size_t)group * n + i]) : 0;
     }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kBeamThreads + tid;
+      uint64_t made = 0;
+      if (i < n) {
+        const int b = i / per, c = i - b * per;
+        const float base = s_base[b], lse = s_lse[b];
+        float score = -INFINITY;
+        uint32_t token = c;
+        bool is = true;
+        if (p.done && p.done[group * p.beams + b]) {
+          // the pad token, then others at -inf in order
+          is = c < k;
+          token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
+          if (c == 0) score = base;
+        } else if (!(fabsf(lse) < INFINITY) || !(fabsf(base) < INFINITY)) {
+          is = c < k;   // the beam has no finite candidate
+        } else {
+          is = key[j] != 0;
+          token = key_index(key[j]);
+          score = base + (key_value(key[j]) - lse);
+        }
+        if (!(score == score)) score = -INFINITY;
+        if (is) made = rank_key(score, (uint32_t)b * p.vocab + token);
+      }
+      key[j] = made;
+      best = made > best ? made : best;
+    }
+    const uint64_t bound = key_bound(best, k, s_warp);
+    if (old && old >= bound) keep(old, s_list, &s_n);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (key[j] && key[j] >= bound) keep(key[j], s_list, &s_n);
+    __syncthreads();
+    const int found = s_n;
+    rank_keys(s_list, found, k, [&](int rank, uint64_t code) { s_top[rank] = code; });
+    kept = min(found, k);
+    __syncthreads();
+    if (tid == 0) s_n = 0;
+    __syncthreads();
   }
+  if (tid < k) {
+    const uint32_t at = key_index(s_top[tid]);
+    p.out_scores[(size_t)group * k + tid] = key_value(s_top[tid]);
+    p.out_parents[(size_t)group * k + tid] = at / p.vocab;
+    p.out_tokens[(size_t)group * k + tid] = at % p.vocab;
+  }
+}
+
+// Keys that can reach the bound in the first pass (up to k threads of a warp
+// have a maximum that does, for k <= 32) and in a batch of the second.
+int list_size(int k) {
+  const int first = k <= 32 && k * kBeamWarps * kPerLane < kChunk ? k * kBeamWarps * kPerLane
+                                                                   : kChunk;
+  const int batch = kBatch * kBeamThreads + kMaxK;
+  return first > batch ? first : batch;
 }
 
 // --------------------------------------------------------------------------
@@ -374,9 +438,11 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   p.stats = reinterpret_cast<float2 *>(w);
   w += align256((size_t)groups * beams * p.chunks * sizeof(float2));
   p.lists = reinterpret_cast<uint64_t *>(w);
-  const size_t smem = (size_t)kBeamWarps * k * sizeof(uint64_t);
-  TLLM_CUDA(launch_pdl(beam_select_kernel, dim3(p.chunks, groups * beams),
-                       dim3(kBeamWarps * 32), smem, resolve(stream), p));
+  const size_t smem = list_size(k) * sizeof(uint64_t);
+  const bool vec = ((uintptr_t)logits & 15) == 0 && p.ld % 4 == 0;
+  TLLM_CUDA(launch_pdl(vec ? beam_select_kernel<true> : beam_select_kernel<false>,
+                       dim3(p.chunks, groups * beams), dim3(kBeamThreads), smem,
+                       resolve(stream), p));
   return TLLM_OK;
 }
 
