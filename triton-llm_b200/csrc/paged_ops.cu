@@ -113,10 +113,142 @@ __global__ void append_kernel(const __grid_constant__ AppendParams p) {
   }
 }
 
+// Four values of the source, and four results to fp32 or bf16.
+__device__ __forceinline__ float4 load4(const float *p) {
+  return __ldcs(reinterpret_cast<const float4 *>(p));
+}
+__device__ __forceinline__ float4 load4(const uint16_t *p) {
+  const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(p));
+  return make_float4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y));
+}
+__device__ __forceinline__ void store4(float *p, float4 v) {
+  *reinterpret_cast<float4 *>(p) = v;
+}
+__device__ __forceinline__ void store4(uint16_t *p, float4 v) {
+  uint2 r;
+  r.x = (uint32_t)f32_to_bf16_bits(v.x) | (uint32_t)f32_to_bf16_bits(v.y) << 16;
+  r.y = (uint32_t)f32_to_bf16_bits(v.z) | (uint32_t)f32_to_bf16_bits(v.w) << 16;
+  *reinterpret_cast<uint2 *>(p) = r;
+}
+
+// Heads of whole 8-value units on 16-byte rows: one thread takes kUnits units
+// of two runs of four values (a pair's two sides, or eight neighbours), with
+// all its loads issued before the row's page is known. One CTA per row: a row
+// moves a few KB, and 12 or more CTAs of an SM cover the chain of loads
+// position -> page -> store. HBM-bound: 12001 rows of 24 + 8 + 8 heads of 128
+// read 246 MB and write 197 MB.
+constexpr int kUnits = 4;
+
+template <typename S, typename T>
+__global__ void __launch_bounds__(512)
+    append_units_kernel(const __grid_constant__ AppendParams p) {
+  griddep_launch();
+  griddep_wait();
+  const int row = blockIdx.x;
+  const int D = p.kv.head_dim, H = p.in.q ? p.in.n_head : 0, K = p.kv.n_kv;
+  const int rot = p.in.cos_t ? p.in.rotary_dim : 0, half = rot >> 1;
+  const unsigned per = D >> 3, n = (H + 2 * K) * per;
+  const size_t from = p.in.row_src ? p.in.row_src[row] : row;
+  float4 x[kUnits], y[kUnits];
+  // runs a and b of unit u of a head
+  auto runs = [&](int head, int u, int *a, int *b) {
+    const bool turned = head < H + K && u < rot >> 3;
+    *a = turned && !p.in.interleaved ? 4 * u : 8 * u;
+    *b = *a + (turned && !p.in.interleaved ? half : 4);
+    return turned;
+  };
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const unsigned at = threadIdx.x + i * blockDim.x;
+    if (at >= n) continue;
+    const int head = at / per, u = at - head * per;
+    int a, b;
+    runs(head, u, &a, &b);
+    const S *src;
+    if (head < H)
+      src = static_cast<const S *>(p.in.q) + from * p.in.q_row_stride +
+            (size_t)head * p.in.q_head_stride;
+    else if (head < H + K)
+      src = static_cast<const S *>(p.in.k) + from * p.in.k_row_stride +
+            (size_t)(head - H) * p.in.k_head_stride;
+    else
+      src = static_cast<const S *>(p.in.v) + from * p.in.v_row_stride +
+            (size_t)(head - H - K) * p.in.v_head_stride;
+    x[i] = load4(src + source_dim(a, D, p.in.blocked));
+    y[i] = load4(src + source_dim(b, D, p.in.blocked));
+  }
+  AppendRow r;
+  if (!append_row(p, row, &r)) return;
+  if (threadIdx.x == 0 && p.in.lens_out) atomicMax(p.in.lens_out + r.seq, r.pos + 1);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const unsigned at = threadIdx.x + i * blockDim.x;
+    if (at >= n) continue;
+    const int head = at / per, u = at - head * per;
+    int a, b;
+    if (runs(head, u, &a, &b)) {
+      const size_t t = (size_t)r.pos * half + 4 * u;
+      const float4 c = __ldg(reinterpret_cast<const float4 *>(p.in.cos_t + t));
+      const float4 s = __ldg(reinterpret_cast<const float4 *>(p.in.sin_t + t));
+      const float4 v = x[i], w = y[i];
+      if (p.in.interleaved) {
+        x[i] = make_float4(v.x * c.x - v.y * s.x, v.y * c.x + v.x * s.x,
+                           v.z * c.y - v.w * s.y, v.w * c.y + v.z * s.y);
+        y[i] = make_float4(w.x * c.z - w.y * s.z, w.y * c.z + w.x * s.z,
+                           w.z * c.w - w.w * s.w, w.w * c.w + w.z * s.w);
+      } else {
+        x[i] = make_float4(v.x * c.x - w.x * s.x, v.y * c.y - w.y * s.y,
+                           v.z * c.z - w.z * s.z, v.w * c.w - w.w * s.w);
+        y[i] = make_float4(w.x * c.x + v.x * s.x, w.y * c.y + v.y * s.y,
+                           w.z * c.z + v.z * s.z, w.w * c.w + v.w * s.w);
+      }
+    }
+    if (head < H) {
+      float *to = p.in.q_out + (size_t)row * p.in.q_out_row_stride +
+                  (size_t)head * p.in.q_out_head_stride;
+      store4(to + a, x[i]);
+      store4(to + b, y[i]);
+    } else {
+      const bool is_v = head >= H + K;
+      T *to = static_cast<T *>(is_v ? p.kv.v : p.kv.k) +
+              p.kv.offset(r.page, head - H - (is_v ? K : 0), r.slot);
+      store4(to + a, x[i]);
+      store4(to + b, y[i]);
+    }
+  }
+}
+
+// Whether every run of four values that the call touches is aligned, and a
+// row fits one CTA.
+bool append_in_units(const AppendParams &p) {
+  const tllm_paged_rows &in = p.in;
+  const int src = in.src_dtype == TLLM_F32 ? 4 : 2;
+  long strides = in.k_row_stride | in.k_head_stride | in.v_row_stride | in.v_head_stride |
+                 p.kv.page_stride | p.kv.head_stride | p.kv.slot_stride;
+  // addresses aligned to four values of their type
+  bool ok = ((uintptr_t)in.k | (uintptr_t)in.v) % (4 * src) == 0 &&
+            ((uintptr_t)p.kv.k | (uintptr_t)p.kv.v) % 16 == 0;
+  if (in.q) {
+    strides |= in.q_row_stride | in.q_head_stride | in.q_out_row_stride | in.q_out_head_stride;
+    ok = ok && (uintptr_t)in.q % (4 * src) == 0 && (uintptr_t)in.q_out % 16 == 0;
+  }
+  if (in.cos_t)
+    ok = ok && ((uintptr_t)in.cos_t | (uintptr_t)in.sin_t) % 16 == 0 && in.rotary_dim % 8 == 0;
+  const long units = ((in.q ? in.n_head : 0) + 2L * p.kv.n_kv) * (p.kv.head_dim / 8);
+  return ok && strides % 4 == 0 && p.kv.head_dim % 8 == 0 && units <= 512 * kUnits;
+}
+
 template <typename S, typename T>
 int launch_append(const AppendParams &p, cudaStream_t st) {
   const int D = p.kv.head_dim, rot = p.in.cos_t ? p.in.rotary_dim : 0;
-  const long items = ((p.in.q ? p.in.n_head : 0) + 2L * p.kv.n_kv) * (D - rot / 2);
+  const long heads = (p.in.q ? p.in.n_head : 0) + 2L * p.kv.n_kv;
+  if (append_in_units(p)) {
+    const long threads = (heads * (D / 8) + kUnits - 1) / kUnits;
+    TLLM_CUDA(launch_pdl(append_units_kernel<S, T>, dim3(p.in.rows),
+                         dim3((unsigned)((threads + 31) / 32 * 32)), 0, st, p));
+    return TLLM_OK;
+  }
+  const long items = heads * (D - rot / 2);
   const int threads = items >= 512 ? 512 : (int)((items + 31) / 32 * 32);
   TLLM_CUDA(launch_pdl(append_kernel<S, T>, dim3(p.in.rows), dim3(threads), 0, st, p));
   return TLLM_OK;
@@ -133,28 +265,39 @@ struct CopyParams {
   int *err;
 };
 
-// One CTA per (copy, plane); units of type U.
+// One CTA per (copy, plane). A warp takes pieces of kDeep units per lane of a
+// run, all loaded before the first is stored: 8 warps x 32 lanes x 8 units of
+// 16 bytes keep 32 KB of a CTA in flight.
+constexpr int kCopyWarps = 8, kDeep = 8;
+
 template <typename U>
-__global__ void page_copy_kernel(const CopyParams p) {
+__global__ void __launch_bounds__(kCopyWarps * 32) page_copy_kernel(const CopyParams p) {
   griddep_launch();
   griddep_wait();
   const int i = blockIdx.x;
-  const int src = p.src[i], dst = p.dst[i];
+  const int src = p.src[i], dst = p.dst[i], fill = p.fill ? p.fill[i] : p.page_size;
   if (src < 0 || dst < 0 || src == dst) return;
-  const int fill = p.fill ? p.fill[i] : p.page_size;
   if (src >= p.n_pages || dst >= p.n_pages || fill < 0 || fill > p.page_size) {
     if (threadIdx.x == 0) atomicOr(p.err, DEV_ERR_PAGE);
     return;
   }
-  char *plane = p.arena + (size_t)blockIdx.y * p.plane_stride;
-  const char *from = plane + (size_t)src * p.page_stride;
-  char *to = plane + (size_t)dst * p.page_stride;
-  const unsigned per = (unsigned)((size_t)fill * p.row_bytes / sizeof(U));
-  for (int h = 0; h < p.heads; ++h) {
+  const size_t plane = (size_t)blockIdx.y * p.plane_stride;
+  const char *from = p.arena + plane + (size_t)src * p.page_stride;
+  char *to = p.arena + plane + (size_t)dst * p.page_stride;
+  const int n = (int)((size_t)fill * p.row_bytes / sizeof(U));   // units of a run
+  const int pieces = (n + 32 * kDeep - 1) / (32 * kDeep);
+  const int lane = threadIdx.x & 31;
+  for (int k = threadIdx.x >> 5; k < pieces * p.heads; k += kCopyWarps) {
+    const int h = k / pieces, first = (k - h * pieces) * 32 * kDeep + lane;
     const U *f = reinterpret_cast<const U *>(from + (size_t)h * p.run_stride);
     U *t = reinterpret_cast<U *>(to + (size_t)h * p.run_stride);
-#pragma unroll 4
-    for (unsigned u = threadIdx.x; u < per; u += blockDim.x) t[u] = f[u];
+    U v[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+      if (first + d * 32 < n) v[d] = f[first + d * 32];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+      if (first + d * 32 < n) t[first + d * 32] = v[d];
   }
 }
 
@@ -239,10 +382,10 @@ extern "C" int tllm_page_copy(void *arena, long plane_stride, int planes, long p
                              run_stride | row_bytes;
   const dim3 grid(n_copies, planes);
   if (bits % 16 == 0)
-    TLLM_CUDA(launch_pdl(page_copy_kernel<uint4>, grid, dim3(256), 0, st, p));
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint4>, grid, dim3(kCopyWarps * 32), 0, st, p));
   else if (bits % 4 == 0)
-    TLLM_CUDA(launch_pdl(page_copy_kernel<uint32_t>, grid, dim3(256), 0, st, p));
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint32_t>, grid, dim3(kCopyWarps * 32), 0, st, p));
   else
-    TLLM_CUDA(launch_pdl(page_copy_kernel<uint8_t>, grid, dim3(256), 0, st, p));
+    TLLM_CUDA(launch_pdl(page_copy_kernel<uint8_t>, grid, dim3(kCopyWarps * 32), 0, st, p));
   return TLLM_OK;
 }
