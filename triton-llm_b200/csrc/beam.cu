@@ -62,22 +62,29 @@ struct BeamParams {
 };
 
 // A bound that at least k keys of the CTA reach, from every thread's largest
-// key `best`: the k-th largest of a warp's 32 (the best of the eight warps'),
-// or for k > 32 the least of the warps' ceil(k / 8)-th largest.
+// key `best`: the least of the nth largest of a warp's 32, found in nth rounds
+// of warp maxima over the values; equal values give up their lowest lane
+// first, and the bound carries the highest index among the lanes taken with
+// its value. For k <= 32, nth = k and the CTA takes the best of the warps'
+// bounds; beyond, nth = ceil(k / 8) of every warp and the least of them.
 __device__ __forceinline__ uint64_t key_bound(uint64_t best, int k, uint64_t *s_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // bitonic sort of the warp's keys, largest first
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      const uint64_t other = __shfl_xor_sync(~0u, best, d);
-      const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
-      best = (other > best) == larger ? other : best;
-    }
   const int nth = k <= 32 ? k : (k + kBeamWarps - 1) / kBeamWarps;
-  best = __shfl_sync(~0u, best, nth - 1);
-  if (lane == 0) s_warp[warp] = best;
+  const uint32_t value = (uint32_t)(best >> 32);
+  uint32_t left = value, top = 0;
+  bool taken = false;
+  for (int i = 0; i < nth; ++i) {
+    top = __reduce_max_sync(~0u, left);
+    const int first = __ffs(__ballot_sync(~0u, left == top && !taken)) - 1;
+    if (lane == first) {
+      taken = true;
+      left = 0;
+    }
+    if (top == 0) break;   // fewer than nth keys: no bound
+  }
+  const uint32_t index =
+      __reduce_max_sync(~0u, taken && value == top ? key_index(best) : 0u);
+  if (lane == 0) s_warp[warp] = top ? ((uint64_t)top << 32) | (uint32_t)~index : 0;
   __syncthreads();
   uint64_t bound = s_warp[0];
 #pragma unroll
@@ -111,6 +118,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
   __shared__ int s_n, s_last;
   __shared__ float s_base[kMaxBeams], s_lse[kMaxBeams];
+  __shared__ int s_done[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = p.k;
@@ -125,7 +133,6 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
     };
     const int left = p.vocab - t0;
     float v[kPerLane];
-    bool nan = false;
     if constexpr (kVec) {
 #pragma unroll
       for (int i = 0; i < kPerLane; i += 4) {
@@ -152,7 +159,6 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
     int at = 0;      // the first largest
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      nan |= v[i] != v[i];
       if (v[i] > m) {
         m = v[i];
         at = index(i);
@@ -162,11 +168,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
     const uint64_t best = at < left ? rank_key(m, (uint32_t)(t0 + at)) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if (__any_sync(~0u, nan)) m = NAN;
+    // (a NaN anywhere, or +inf, makes the sum NaN; -inf alone leaves it 0)
+    const float zero = m == -INFINITY ? 0.f : m;
     float s = 0.f;
-    if (m != -INFINITY)
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) s += fast_exp2((v[i] - m) * kLog2e);
+    for (int i = 0; i < kPerLane; ++i) s += fast_exp2((v[i] - zero) * kLog2e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane == 0) {
@@ -188,14 +194,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
     for (int i = n + tid; i < k; i += kBeamThreads) list[i] = 0;   // a short last chunk
     if (tid == 0) {
       float mm = -INFINITY, ss = 0.f;
-      bool bad = false;
-      for (int w = 0; w < kBeamWarps; ++w) {
-        bad |= s_m[w] != s_m[w];
-        mm = fmaxf(mm, s_m[w]);
-      }
+#pragma unroll
+      for (int w = 0; w < kBeamWarps; ++w) mm = fmaxf(mm, s_m[w]);
+#pragma unroll
       for (int w = 0; w < kBeamWarps; ++w)
-        if (s_m[w] != -INFINITY) ss += s_s[w] * fast_exp2((s_m[w] - mm) * kLog2e);
-      p.stats[(size_t)row * p.chunks + chunk] = make_float2(bad ? NAN : mm, ss);
+        ss += s_m[w] == -INFINITY ? s_s[w] : s_s[w] * fast_exp2((s_m[w] - mm) * kLog2e);
+      p.stats[(size_t)row * p.chunks + chunk] = make_float2(mm, ss);
     }
   }
   __threadfence();
@@ -210,49 +214,50 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
   if (!s_last) return;
   __threadfence();
 
-  // ---- the last CTA of the group: the rows' logsumexp, then the k best
+  // ---- the last CTA of the group: the rows' logsumexp, then the k best.
+  // The first batch of candidates is loaded beside the statistics.
+  const int per = p.chunks * k, n = p.beams * per;
+  const uint64_t *lists = p.lists + (size_t)group * n;
+  uint64_t key[kBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kBeamThreads + tid;
+      key[j] = i < n ? __ldcg(lists + i) : 0;
+    }
+  };
+  load(0);
   for (int b = warp; b < p.beams; b += kBeamWarps) {
     const int r = group * p.beams + b;
-    float mm = -INFINITY, ss = 0.f;
-    if (!(p.done && p.done[r])) {
-      const float2 *stats = p.stats + (size_t)r * p.chunks;
-      const float2 own = lane < p.chunks ? __ldcg(stats + lane) : make_float2(-INFINITY, 0.f);
-      bool bad = own.x != own.x;
-      mm = own.x;
-      for (int c = lane + 32; c < p.chunks; c += 32) {
-        const float m = __ldcg(stats + c).x;
-        bad |= m != m;
-        mm = fmaxf(mm, m);
-      }
+    const bool done = p.done && p.done[r];
+    const float base = p.scores[r];
+    const float2 *stats = p.stats + (size_t)r * p.chunks;
+    const float2 own = !done && lane < p.chunks ? __ldcg(stats + lane)
+                                                : make_float2(-INFINITY, 0.f);
+    float mm = own.x, ss = 0.f;
+    if (!done)
+      for (int c = lane + 32; c < p.chunks; c += 32) mm = fmaxf(mm, __ldcg(stats + c).x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
-      if (__any_sync(~0u, bad)) mm = NAN;
-      if (own.x != -INFINITY) ss = own.y * expf(own.x - mm);
-      for (int c = lane + 32; c < p.chunks; c += 32) {
-        const float2 st = __ldcg(stats + c);
-        if (st.x != -INFINITY) ss += st.y * expf(st.x - mm);
-      }
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+    auto add = [&](float2 st) { ss += st.x == -INFINITY ? st.y : st.y * expf(st.x - mm); };
+    add(own);
+    if (!done)
+      for (int c = lane + 32; c < p.chunks; c += 32) add(__ldcg(stats + c));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-    }
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
     if (lane == 0) {
-      s_base[b] = p.scores[r];
+      s_done[b] = done;
+      s_base[b] = base;
       s_lse[b] = mm + logf(ss);
     }
   }
   __syncthreads();
   // candidates in batches of kBatch per thread beside the best of those before
-  const int per = p.chunks * k, n = p.beams * per;
   int kept = 0;
   for (int i0 = 0; i0 < n; i0 += kBatch * kBeamThreads) {
-    uint64_t key[kBatch], best = tid < kept ? s_top[tid] : 0;
+    if (i0 > 0) load(i0);
+    uint64_t best = tid < kept ? s_top[tid] : 0;
     const uint64_t old = best;
-    // (the loads of a batch are in flight together)
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int i = i0 + j * kBeamThreads + tid;
-      key[j] = i < n ? __ldcg(&p.lists[(size_t)group * n + i]) : 0;
-    }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int i = i0 + j * kBeamThreads + tid;
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
         float score = -INFINITY;
         uint32_t token = c;
         bool is = true;
-        if (p.done && p.done[group * p.beams + b]) {
+        if (s_done[b]) {
           // the pad token, then others at -inf in order
           is = c < k;
           token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
@@ -312,7 +317,9 @@ int list_size(int k) {
 }
 
 // --------------------------------------------------------------------------
-// Reordering: one CTA per group, one thread per table column.
+// Reordering: one CTA per group, one thread per table column, which holds the
+// column's entries of all beams (so the tables can change in place). Every
+// warp works out the beams' parents by itself; no barriers.
 // --------------------------------------------------------------------------
 struct ReorderParams {
   const int *parents, *lens, *table_in;
@@ -322,62 +329,59 @@ struct ReorderParams {
   int *err;
 };
 
-__global__ void beam_reorder_kernel(const ReorderParams p) {
+template <int kBeams>   // at least p.beams
+__global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderParams p) {
   griddep_launch();
   griddep_wait();
-  __shared__ int s_parent[kMaxBeams], s_target[kMaxBeams], s_ok;
-  const int g = blockIdx.x, W = p.beams, tid = threadIdx.x;
-  const size_t row0 = (size_t)g * W;
+  __shared__ int s_ends[8][32];
+  const int W = p.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const size_t row0 = (size_t)blockIdx.x * W;
   const int len = p.lens[row0];
+  const int up = lane < W ? p.parents[row0 + lane] : 0;
   const int c = len / p.page_size, f = len - c * p.page_size;
-  if (tid < 32) {
-    const int up = tid < W ? p.parents[row0 + tid] : 0;
-    const bool good = up >= 0 && up < W && len >= 0 && (f > 0 ? c < p.cols : c <= p.cols);
-    const bool ok = __all_sync(~0u, good);
-    // first children keep their parent's page, in order the others take those
-    // of the beams without a child
-    uint32_t parents_seen = 0;   // beams that have a child
-    for (int i = 0; i < W; ++i) parents_seen |= 1u << (__shfl_sync(~0u, up, i) & 31);
-    bool first = tid < W;
-    for (int i = 0; i < W; ++i) {
-      const int other = __shfl_sync(~0u, up, i);
-      if (i < tid && other == up) first = false;
-    }
-    const uint32_t extra = __ballot_sync(~0u, tid < W && !first);
-    const uint32_t all = W == 32 ? ~0u : (1u << W) - 1;
-    const uint32_t ends = all & ~parents_seen;
-    int target = up;
-    if (tid < W && !first) {
-      const int nth = __popc(extra & ((1u << tid) - 1));
-      target = __fns(ends, 0, nth + 1);
-    }
-    if (tid < W) {
-      s_parent[tid] = ok ? up : tid;
-      s_target[tid] = ok ? target : tid;
-      int src = -1, dst = -1;
-      if (ok && f > 0) {
-        src = p.table_in[(row0 + up) * p.cols + c];
-        dst = p.table_in[(row0 + target) * p.cols + c];
-      }
-      p.copy_src[row0 + tid] = src;
-      p.copy_dst[row0 + tid] = dst;
-      p.copy_fill[row0 + tid] = ok && f > 0 ? f : 0;
-    }
-    if (tid == 0) {
-      s_ok = ok;
-      if (!ok) atomicOr(p.err, DEV_ERR_PAGE);
-    }
+  const bool ok = __all_sync(~0u, up >= 0 && up < W && len >= 0 &&
+                                      (f > 0 ? c < p.cols : c <= p.cols));
+  // the page of column c: first children keep their parent's, in order the
+  // others take those of the beams without a child
+  const uint32_t same = __match_any_sync(~0u, lane < W ? up : -1 - lane);
+  const bool first = (int)__ffs(same) - 1 == lane;
+  uint32_t parents = lane < W ? 1u << (up & 31) : 0u;
+  parents = __reduce_or_sync(~0u, parents);
+  const uint32_t ends = (W == 32 ? ~0u : (1u << W) - 1) & ~parents;
+  const uint32_t below = (1u << lane) - 1;
+  if (ends >> lane & 1) s_ends[warp][__popc(ends & below)] = lane;
+  __syncwarp();
+  const uint32_t extra = __ballot_sync(~0u, lane < W && !first);
+  const int target = lane < W && !first && ok ? s_ends[warp][__popc(extra & below)] : up;
+
+  if (tid < W && !(ok && f > 0)) {
+    p.copy_src[row0 + tid] = p.copy_dst[row0 + tid] = -1;
+    p.copy_fill[row0 + tid] = 0;
   }
-  __syncthreads();
-  const bool ok = s_ok;
-  for (int j = tid; j < p.cols; j += blockDim.x) {
-    if (p.table_out == p.table_in && (!ok || j > c || (j == c && f == 0))) continue;
-    int v[kMaxBeams];
-    for (int i = 0; i < W; ++i) {
-      const int from = !ok ? i : j < c ? s_parent[i] : j == c && f > 0 ? s_target[i] : i;
-      v[i] = p.table_in[(row0 + from) * p.cols + j];
+  if (tid == 0 && !ok) atomicOr(p.err, DEV_ERR_PAGE);
+  for (int j0 = 0; j0 < p.cols; j0 += blockDim.x) {
+    const int j = j0 + tid;
+    const bool moved = ok && j < c, split = ok && j == c && f > 0;
+    const bool work = j < p.cols && (p.table_out != p.table_in || moved || split);
+    const int *in = p.table_in + row0 * p.cols + j;
+    int v[kBeams], old[kBeams];
+#pragma unroll
+    for (int i = 0; i < kBeams; ++i) {
+      const int u = __shfl_sync(~0u, up, i), t = __shfl_sync(~0u, target, i);
+      if (i >= W || !work) continue;
+      v[i] = in[(size_t)(moved ? u : split ? t : i) * p.cols];
+      if (split) old[i] = in[(size_t)u * p.cols];
     }
-    for (int i = 0; i < W; ++i) p.table_out[(row0 + i) * p.cols + j] = v[i];
+#pragma unroll
+    for (int i = 0; i < kBeams; ++i) {
+      if (i >= W || !work) continue;
+      p.table_out[(row0 + i) * p.cols + j] = v[i];
+      if (split) {
+        p.copy_src[row0 + i] = old[i];
+        p.copy_dst[row0 + i] = v[i];
+        p.copy_fill[row0 + i] = f;
+      }
+    }
   }
 }
 
@@ -476,7 +480,7 @@ extern "C" int tllm_beam_reorder(const int32_t *parents, const int32_t *lens,
   const int threads = table_cols >= 256 ? 256 : (table_cols + 31) / 32 * 32 > 32
                                                     ? (table_cols + 31) / 32 * 32
                                                     : 32;
-  TLLM_CUDA(launch_pdl(beam_reorder_kernel, dim3(groups), dim3(threads), 0,
-                       resolve(stream), p));
+  TLLM_CUDA(launch_pdl(beams <= 8 ? beam_reorder_kernel<8> : beam_reorder_kernel<kMaxBeams>,
+                       dim3(groups), dim3(threads), 0, resolve(stream), p));
   return TLLM_OK;
 }
