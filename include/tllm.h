@@ -283,8 +283,9 @@ typedef struct {
  * device error word). bf16 and fp32 caches; head_dim up to 512 whose rows
  * are whole 16-byte units. Scratch: partial (tllm_paged_attention_workspace;
  * fewer bytes give fewer, longer splits) and counters, zero-filled once and
- * zero again after every call; a call that overlaps another on the GPU needs
- * its own. No counterpart in the reference (its decode attention over the
+ * zero again after every call (but for one that set bit 1 of the device error
+ * word: fill them again); a call that overlaps another on the GPU needs its
+ * own. No counterpart in the reference (its decode attention over the
  * preallocated cache: triton_llm/kernels/attention_gqa.py:149-269).
  */
 int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_head,

@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 constexpr int kStages = 3;
 constexpr int kRowBlock = 512;   // rows that share one axis (and one grid row)
 constexpr int kMaxPerSm = 2;     // CTAs that the shared memory lets an SM hold
+constexpr int kSegs = 2;         // segments announced to the consumers
 constexpr int kMinTiles = 2;     // least tiles of a share
 constexpr int kJoinTiles = 4;    // tiles that a CTA reads in the time of a join
 
@@ -414,8 +415,8 @@ struct Tile {
   static constexpr int BYTES = SUB * SUB_BYTES;    // K or V of a tile: 16 KB
   static constexpr int NCW = 4;                    // consumer warps
   static constexpr int KB = KT / NCW / 16;         // 16-key blocks of a warp
-  static constexpr int THREADS = (NCW + 1) * 32;
-  static constexpr size_t SMEM = 2 * (size_t)kStages * BYTES + 2 * kStages * 8;
+  static constexpr int THREADS = (NCW + 2) * 32;   // a producer warp and a joining one
+  static constexpr size_t SMEM = 2 * (size_t)kStages * BYTES + 2 * (kStages + kSegs + 1) * 8;
 };
 
 // 4-D tiled TMA load, completion on bar.
@@ -482,85 +483,186 @@ __device__ __forceinline__ PageSpan page_span(const AttnParams &p, int len, int 
   return g;
 }
 
-// The tiles of all (row, head group) pairs, in that order, as one axis cut
-// into equal shares, one for each CTA. A pair is a segment of the axis; a
-// share holds the end of one, some whole ones and the start of another.
+// The tiles of all (row, head group) pairs, in that order, are one axis, cut
+// into equal shares, one for each CTA. The part of a pair that lies in one
+// share is a segment: a share holds the end of one pair, some whole ones and
+// the start of another. (Short intervals at the end of the shares, for the CTAs
+// that are done first, balance the SMs' bandwidth, but every further segment
+// costs its CTA about 2 us and its pair's join 0.15 us: 64 x 24/8/128 took 200
+// us with them and 192 without, one row of 131071 keys 93 and 96.)
 struct Segment {
-  int row, y;      // row of this block of rows, head group
-  int nt, t0, t1;  // tiles of the pair, and those of this share
+  int row, y;      // row of this block of rows, head group; row < 0: no more
+  int t0, t1;      // tiles of the pair
+  int first, parts;   // the shares that hold the pair: parts == 1: it is whole
 };
 
 __device__ __forceinline__ void bar_consumers(int threads) {
   asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
 }
+// The same, and whether any of the threads says so.
+__device__ __forceinline__ bool bar_any(int threads, bool say) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, 1, %1, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(threads), "r"((uint32_t)say)
+      : "memory");
+  return r != 0;
+}
 
-// The n parts of one pair joined by NCW consumer warps: part 0 lies in slot
-// base + 1 of the partials, part i > 0 in slot base + 2 i. (Not inlined: its
-// registers would take away from those of the tile loop.)
-template <int D, int NCW>
-__device__ __noinline__ void join_parts(const AttnParams &p, size_t base, int n, int G,
-                                        float *sw, size_t out_row) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  __threadfence();
-  // Loads are issued in batches of kJoin whose count does not depend on
-  // n, the first of them beside those of the statistics: a join of up to
-  // kJoin parts waits for one round trip to L2.
-  constexpr int kJoin = 8;
-  const float4 *acc4 = reinterpret_cast<const float4 *>(p.part_acc);
-  const size_t step = (size_t)p.g_tile * (D / 4);
-  auto load = [&](float4 (&v)[kJoin], int k0, int i) {
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      const int c = min(k0 + k, n - 1);
-      v[k] = __ldcg(acc4 + (base + 2 * c + (c == 0)) * step + i);
-    }
-  };
-  float4 v[kJoin];
-  if (tid < G * (D / 4)) load(v, 0, tid);
-  // sw: [G][n] weights of the parts
-  for (int h = warp; h < G; h += NCW) {
-    auto stats = [&](int i) {
-      return i < n ? __ldcg(reinterpret_cast<const float2 *>(p.part_ml) +
-                            (base + 2 * i + (i == 0)) * p.g_tile + h)
-                   : make_float2(-INFINITY, 0.f);
-    };
-    const float2 ml0 = stats(lane), ml1 = stats(lane + 32);
-    float mx = fmaxf(ml0.x, ml1.x), den = 0.f;
-    for (int i = lane + 64; i < n; i += 32) mx = fmaxf(mx, stats(i).x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
-    auto weigh = [&](int i, float2 ml) {
-      if (i >= n) return;
-      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
-      sw[h * n + i] = f;
-      den = fmaf(ml.y, f, den);
-    };
-    weigh(lane, ml0);
-    weigh(lane + 32, ml1);
-    for (int i = lane + 64; i < n; i += 32) weigh(i, stats(i));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) den += __shfl_xor_sync(~0u, den, d);
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    __syncwarp();
-    for (int i = lane; i < n; i += 32) sw[h * n + i] *= inv;
+// Slot of the partials for a segment: a share may hold the end of one pair and
+// the start of another.
+__device__ __forceinline__ size_t part_slot(size_t share, bool starts) {
+  return share * 2 + starts;
+}
+
+// Waits for a phase of bar, but not after a failure in this CTA; false if the
+// (bounded) wait ran out or there is one.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t phase, volatile int *fail) {
+  for (uint32_t i = 0; i < 1u << 22; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if (*fail) return false;
   }
-  bar_consumers(NCW * 32);
-  for (int i = tid; i < G * (D / 4); i += NCW * 32) {
-    const int h = i / (D / 4);
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < n; k0 += kJoin) {
-      if (i != tid || k0 > 0) load(v, k0, i);
+  return false;
+}
+
+// Maximum and 1 / sum over the n parts of one pair, for head h; by one warp.
+__device__ __forceinline__ void part_stats(const AttnParams &p, size_t base, int n, int h,
+                                           float *top_out, float *inv_out) {
+  const int lane = threadIdx.x & 31;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml);
+  float mx = -INFINITY, den = 0.f;   // of this lane's parts
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const float2 v = __ldcg(ml + part_slot(base + i, i == 0) * p.g_tile + h);
+    const float top = fmaxf(mx, v.x), zero = top == -INFINITY ? 0.f : top;
+    den = den * fast_exp2(mx - zero) + v.y * fast_exp2(v.x - zero);
+    mx = top;
+  }
+  float top = mx;
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k) {
-        if (k0 + k >= n) continue;
-        const float f = sw[h * n + k0 + k];
-        r.x = fmaf(f, v[k].x, r.x);
-        r.y = fmaf(f, v[k].y, r.y);
-        r.z = fmaf(f, v[k].z, r.z);
-        r.w = fmaf(f, v[k].w, r.w);
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  if (mx != -INFINITY) den *= fast_exp2(mx - top);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) den += __shfl_xor_sync(~0u, den, d);
+  *top_out = top;
+  *inv_out = den == 0.f ? 0.f : 1.f / den;
+}
+__device__ __forceinline__ float part_weight(float m, float top, float inv) {
+  return m == -INFINITY ? 0.f : fast_exp2(m - top) * inv;
+}
+
+// The parts of one pair joined by the consumer warps at the end of their CTA;
+// part i lies in share base + i. As many parts as fit the ring, which is free
+// by then, are copied there at once (64 of 3 x 128 values: one round trip to
+// L2, beside that of the statistics) and summed in order. The code is short on
+// purpose: it runs once per CTA, from a cold instruction cache. (Not inlined:
+// its registers would take away from those of the tile loop.)
+template <int D, int THREADS>
+__device__ __noinline__ void join_parts(const AttnParams &p, size_t base, int n, int G,
+                                        float4 *ring, float *s_top, float *s_inv,
+                                        size_t out_row) {
+  constexpr int kWeights = 1024;                              // of 16 bytes, for weights
+  constexpr int kUnits = 2 * kStages * Tile<D>::BYTES / 16 - kWeights;   // and for values
+  constexpr int kMost = 16 * D / 4 / THREADS;                 // columns of a thread
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int cols = G * (D / 4), batch = min(kUnits / cols, 4 * kWeights / G);
+  const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml);
+  const float4 *acc = reinterpret_cast<const float4 *>(p.part_acc);
+  const size_t step = (size_t)p.g_tile * (D / 4);
+  float *s_w = reinterpret_cast<float *>(ring + kUnits);
+  float4 r[kMost];
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += batch) {
+    const int m = min(batch, n - i0);
+    for (int i = tid; i < m * cols; i += THREADS) {
+      const int part = i / cols;
+      const float4 *from =
+          acc + part_slot(base + i0 + part, i0 + part == 0) * step + (i - part * cols);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + i)),
+                   "l"(from)
+                   : "memory");
+    }
+    if (i0 == 0) {
+      for (int h = warp; h < G; h += THREADS / 32) {
+        float top, inv;
+        part_stats(p, base, n, h, &top, &inv);
+        if ((tid & 31) == 0) {
+          s_top[h] = top;
+          s_inv[h] = inv;
+        }
+      }
+      bar_consumers(THREADS);
+    }
+    for (int i = tid; i < m * G; i += THREADS) {
+      const int part = i / G, h = i - part * G;
+      const float x = __ldcg(&ml[part_slot(base + i0 + part, i0 + part == 0) * p.g_tile + h].x);
+      s_w[i] = part_weight(x, s_top[h], s_inv[h]);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    bar_consumers(THREADS);
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      const int col = tid + j * THREADS;
+      if (col >= cols) break;
+      const int h = col / (D / 4);
+#pragma unroll 4
+      for (int k = 0; k < m; ++k) {
+        const float4 v = ring[k * cols + col];
+        const float f = s_w[k * G + h];
+        r[j].x = fmaf(f, v.x, r[j].x);
+        r[j].y = fmaf(f, v.y, r[j].y);
+        r[j].z = fmaf(f, v.z, r[j].z);
+        r[j].w = fmaf(f, v.w, r[j].w);
       }
     }
-    const size_t at = out_row + (size_t)h * p.o_sh + (i - h * (D / 4)) * 4;
+    bar_consumers(THREADS);
+  }
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int col = tid + j * THREADS;
+    if (col >= cols) break;
+    const int h = col / (D / 4);
+    const size_t at = out_row + (size_t)h * p.o_sh + (col - h * (D / 4)) * 4;
+    store_out(p, at, r[j].x);
+    store_out(p, at + 1, r[j].y);
+    store_out(p, at + 2, r[j].z);
+    store_out(p, at + 3, r[j].w);
+  }
+}
+
+// A segment that ended before its CTA's last one, for the joining warp.
+struct Job {
+  size_t base, out_row;   // the pair's first share, its output
+  int first, parts, G;    // parts == 0: no more
+};
+
+// The same sums by one warp, while the others go on with the next segment.
+template <int D>
+__device__ __noinline__ void join_by_warp(const AttnParams &p, const Job &job) {
+  const int lane = threadIdx.x & 31;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml);
+  const float4 *acc = reinterpret_cast<const float4 *>(p.part_acc);
+  for (int h = 0; h < job.G; ++h) {
+    float top, inv;
+    part_stats(p, job.base, job.parts, h, &top, &inv);
+    if (lane >= D / 4) continue;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = 0; i < job.parts; ++i) {
+      const size_t at = part_slot(job.base + i, i == 0) * p.g_tile + h;
+      const float4 v = __ldcg(acc + at * (D / 4) + lane);
+      const float f = part_weight(__ldcg(ml + at).x, top, inv);
+      r.x = fmaf(f, v.x, r.x);
+      r.y = fmaf(f, v.y, r.y);
+      r.z = fmaf(f, v.z, r.z);
+      r.w = fmaf(f, v.w, r.w);
+    }
+    const size_t at = job.out_row + (size_t)h * p.o_sh + lane * 4;
     store_out(p, at, r.x);
     store_out(p, at + 1, r.y);
     store_out(p, at + 2, r.z);
@@ -578,9 +680,13 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   extern __shared__ __align__(1024) uint8_t smem[];   // stages of (K, V)
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + 2 * kStages * T::BYTES);
   uint64_t *empty = full + kStages;
+  uint64_t *seg_full = empty + kStages, *seg_empty = seg_full + kSegs;
+  uint64_t *job_full = seg_empty + kSegs, *job_empty = job_full + 1;
   __shared__ uint32_t s_bad[kStages];                 // bad pages of a stage's tile
+  __shared__ Segment s_seg[kSegs];
+  __shared__ Job s_job;
   __shared__ int s_cum[kRowBlock + 1], s_len[kRowBlock];
-  __shared__ int s_warp[2][NCW + 1], s_last;
+  __shared__ int s_warp[2][NCW + 2], s_last;
   __shared__ volatile int s_fail;
   __shared__ float s_m[NCW][16], s_l[NCW][16];
   const int row0 = blockIdx.y * kRowBlock, nrows = min(kRowBlock, p.rows - row0);
@@ -595,6 +701,12 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], NCW);
     }
+    for (int s = 0; s < kSegs; ++s) {
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], NCW);
+    }
+    mbar_init(job_full, 1);
+    mbar_init(job_empty, 1);
     fence_mbar_init();
     s_fail = 0;
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
@@ -639,7 +751,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   __syncthreads();
   int before = scan - sum, total = 0;
 #pragma unroll
-  for (int w = 0; w <= NCW; ++w) {
+  for (int w = 0; w < NCW + 2; ++w) {
     if (w < warp) before += s_warp[0][w];
     total += s_warp[0][w];
     most = max(most, s_warp[1][w]);
@@ -652,51 +764,14 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   if (tid == 0) s_cum[nrows] = total;
   __syncthreads();
 
-  // ---- this CTA's share [w0, w1) of the axis. Where every pair can have a
-  // CTA of its own and sharing would save less than kJoinTiles, pairs stay
-  // whole: joining the parts costs about as much.
+  // ---- shares. Where every pair can have a CTA of its own and sharing would
+  // save less than kJoinTiles, pairs stay whole: joining costs about as much.
   const int ncta = gridDim.x;
   const long work = (long)total * p.n_y;
   int share = (int)((work + ncta - 1) / ncta);
   if (share < kMinTiles) share = kMinTiles;
   const bool whole_pairs = (long)nrows * p.n_y <= ncta && most <= share + kJoinTiles;
-  long w0 = (long)blockIdx.x * share;
-  const long w1 = min(w0 + share, work);
-  Segment first;
-  if (whole_pairs) {
-    if (blockIdx.x >= nrows * p.n_y) return;
-    first.row = blockIdx.x / p.n_y;
-    first.y = blockIdx.x - first.row * p.n_y;
-    first.nt = s_cum[first.row + 1] - s_cum[first.row];
-    first.t0 = 0;
-    first.t1 = first.nt;
-  } else {
-    if (w0 >= work) return;
-    int lo = 0, hi = nrows;   // s_cum[lo] * n_y <= w0 < s_cum[hi] * n_y
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((long)s_cum[mid] * p.n_y <= w0) lo = mid; else hi = mid;
-    }
-    first.row = lo;
-    first.nt = s_cum[lo + 1] - s_cum[lo];
-    const int rem = (int)(w0 - (long)s_cum[lo] * p.n_y);
-    first.y = rem / first.nt;
-    first.t0 = rem - first.y * first.nt;
-    first.t1 = (int)min((long)first.nt, first.t0 + w1 - w0);
-  }
-  // the segment after g, w = position of its first tile on the axis
-  auto advance = [&](Segment &g, long &w) {
-    w += g.t1 - g.t0;
-    if (whole_pairs || w >= w1) return false;
-    if (++g.y == p.n_y) {
-      g.y = 0;
-      ++g.row;
-      g.nt = s_cum[g.row + 1] - s_cum[g.row];
-    }
-    g.t0 = 0;
-    g.t1 = (int)min((long)g.nt, w1 - w);
-    return true;
-  };
+  const size_t base = (size_t)blockIdx.y * ncta;   // of the shares
   const int P = p.kv.page_size, box = min(P, KT);   // slots of one load
 
   if (warp == NCW) {
@@ -706,10 +781,24 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     const bool mine = is_v < 2;
     const uint32_t dst0 = smem_u32(smem) + (is_v ? T::BYTES : 0) + sub * T::SUB_BYTES +
                           j * box * 128;
-    Segment g = first;
-    int it = 0;        // tiles issued
-    bool more = true, failed = false;
-    while (more && !failed) {
+    int it = 0, segs = 0;   // tiles issued, segments announced
+    bool failed = false;
+    auto announce = [&](const Segment &g) {
+      const int s = segs % kSegs;
+      if (segs >= kSegs && !wait_phase(&seg_empty[s], (segs / kSegs - 1) & 1, &s_fail))
+        failed = true;
+      failed = __any_sync(~0u, failed);
+      if (failed) return;
+      if (lane == 0) {
+        s_seg[s] = g;
+        arrive(&seg_full[s]);
+      }
+      ++segs;
+    };
+    // announces and loads one segment
+    auto stream = [&](const Segment &g) {
+      announce(g);
+      if (failed) return;
       int xs, xa;
       const PageSpan ps = page_span(p, s_len[g.row], &xs, &xa);
       const int seq = p.row_seq ? p.row_seq[row0 + g.row] : row0 + g.row;
@@ -729,12 +818,10 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         next1 = entry(t + 2);
         const uint32_t good = __ballot_sync(~0u, mine && page >= 0);
         const uint32_t bad = __ballot_sync(~0u, lane < pt && page == -2);
-        if (it >= kStages && (s_fail || !mbar_wait_bounded(&empty[s], (it / kStages - 1) & 1)))
+        if (it >= kStages && !wait_phase(&empty[s], (it / kStages - 1) & 1, &s_fail))
           failed = true;
-        if (__any_sync(~0u, failed)) {
-          failed = true;
-          break;
-        }
+        failed = __any_sync(~0u, failed);
+        if (failed) return;
         if (lane == 0) {
           s_bad[s] = bad;
           mbar_expect_tx(&full[s], __popc(good) * box * 128);
@@ -748,8 +835,48 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
                       slots_first ? kvh : slot, slots_first ? slot : kvh, page);
         }
       }
-      more = advance(g, w0);
+    };
+    Segment g;
+    if (whole_pairs) {
+      if (blockIdx.x < nrows * p.n_y) {
+        g.row = blockIdx.x / p.n_y;
+        g.y = blockIdx.x - g.row * p.n_y;
+        g.t0 = 0;
+        g.t1 = s_cum[g.row + 1] - s_cum[g.row];
+        g.parts = 1;
+        stream(g);
+      }
+    } else {
+      long w = (long)blockIdx.x * share;
+      const long w1 = min(w + share, work);
+      int lo = 0, hi = nrows;   // s_cum[lo] * n_y <= w < s_cum[hi] * n_y
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((long)s_cum[mid] * p.n_y <= w) lo = mid; else hi = mid;
+      }
+      g.row = lo;
+      int nt = s_cum[lo + 1] - s_cum[lo];
+      const int rem = (int)(w - (long)s_cum[lo] * p.n_y);
+      g.y = rem / nt;
+      g.t0 = rem - g.y * nt;
+      while (w < w1 && !failed) {
+        g.t1 = (int)min((long)nt, g.t0 + w1 - w);
+        const long begin = w - g.t0;
+        g.first = (int)(begin / share);
+        g.parts = (int)((begin + nt - 1) / share) - g.first + 1;
+        stream(g);
+        w += g.t1 - g.t0;
+        g.t0 = 0;
+        if (++g.y == p.n_y) {
+          g.y = 0;
+          ++g.row;
+          if (g.row < nrows) nt = s_cum[g.row + 1] - s_cum[g.row];
+        }
+      }
     }
+    Segment none;
+    none.row = -1;
+    if (!failed) announce(none);
     if (failed) {
       // let the copies in flight land (bounded) before the CTA exits
       if (lane == 0) {
@@ -763,24 +890,84 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     return;
   }
 
+  auto last_part = [&](int first, int parts) {   // one thread's: takes a ticket
+    int *ticket = p.counters + base + first;
+    __threadfence();   // (of all writes that a barrier has ordered before)
+    const bool last = atomicAdd(ticket, 1) == parts - 1;
+    if (last) *ticket = 0;
+    __threadfence();
+    return last;
+  };
+  if (warp == NCW + 1) {
+    // ---- joining warp
+    for (int jobs = 0;; ++jobs) {
+      if (!__all_sync(~0u, wait_phase(job_full, jobs & 1, &s_fail))) return;
+      const Job job = s_job;
+      __syncwarp();
+      if (lane == 0) arrive(job_empty);
+      if (job.parts == 0) return;
+      bool last = false;
+      if (lane == 0) last = last_part(job.first, job.parts);
+      last = __any_sync(~0u, last);
+      __syncwarp();
+      if (last) join_by_warp<D>(p, job);
+    }
+  }
+
   // ---- consumers. Fragments: rows (keys, or dims of O^T) r0 and r0 + 8,
   // columns (heads) cq and cq + 1 of every block of 8. A wait that runs out
-  // sets s_fail and an error bit; the CTA then goes through its segments
-  // without waiting, so that barriers and tickets stay in step.
+  // sets s_fail and an error bit; the CTA then goes through its segment
+  // without waiting, so that barriers stay in step, and ends.
   const int r0 = lane >> 2, cq = (lane & 3) * 2;
   // ldmatrix rows: K as the A operand, V^T by the transposing load
   const int key0 = warp * KB * 16;   // this warp's first key of a tile
   const int a_key = key0 + ((lane >> 3) & 1) * 8 + (lane & 7), a_dim = (lane >> 4) * 8;
   const int t_key = key0 + (lane >> 4) * 8 + (lane & 7), t_dim = ((lane >> 3) & 1) * 8;
-  Segment g = first;
-  int it = 0;
-  bool more = true;
-  while (more) {
+  // the next segment announced; false on a failure (for all warps or none)
+  int segs = 0;
+  auto next_segment = [&](Segment *g) {
+    const int s = segs % kSegs;
+    const bool told = wait_phase(&seg_full[s], (segs / kSegs) & 1, &s_fail);
+    if (!told) {
+      if (!s_fail) atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+      s_fail = 1;
+    }
+    if (bar_any(NCW * 32, !told)) return false;
+    *g = s_seg[s];
+    ++segs;
+    return true;
+  };
+  struct Heads { int head0, G; };
+  auto heads_of = [&](const Segment &g) {
+    const int kvh = g.y / p.n_gsub, gofs = (g.y - kvh * p.n_gsub) * p.g_tile;
+    return Heads{kvh * p.group + gofs, min(p.g_tile, p.group - gofs)};
+  };
+  float2 qv[QB][D / 16][2];   // q of the segment that comes next
+  auto load_q = [&](const Segment &g) {
+    const Heads hd = heads_of(g);
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const float *q = p.q + (size_t)(row0 + g.row) * p.q_sr +
+                       (size_t)(hd.head0 + qb * 8 + r0) * p.q_sh + cq;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+          qv[qb][kk][f] = qb * 8 + r0 < hd.G
+                              ? *reinterpret_cast<const float2 *>(q + kk * 16 + 8 * f)
+                              : make_float2(0.f, 0.f);
+    }
+  };
+  int it = 0, jobs = 0;
+  Segment g;
+  if (!next_segment(&g)) return;
+  if (QB == 1 && g.row >= 0) load_q(g);
+  while (g.row >= 0) {
+    if (QB > 1) load_q(g);
     const int row = row0 + g.row;
     int xs, xa;
     const PageSpan ps = page_span(p, s_len[g.row], &xs, &xa);
-    const int kvh = g.y / p.n_gsub, gofs = (g.y - kvh * p.n_gsub) * p.g_tile;
-    const int G = min(p.g_tile, p.group - gofs), head0 = kvh * p.group + gofs;
+    const int head0 = heads_of(g).head0, G = heads_of(g).G;
     const int sink_keys = ps.sink_pages * P;
     float o[QB][D / 16][4], m_r[QB][2], l_r[QB][2];
     uint32_t qf[QB][D / 16][2][3];
@@ -793,20 +980,14 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[qb][kk][e] = 0.f;
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          float2 v = make_float2(0.f, 0.f);
-          if (qb * 8 + r0 < G)
-            v = *reinterpret_cast<const float2 *>(p.q + (size_t)row * p.q_sr +
-                                                  (size_t)(head0 + qb * 8 + r0) * p.q_sh +
-                                                  kk * 16 + cq + 8 * f);
-          split3(v.x * p.qscale, v.y * p.qscale, qf[qb][kk][f]);
-        }
+        for (int f = 0; f < 2; ++f)
+          split3(qv[qb][kk][f].x * p.qscale, qv[qb][kk][f].y * p.qscale, qf[qb][kk][f]);
       }
     }
 
     for (int t = g.t0; t < g.t1; ++t, ++it) {
       const int s = it % kStages;
-      const bool ok = !s_fail && mbar_wait_bounded(&full[s], (it / kStages) & 1);
+      const bool ok = wait_phase(&full[s], (it / kStages) & 1, &s_fail);
       if (!__all_sync(~0u, ok)) {
         if (lane == 0 && !s_fail) atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
         s_fail = 1;
@@ -949,10 +1130,13 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     }
 
     // ---- join the warps through the last stage's 32 KB, which the producer
-    // gets back afterwards; it loads the next segment's tiles meanwhile
+    // gets back afterwards; it loads the next segment's tiles meanwhile, and
+    // its q is on the way
     const int held = (it - 1) % kStages;
+    Segment next;
+    if (!next_segment(&next)) return;   // (a barrier: all have read the stage)
+    if (QB == 1 && next.row >= 0) load_q(next);   // (two blocks take too many registers)
     float *w_acc = reinterpret_cast<float *>(smem + held * 2 * T::BYTES);   // [NCW][G][D]
-    bar_consumers(NCW * 32);   // all have read the stage
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -973,12 +1157,9 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         }
       }
     bar_consumers(NCW * 32);
-    const bool part = g.t0 > 0 || g.t1 < g.nt;
+    const bool part = g.parts > 1;
     const size_t out_row = (size_t)row * p.o_sr + (size_t)head0 * p.o_sh;
-    const long begin = w0 - g.t0;   // of the pair on the axis
-    const size_t cta = (size_t)blockIdx.y * ncta + blockIdx.x;
-    float *mine = p.part_acc + (cta * 2 + (g.t0 == 0)) * p.g_tile * D;
-    float *mine_ml = p.part_ml + (cta * 2 + (g.t0 == 0)) * p.g_tile * 2;
+    const size_t mine = part_slot(base + blockIdx.x, g.t0 == 0) * p.g_tile;
     for (int i = tid; i < G * D; i += NCW * 32) {
       const int h = i / D;
       float mx = -INFINITY;
@@ -996,35 +1177,46 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
       if (!part) {
         store_out(p, out_row + (size_t)h * p.o_sh + (i - h * D), den == 0.f ? 0.f : num / den);
       } else {
-        mine[i] = num;
+        p.part_acc[mine * D + i] = num;
         if (i == h * D) {
-          mine_ml[h * 2] = mx;
-          mine_ml[h * 2 + 1] = den;
+          p.part_ml[(mine + h) * 2] = mx;
+          p.part_ml[(mine + h) * 2 + 1] = den;
         }
       }
     }
     if (part) {
-      // parts of a pair lie in the second slot of the CTA that starts it and
-      // the first slots of those after it; the last one to finish joins them
-      const int c0 = (int)(begin / share), c1 = (int)((begin + g.nt - 1) / share);
-      const int n = c1 - c0 + 1;
-      __threadfence();
+      // the CTA that finishes a pair's last part joins them all: the joining
+      // warp, or at the end of the share all consumers
       bar_consumers(NCW * 32);
-      if (tid == 0) {
-        int *ctr = p.counters + (size_t)blockIdx.y * ncta + c0;
-        s_last = atomicAdd(ctr, 1) == n - 1;
-        if (s_last) *ctr = 0;   // all other parts took their ticket
-      }
-      bar_consumers(NCW * 32);
-      if (s_last) {
-        const size_t base = ((size_t)blockIdx.y * ncta + c0) * 2;
-        join_parts<D, NCW>(p, base, n, G, w_acc, out_row);
+      if (next.row >= 0) {
+        if (tid == 0) {
+          if (jobs > 0 && !wait_phase(job_empty, (jobs - 1) & 1, &s_fail)) s_fail = 1;
+          s_job = Job{base + g.first, out_row, g.first, g.parts, G};
+          arrive(job_full);
+        }
+        ++jobs;
+      } else {
+        if (tid == 0) s_last = last_part(g.first, g.parts);
+        bar_consumers(NCW * 32);
+        if (s_last)
+          join_parts<D, NCW * 32>(p, base + g.first, g.parts, G,
+                                  reinterpret_cast<float4 *>(smem), s_m[0], s_l[0], out_row);
       }
     }
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) arrive(&empty[held]);
-    more = advance(g, w0);
+    if (next.row >= 0) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        arrive(&empty[held]);
+        arrive(&seg_empty[(segs - 2) % kSegs]);
+      }
+    }
+    g = next;
+  }
+  if (tid == 0) {
+    if (jobs > 0 && !wait_phase(job_empty, (jobs - 1) & 1, &s_fail)) s_fail = 1;
+    s_job.parts = 0;
+    arrive(job_full);
   }
 }
 
@@ -1175,18 +1367,20 @@ extern "C" int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_hea
                  n_head, n_kv_head);
   // One token per row and split (heads of a KV head padded to a tile of 1, 2, 4
   // or 8): splits that fill the GPU a few times over, at least 8. Or two parts
-  // of up to 16 heads per CTA and block of rows of the tensor-core kernel.
+  // of up to 16 heads per share of the tensor-core kernel.
   long splits = 8192 / ((long)(rows > 0 ? rows : 1) * n_kv_head);
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 8) splits = 8;
   const size_t row = (head_dim + 2) * sizeof(float);
-  const size_t ctas = (size_t)(rows + kRowBlock - 1) / kRowBlock * kMaxPerSm * sm_count();
+  const size_t blocks = (size_t)(rows + kRowBlock - 1) / kRowBlock;
+  const size_t ctas = (size_t)kMaxPerSm * sm_count();
   const int group = n_head / n_kv_head;
   const size_t a = (size_t)rows * n_head * 2 * splits * row;
-  const size_t b = ctas * 2 * (group < 16 ? group : 16) * row;
+  const size_t b = blocks * ctas * 2 * (group < 16 ? group : 16) * row;
   *partial_bytes = a > b ? a : b;
   const size_t c = (size_t)rows * n_head;
-  *counter_bytes = (c > ctas ? c : ctas) * sizeof(int32_t);
+  const size_t d = blocks * ctas;
+  *counter_bytes = (c > d ? c : d) * sizeof(int32_t);
   return TLLM_OK;
 }
 
@@ -1275,7 +1469,7 @@ extern "C" int tllm_paged_attention(
     one = (size_t)blocks * 2 * g_tile * (D + 2) * sizeof(float);
     if (ctas > 1 && one * ctas > partial_bytes) ctas = partial_bytes / one;
     if (ctas < 1) ctas = 1;
-    count = ctas > 1 ? blocks * ctas : 0;
+    count = ctas > 1 ? blocks * ctas : 0;   // (one CTA takes all pairs whole)
   } else {
     chunk = plan_chunk(tile, rows, n_y, keys, most, 4L * sm_count());
     splits = most > 0 ? (most + chunk - 1) / chunk : 1;
