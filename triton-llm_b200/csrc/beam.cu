@@ -4,15 +4,16 @@
 //
 // Selection: candidate (b, t) of a group scores s_b + (x_bt - L_b) with
 // L_b = max + log sum exp(x_bt - max). Within a beam the order is that of its
-// logits, so a CTA that reads a chunk of one row needs to keep only the
-// chunk's max, its sum of exponentials and its k largest logits; the last CTA
-// of a group to finish joins them. Each logit is read once.
+// logits, so a CTA that reads a part of one row needs to keep only the part's
+// max, its sum of exponentials and its k largest logits; the last CTA of a
+// group to finish joins them. Each logit is read once.
 //
-// The k largest of a CTA's values: the k-th largest of any set of at least k
-// of them is a bound that the k largest reach. With the threads' own maxima as
-// that set the bound leaves few values over, which go to shared memory and are
-// ranked by counting. Values carry their index in a 64-bit code, so all are
-// distinct and ties are in order.
+// Values carry their index in a 64-bit code, so all are distinct and ties are
+// in order. A warp reads 512 values at a time, the next 512 on the way, and
+// lists those above the best bound that a warp of the CTA has found so far (a
+// key that k others reach, so the k largest do too); after the first steps
+// hardly any is, and a value costs a maximum, an exponential and a share of a
+// comparison. Warps meet once, at the end of their part.
 #include <cmath>
 
 #include "mma_sync.cuh"
@@ -25,8 +26,10 @@ constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kBeamWarps = 8;
 constexpr int kBeamThreads = kBeamWarps * 32;
-constexpr int kPerLane = 16;                          // logits of a thread
-constexpr int kChunk = kBeamThreads * kPerLane;       // logits of a CTA
+constexpr int kPerLane = 16;                          // logits of a lane in one step
+constexpr int kStep = kBeamThreads * kPerLane;        // logits of a CTA in one step
+constexpr int kListed = 128;                          // keys of a warp's list, >= kMaxK + 32
+constexpr int kCtasPerSm = 4;                         // parts are cut for so many
 constexpr int kBatch = 8;                             // listed candidates of a thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxRows = 65535;
@@ -53,44 +56,93 @@ struct BeamParams {
   long ld;
   const float *scores;
   const int *done;
-  int pad, groups, beams, vocab, k, chunks;
+  int pad, groups, beams, vocab, k;
+  int chunks, chunk;    // parts of a row, their logits (whole steps)
   float *out_scores;
   int *out_parents, *out_tokens;
   int *counters;        // (groups)
-  float2 *stats;        // (rows, chunks): max, sum
+  float2 *stats;        // (rows, chunks): max, sum of exponentials
   uint64_t *lists;      // (rows, chunks, k)
 };
 
-// A bound that at least k keys of the CTA reach, from every thread's largest
-// key `best`: the least of the nth largest of a warp's 32, found in nth rounds
-// of warp maxima over the values; equal values give up their lowest lane
-// first, and the bound carries the highest index among the lanes taken with
-// its value. For k <= 32, nth = k and the CTA takes the best of the warps'
-// bounds; beyond, nth = ceil(k / 8) of every warp and the least of them.
-__device__ __forceinline__ uint64_t key_bound(uint64_t best, int k, uint64_t *s_warp) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int nth = k <= 32 ? k : (k + kBeamWarps - 1) / kBeamWarps;
+// A key that at least nth lanes' `best` reach: nth rounds of warp maxima over
+// the values; equal values give up their lowest lane first, and the bound
+// carries the highest index among the lanes taken with its value. 0 if fewer
+// lanes have a key.
+__device__ __forceinline__ uint64_t warp_bound(uint64_t best, int nth) {
+  const int lane = threadIdx.x & 31;
   const uint32_t value = (uint32_t)(best >> 32);
   uint32_t left = value, top = 0;
   bool taken = false;
   for (int i = 0; i < nth; ++i) {
     top = __reduce_max_sync(~0u, left);
-    const int first = __ffs(__ballot_sync(~0u, left == top && !taken)) - 1;
+    if (top == 0) return 0;
+    const int first = __ffs(__ballot_sync(~0u, left == top)) - 1;
     if (lane == first) {
       taken = true;
       left = 0;
     }
-    if (top == 0) break;   // fewer than nth keys: no bound
   }
   const uint32_t index =
       __reduce_max_sync(~0u, taken && value == top ? key_index(best) : 0u);
-  if (lane == 0) s_warp[warp] = top ? ((uint64_t)top << 32) | (uint32_t)~index : 0;
+  return ((uint64_t)top << 32) | (uint32_t)~index;
+}
+
+// A bound that at least k keys of the CTA reach, from every thread's largest:
+// for k <= 32 the best of the warps' k-th largest, beyond that the least of
+// their ceil(k / 8)-th largest.
+__device__ __forceinline__ uint64_t block_bound(uint64_t best, int k, uint64_t *s_warp) {
+  const uint64_t mine = warp_bound(best, k <= 32 ? k : (k + kBeamWarps - 1) / kBeamWarps);
+  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = mine;
   __syncthreads();
   uint64_t bound = s_warp[0];
 #pragma unroll
   for (int w = 1; w < kBeamWarps; ++w)
     bound = (s_warp[w] > bound) == (k <= 32) ? s_warp[w] : bound;
   return bound;
+}
+
+// A warp's list of keys in shared memory, n of them, cut down to its k largest
+// in order: every key goes to the place that the number of larger ones gives.
+// All lanes; returns the new n.
+template <int kSlots>
+__device__ __forceinline__ void cut_slots(uint64_t *list, int n, int k) {
+  const int lane = threadIdx.x & 31;
+  uint64_t key[kSlots];
+  int rank[kSlots] = {};
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q) key[q] = q * 32 + lane < n ? list[q * 32 + lane] : 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = list[j];
+#pragma unroll
+    for (int q = 0; q < kSlots; ++q) rank[q] += other > key[q];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q)
+    if (key[q] && rank[q] < k) list[rank[q]] = key[q];
+}
+__device__ __noinline__ int cut_list(uint64_t *list, int n, int k) {
+  __syncwarp();
+  if (n <= 32)
+    cut_slots<1>(list, n, k);
+  else
+    cut_slots<kListed / 32>(list, n, k);
+  __syncwarp();
+  return min(n, k);
+}
+
+// Number of keys larger than `key` in the warps' lists.
+__device__ __forceinline__ int rank_of(const uint64_t *lists, const int *counts, uint64_t key) {
+  int rank = 0;
+  for (int w = 0; w < kBeamWarps; ++w) {
+    const uint64_t *other = lists + w * kListed;
+    const int n = counts[w];
+#pragma unroll 4
+    for (int q = 0; q < n; ++q) rank += other[q] > key;
+  }
+  return rank;
 }
 
 __device__ __forceinline__ void keep(uint64_t key, uint64_t *list, int *n) {
@@ -110,96 +162,206 @@ __device__ __forceinline__ void rank_keys(const uint64_t *list, int n, int k, F 
 }
 
 template <bool kVec>
-__global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
+    beam_select_kernel(const BeamParams p) {
   griddep_launch();
   griddep_wait();
-  extern __shared__ __align__(16) uint64_t s_list[];
+  constexpr int kKeys = kBatch * kBeamThreads + kMaxK;
+  static_assert(kBeamWarps * kListed <= kKeys, "the warps' lists use the same memory");
+  __shared__ uint64_t s_list[kKeys];
   __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
+  __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
-  __shared__ int s_n, s_last;
+  __shared__ int s_n, s_count[kBeamWarps], s_last;
   __shared__ float s_base[kMaxBeams], s_lse[kMaxBeams];
   __shared__ int s_done[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = p.k;
-  if (tid == 0) s_n = 0;
 
   if (!(p.done && p.done[row])) {
     const float *x = p.logits + (size_t)row * p.ld;
-    const int t0 = chunk * kChunk;
-    // value i of this thread: token t0 + index(i), ascending in i
-    auto index = [&](int i) {
-      return kVec ? (i >> 2) * 4 * kBeamThreads + 4 * tid + (i & 3) : i * kBeamThreads + tid;
+    const int end = min(p.vocab, (chunk + 1) * p.chunk);
+    // value i of this lane in a step: token t0 + at(i), ascending in i
+    auto at = [&](int i) {
+      return kVec ? (i >> 2) * 128 + 4 * lane + (i & 3) : i * 32 + lane;
     };
-    const int left = p.vocab - t0;
-    float v[kPerLane];
-    if constexpr (kVec) {
+    auto load = [&](int t0, float (&v)[kPerLane]) {
+      if (kVec && t0 + 32 * kPerLane <= end) {
 #pragma unroll
-      for (int i = 0; i < kPerLane; i += 4) {
-        const int at = index(i);
-        float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (at + 3 < left) {
-          f = __ldcs(reinterpret_cast<const float4 *>(x + t0 + at));
-        } else {
-          if (at < left) f.x = x[t0 + at];
-          if (at + 1 < left) f.y = x[t0 + at + 1];
-          if (at + 2 < left) f.z = x[t0 + at + 2];
+        for (int i = 0; i < kPerLane; i += 4) {
+          const float4 f = __ldcs(reinterpret_cast<const float4 *>(x + t0 + at(i)));
+          v[i] = f.x;
+          v[i + 1] = f.y;
+          v[i + 2] = f.z;
+          v[i + 3] = f.w;
         }
-        v[i] = f.x;
-        v[i + 1] = f.y;
-        v[i + 2] = f.z;
-        v[i + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+          v[i] = t0 + at(i) < end ? __ldcs(x + t0 + at(i)) : -INFINITY;
       }
-    } else {
+    };
+    uint64_t *list = s_list + warp * kListed;
+    int n = 0;
+    uint64_t bound = 0;      // keys below it are out
+    float least = -INFINITY; // its value
+    float m = -INFINITY, s = 0.f;   // of this lane's values
+    int t0 = chunk * p.chunk + warp * 32 * kPerLane;
+    auto raise = [&](uint64_t to) {
+      bound = to;
+      least = key_value(to);
+      if (lane == 0) atomicMax(&s_bound, to);
+    };
+    auto follow = [&]() {   // the best bound of the CTA's warps
+      const uint64_t others = *(volatile unsigned long long *)&s_bound;
+      if (others > bound) {
+        bound = others;
+        least = key_value(others);
+      }
+    };
+    // lists the values that reach the bound
+    auto scan = [&](const float (&v)[kPerLane], float top) {
+      if (!__any_sync(~0u, top >= least)) return;
+      uint32_t hits = 0;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i)
-        v[i] = index(i) < left ? __ldcs(x + t0 + index(i)) : -INFINITY;
-    }
-    float m = -INFINITY;
-    int at = 0;      // the first largest
+        if (v[i] >= least) hits |= 1u << i;
+      if (n + (int)__reduce_add_sync(~0u, __popc(hits)) <= kListed) {
+        int *count = &s_count[warp];
+        if (lane == 0) *count = n;
+        __syncwarp();
+        auto add = [&](float x, int i) {
+          const uint64_t key = rank_key(x, (uint32_t)(t0 + at(i)));
+          if (key >= bound && t0 + at(i) < end) list[atomicAdd(count, 1)] = key;
+        };
+        if (__any_sync(~0u, hits & (hits - 1))) {
+          if (hits) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      if (v[i] > m) {
-        m = v[i];
-        at = index(i);
+            for (int i = 0; i < kPerLane; ++i)
+              if (hits >> i & 1) add(v[i], i);
+          }
+        } else if (hits) {
+          add(top, __ffs(hits) - 1);   // a lane's only one is its largest
+        }
+        __syncwarp();
+        n = *count;
+        __syncwarp();
+      } else {
+        // long runs of equal or rising values: in order, cutting the list
+        for (int i = 0; i < kPerLane; ++i) {
+          const int t = t0 + at(i);
+          uint64_t key = 0;
+          if (hits >> i & 1 && t < end) {
+            float x = 0.f;   // v[i], without a copy of v in memory
+#pragma unroll
+            for (int j = 0; j < kPerLane; ++j) x = j == i ? v[j] : x;
+            key = rank_key(x, (uint32_t)t);
+          }
+          uint32_t in = __ballot_sync(~0u, key && key >= bound);
+          if (!in) continue;
+          if (n + __popc(in) > kListed) {
+            n = cut_list(list, n, k);
+            // (a full list holds more than k; its k-th itself is listed)
+            if (list[k - 1] >= bound) raise(list[k - 1]);
+            in = __ballot_sync(~0u, key && key >= bound && key != list[k - 1]);
+          }
+          if (in >> lane & 1) list[n + __popc(in & ((1u << lane) - 1))] = key;
+          n += __popc(in);
+        }
+      }
+      // a tighter bound once the list has grown
+      if (n >= 2 * k && n > 20) {
+        n = cut_list(list, n, k);
+        if (list[k - 1] > bound) raise(list[k - 1]);
+      }
+    };
+    // maximum and sum of exponentials; returns the largest of v
+    auto sum_up = [&](const float (&v)[kPerLane]) {
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, v[i]);
+      // (a NaN anywhere, or +inf, makes the sum NaN; -inf alone leaves it 0)
+      const float mn = fmaxf(m, top), zero = mn == -INFINITY ? 0.f : mn * kLog2e;
+      float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2(fmaf(v[i], kLog2e, -zero));
+      s = s * fast_exp2(fmaf(m, kLog2e, -zero)) + ((add[0] + add[1]) + (add[2] + add[3]));
+      m = mn;
+      return top;
+    };
+    // two steps' values are in registers, one in use and one on the way
+    float va[kPerLane], vb[kPerLane];
+    load(t0, va);
+    load(t0 + kStep, vb);
+    if (tid == 0) s_bound = 0;
+    __syncthreads();
+    {
+      // the first step: k lanes' own maxima bound the k largest; all warps'
+      // bounds, then the k-th largest of what they have listed
+      const float top = sum_up(va);
+      int first = 0;
+#pragma unroll
+      for (int i = kPerLane - 1; i >= 0; --i) first = va[i] == top ? at(i) : first;
+      if (top == -INFINITY) first = at(0);
+      if (k <= 32) {
+        const uint64_t own =
+            warp_bound(t0 + first < end ? rank_key(top, (uint32_t)(t0 + first)) : 0, k);
+        if (own) raise(own);
+      }
+      __syncthreads();
+      follow();
+      scan(va, top);
+      t0 += kStep;
+      if (p.chunk > 2 * kStep) {
+        if (lane == 0) s_count[warp] = n;
+        __syncthreads();
+        for (int i = lane; i < n; i += 32)
+          if (rank_of(s_list, s_count, list[i]) == k - 1) atomicMax(&s_bound, list[i]);
+        __syncthreads();
       }
     }
-    if (m == -INFINITY) at = index(0);
-    const uint64_t best = at < left ? rank_key(m, (uint32_t)(t0 + at)) : 0;
+    while (t0 < end) {
+      load(t0 + kStep, va);
+      follow();
+      scan(vb, sum_up(vb));
+      t0 += kStep;
+      if (t0 >= end) break;
+      load(t0 + kStep, vb);
+      follow();
+      scan(va, sum_up(va));
+      t0 += kStep;
+    }
+    float mm = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    // (a NaN anywhere, or +inf, makes the sum NaN; -inf alone leaves it 0)
-    const float zero = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) s += fast_exp2((v[i] - zero) * kLog2e);
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+    s = m == -INFINITY ? s : s * fast_exp2((m - mm) * kLog2e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane == 0) {
-      s_m[warp] = m;
+      s_m[warp] = mm;
       s_s[warp] = s;
+      s_count[warp] = n;
     }
-    const uint64_t bound = key_bound(best, k, s_warp);
-    const float least = bound ? key_value(bound) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (v[i] >= least && index(i) < left) {
-        const uint64_t key = rank_key(v[i], (uint32_t)(t0 + index(i)));
-        if (key >= bound) keep(key, s_list, &s_n);
-      }
     __syncthreads();
-    uint64_t *list = p.lists + ((size_t)row * p.chunks + chunk) * k;
-    const int n = s_n;
-    rank_keys(s_list, n, k, [&](int rank, uint64_t key) { list[rank] = key; });
-    for (int i = n + tid; i < k; i += kBeamThreads) list[i] = 0;   // a short last chunk
-    if (tid == 0) {
-      float mm = -INFINITY, ss = 0.f;
+    // the part's k largest of what its warps have listed
+    uint64_t *out = p.lists + ((size_t)row * p.chunks + chunk) * k;
+    int total = 0;
 #pragma unroll
-      for (int w = 0; w < kBeamWarps; ++w) mm = fmaxf(mm, s_m[w]);
+    for (int w = 0; w < kBeamWarps; ++w) total += s_count[w];
+    for (int i = lane; i < n; i += 32) {
+      const int rank = rank_of(s_list, s_count, list[i]);
+      if (rank < k) out[rank] = list[i];
+    }
+    for (int i = total + tid; i < k; i += kBeamThreads) out[i] = 0;   // a short last part
+    if (tid == 0) {
+      float all = -INFINITY, ss = 0.f;
+#pragma unroll
+      for (int w = 0; w < kBeamWarps; ++w) all = fmaxf(all, s_m[w]);
 #pragma unroll
       for (int w = 0; w < kBeamWarps; ++w)
-        ss += s_m[w] == -INFINITY ? s_s[w] : s_s[w] * fast_exp2((s_m[w] - mm) * kLog2e);
-      p.stats[(size_t)row * p.chunks + chunk] = make_float2(mm, ss);
+        ss += s_m[w] == -INFINITY ? s_s[w] : s_s[w] * fast_exp2((s_m[w] - all) * kLog2e);
+      p.stats[(size_t)row * p.chunks + chunk] = make_float2(all, ss);
     }
   }
   __threadfence();
@@ -286,7 +448,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
       key[j] = made;
       best = made > best ? made : best;
     }
-    const uint64_t bound = key_bound(best, k, s_warp);
+    const uint64_t bound = block_bound(best, k, s_warp);
     if (old && old >= bound) keep(old, s_list, &s_n);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
@@ -307,13 +469,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamPar
   }
 }
 
-// Keys that can reach the bound in the first pass (up to k threads of a warp
-// have a maximum that does, for k <= 32) and in a batch of the second.
-int list_size(int k) {
-  const int first = k <= 32 && k * kBeamWarps * kPerLane < kChunk ? k * kBeamWarps * kPerLane
-                                                                   : kChunk;
-  const int batch = kBatch * kBeamThreads + kMaxK;
-  return first > batch ? first : batch;
+// Parts of a row: whole steps, as many parts as give every SM its CTAs.
+int parts_of(int rows, int vocab, int *chunk) {
+  const int steps = (vocab + kStep - 1) / kStep;
+  long parts = (long)kCtasPerSm * sm_count() / (rows > 0 ? rows : 1);
+  if (parts < 1) parts = 1;
+  if (parts > steps) parts = steps;
+  const int per = (int)((steps + parts - 1) / parts);
+  *chunk = per * kStep;
+  return (steps + per - 1) / per;
 }
 
 // --------------------------------------------------------------------------
@@ -399,7 +563,9 @@ extern "C" int tllm_beam_workspace(int groups, int beams, int vocab, int k, size
   TLLM_CHECK_ARG(vocab >= 1 && vocab < (1 << 27), "vocab (%d) must be in [1, 2^27)", vocab);
   TLLM_CHECK_ARG(k >= 1 && k <= kMaxK && k <= vocab, "k (%d) must be in [1, %d] and <= vocab (%d)",
                  k, kMaxK, vocab);
-  const size_t rows = (size_t)groups * beams, chunks = (vocab + kChunk - 1) / kChunk;
+  const size_t rows = (size_t)groups * beams;
+  int chunk;
+  const size_t chunks = parts_of((int)rows, vocab, &chunk);
   *bytes = kCounterBytes + align256(rows * chunks * sizeof(float2)) +
            rows * chunks * k * sizeof(uint64_t);
   return TLLM_OK;
@@ -432,7 +598,7 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   p.beams = beams;
   p.vocab = vocab;
   p.k = k;
-  p.chunks = (vocab + kChunk - 1) / kChunk;
+  p.chunks = parts_of(groups * beams, vocab, &p.chunk);
   p.out_scores = out_scores;
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;
@@ -442,10 +608,9 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   p.stats = reinterpret_cast<float2 *>(w);
   w += align256((size_t)groups * beams * p.chunks * sizeof(float2));
   p.lists = reinterpret_cast<uint64_t *>(w);
-  const size_t smem = list_size(k) * sizeof(uint64_t);
   const bool vec = ((uintptr_t)logits & 15) == 0 && p.ld % 4 == 0;
   TLLM_CUDA(launch_pdl(vec ? beam_select_kernel<true> : beam_select_kernel<false>,
-                       dim3(p.chunks, groups * beams), dim3(kBeamThreads), smem,
+                       dim3(p.chunks, groups * beams), dim3(kBeamThreads), 0,
                        resolve(stream), p));
   return TLLM_OK;
 }

@@ -21,12 +21,14 @@ def upload_f32(arr):
 # tensors have data_ptr(), shape and dtype, met by the name of the dtype
 _CODES = {np.dtype(np.float32): _lib.F32, np.dtype(np.int32): _lib.I32}
 _NAMES = {"float32": _lib.F32, "bfloat16": _lib.BF16, "int32": _lib.I32}
+_WORDS = {_lib.F32: "float32", _lib.BF16: "bfloat16", _lib.I32: "int32"}
+_Device = gpu.DeviceTensor
 
 
 def dtype_code(t, name="tensor"):
     """TLLM_F32, TLLM_BF16 or TLLM_I32 of a device tensor: a DeviceTensor, or
     an object with data_ptr(), shape and dtype (a torch CUDA tensor)."""
-    if getattr(t, "is_bf16", False):
+    if type(t) is _Device and t.is_bf16:
         return _lib.BF16
     code = _CODES.get(t.dtype)
     if code is None:
@@ -39,7 +41,7 @@ def dtype_code(t, name="tensor"):
 
 def strides(t):
     """Element strides of a device tensor (a DeviceTensor is contiguous)."""
-    if hasattr(t, "stride"):
+    if type(t) is not _Device and hasattr(t, "stride"):
         return tuple(t.stride())
     out, n = [], 1
     for s in reversed(t.shape):
@@ -48,15 +50,20 @@ def strides(t):
     return tuple(reversed(out))
 
 
+def require_gpu(t, name):
+    if type(t) is not _Device and not getattr(t, "is_cuda", True):
+        raise ValueError(f"{name} is not on the GPU")
+
+
 def on_device(t, name, code=None, shape=None):
     """Address of a contiguous device tensor, its type and shape checked."""
     if code is not None and dtype_code(t, name) != code:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected "
-                         f"{ {0: 'float32', 1: 'bfloat16', 2: 'int32'}[code]}")
-    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected {_WORDS[code]}")
+    if shape is not None and t.shape != shape and tuple(t.shape) != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if not getattr(t, "is_cuda", True):
-        raise ValueError(f"{name} is not on the GPU")
+    if type(t) is _Device:
+        return t.ptr.value
+    require_gpu(t, name)
     contiguous = getattr(t, "is_contiguous", None)
     if contiguous is not None and not contiguous():
         raise ValueError(f"{name} must be contiguous")

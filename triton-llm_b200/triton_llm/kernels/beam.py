@@ -12,7 +12,7 @@ import ctypes
 import numpy as np
 
 from triton_llm import gpu, _lib
-from ._common import dtype_code, on_device, strides
+from ._common import dtype_code, on_device, require_gpu, strides
 from .paged import _workspace
 
 
@@ -55,8 +55,7 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     vocab = int(logits.shape[1])
     if sl[1] != 1 and vocab > 1:
         raise ValueError("rows of logits must be contiguous")
-    if not getattr(logits, "is_cuda", True):
-        raise ValueError("logits is not on the GPU")
+    require_gpu(logits, "logits")
     if len(out_scores.shape) != 2 or out_scores.shape[0] != groups:
         raise ValueError(f"out_scores must be ({groups}, k), got {tuple(out_scores.shape)}")
     shape = tuple(out_scores.shape)
@@ -76,8 +75,8 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     if workspace is None:
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
-        key = (groups, beams, vocab, k)
-        workspace = _workspace("beam", key, lambda: BeamWorkspace(*key))
+        workspace = _workspace(lambda: BeamWorkspace(groups, beams, vocab, k), "beam",
+                               gpu.current_device(), groups, beams, vocab, k)
     _lib.call("tllm_beam_select", logits.data_ptr(), sl[0] if groups * beams > 1 else 0,
               args[0], flags, int(pad_token), groups, beams, vocab, k, args[1], args[2],
               args[3], workspace.ptr, workspace.nbytes, stream)

@@ -21,7 +21,7 @@ import ctypes
 import numpy as np
 
 from triton_llm import gpu, _lib
-from ._common import dtype_code, on_device, strides
+from ._common import dtype_code, on_device, require_gpu, strides
 
 
 class PagedKV:
@@ -58,8 +58,7 @@ class PagedKV:
         if dtype_code(table, "table") != _lib.I32:
             raise ValueError(f"table must be int32, got {table.dtype}")
         for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (table, "table")):
-            if not getattr(t, "is_cuda", True):
-                raise ValueError(f"{name} is not on the GPU")
+            require_gpu(t, name)
         st = strides(table)
         if st[1] != 1 and table.shape[1] > 1:
             raise ValueError("rows of the page table must be contiguous")
@@ -71,6 +70,7 @@ class PagedKV:
         self.head_dim = int(k_pages.shape[3])
         self.n_seq, self.columns = int(table.shape[0]), int(table.shape[1])
         self.dtype = code
+        self.device = None   # of the library stream's workspaces, once needed
         self._c = _lib.PagedKVStruct(
             k_pages.data_ptr(), v_pages.data_ptr(), code, self.n_pages, self.page_size,
             self.n_kv_head, self.head_dim, self.n_seq, self.columns, 0, sk[0], sk[a],
@@ -96,25 +96,20 @@ class PagedWorkspace:
 _workspaces: dict = {}
 
 
-def _workspace(kind, key, make):
-    """The library stream's own workspace of the current device: calls on that
-    stream run one after another, so they can share it."""
-    at = (gpu.current_device(), kind, key)
-    ws = _workspaces.get(at)
+def _workspace(make, *key):
+    """The library stream's own workspace of a device: calls on that stream run
+    one after another, so they can share it."""
+    ws = _workspaces.get(key)
     if ws is None:
-        ws = _workspaces[at] = make()
+        ws = _workspaces[key] = make()
     return ws
-
-
-def _rows_pow2(rows):
-    return 1 << max(0, int(rows) - 1).bit_length()
 
 
 def _out_args(out, rows, n_head, head_dim):
     """(address, dtype code, plane rows, row stride, head stride) of an
     attention output: fp32 or bf16 (rows, n_head, head_dim), or an operand
     buffer (``gpu.act_empty``) of at least n_head * head_dim columns."""
-    if getattr(out, "is_split", False):
+    if type(out) is gpu.DeviceTensor and out.is_split:
         planes, prows, cols = out.shape
         if prows < rows or cols < n_head * head_dim:
             raise ValueError(f"out holds {prows} rows of {cols}, {rows} of "
@@ -158,8 +153,7 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     sq = strides(q)
     if sq[2] != 1 and kv.head_dim > 1:
         raise ValueError("the last axis of q must be contiguous")
-    if not getattr(q, "is_cuda", True):
-        raise ValueError("q is not on the GPU")
+    require_gpu(q, "q")
     o = _out_args(out, rows, n_head, kv.head_dim)
     if n_head % kv.n_kv_head:
         raise ValueError(f"n_head ({n_head}) must be divisible by n_kv_head ({kv.n_kv_head})")
@@ -168,8 +162,12 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     if workspace is None:
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
-        key = (_rows_pow2(rows), n_head, kv.n_kv_head, kv.head_dim)
-        workspace = _workspace("attention", key, lambda: PagedWorkspace(*key))
+        if kv.device is None:
+            kv.device = gpu.current_device()
+        n = 1 << max(0, rows - 1).bit_length()
+        workspace = _workspace(
+            lambda: PagedWorkspace(n, n_head, kv.n_kv_head, kv.head_dim),
+            "attention", kv.device, n, n_head, kv.n_kv_head, kv.head_dim)
     _lib.call("tllm_paged_attention", kv._ref, q.data_ptr(), sq[0], sq[1], seq, lens, o[0],
               o[1], o[2], o[3], o[4], rows, n_head, int(max_len), int(keys_hint),
               int(window), int(sinks), float(sm_scale or 0.0), workspace.partial,
@@ -177,27 +175,22 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     return out
 
 
-def _tables(rows, cos, sin):
-    if (cos is None) != (sin is None):
+def _tables(cos, sin):
+    """(cos, sin, positions, rotary values) of rotary tables, zeros for none."""
+    if cos is None and sin is None:
+        return None, None, 0, 0
+    if cos is None or sin is None:
         raise ValueError("cos and sin go together")
-    if cos is None:
-        return
-    if len(cos.shape) != 2 or tuple(sin.shape) != tuple(cos.shape):
+    shape = cos.shape
+    if len(shape) != 2 or tuple(sin.shape) != tuple(shape):
         raise ValueError(f"cos and sin must be 2D with the same shape, got "
-                         f"{tuple(cos.shape)} and {tuple(sin.shape)}")
-    rows.cos_t = on_device(cos, "cos", _lib.F32)
-    rows.sin_t = on_device(sin, "sin", _lib.F32)
-    rows.n_pos, rows.rotary_dim = int(cos.shape[0]), 2 * int(cos.shape[1])
+                         f"{tuple(shape)} and {tuple(sin.shape)}")
+    return (on_device(cos, "cos", _lib.F32), on_device(sin, "sin", _lib.F32),
+            int(shape[0]), 2 * int(shape[1]))
 
 
-def _indices(rows, n, row_pos, row_seq, row_src, lens_out):
-    rows.row_pos = on_device(row_pos, "row_pos", _lib.I32, (n,))
-    if row_seq is not None:
-        rows.row_seq = on_device(row_seq, "row_seq", _lib.I32, (n,))
-    if row_src is not None:
-        rows.row_src = on_device(row_src, "row_src", _lib.I32, (n,))
-    if lens_out is not None:
-        rows.lens_out = on_device(lens_out, "lens_out", _lib.I32)
+def _index(t, name, n):
+    return None if t is None else on_device(t, name, _lib.I32, (n,))
 
 
 def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq=None,
@@ -218,32 +211,30 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
     rows     use only the first ``rows`` rows
     """
     D, K = kv.head_dim, kv.n_kv_head
-    cols = (n_head + 2 * K) * D
-    if len(qkv.shape) != 2 or qkv.shape[1] != cols:
-        raise ValueError(f"qkv must be (rows, {cols}), got {tuple(qkv.shape)}")
+    shape, cols = qkv.shape, (n_head + 2 * K) * D
+    if len(shape) != 2 or shape[1] != cols:
+        raise ValueError(f"qkv must be (rows, {cols}), got {tuple(shape)}")
     if dtype_code(qkv, "qkv") != _lib.F32:
         raise ValueError(f"qkv must be float32, got {qkv.dtype}")
-    sq = strides(qkv)
-    if sq[1] != 1:
+    ld, one = strides(qkv)
+    if one != 1:
         raise ValueError("rows of qkv must be contiguous")
-    if not getattr(qkv, "is_cuda", True):
-        raise ValueError("qkv is not on the GPU")
-    n = int(qkv.shape[0]) if rows is None else int(rows)
-    if n > qkv.shape[0]:
-        raise ValueError(f"{n} rows of a qkv of {qkv.shape[0]}")
-    if len(q_out.shape) != 3 or q_out.shape[0] < n or tuple(q_out.shape[1:]) != (n_head, D):
-        raise ValueError(f"q_out must be ({n}, {n_head}, {D}), got {tuple(q_out.shape)}")
-    r = _lib.PagedRowsStruct()
+    require_gpu(qkv, "qkv")
+    n = int(shape[0]) if rows is None else int(rows)
+    if n > shape[0]:
+        raise ValueError(f"{n} rows of a qkv of {shape[0]}")
+    shape = q_out.shape
+    if len(shape) != 3 or shape[0] < n or shape[1] != n_head or shape[2] != D:
+        raise ValueError(f"q_out must be ({n}, {n_head}, {D}), got {tuple(shape)}")
+    cos_t, sin_t, n_pos, rotary = _tables(cos, sin)
     at = qkv.data_ptr()
-    r.q, r.k, r.v = at, at + n_head * D * 4, at + (n_head + K) * D * 4
-    r.q_row_stride = r.k_row_stride = r.v_row_stride = sq[0]
-    r.q_head_stride = r.k_head_stride = r.v_head_stride = D
-    r.q_out = on_device(q_out, "q_out", _lib.F32)
-    r.q_out_row_stride, r.q_out_head_stride = n_head * D, D
-    r.src_dtype, r.rows, r.n_head = _lib.F32, n, n_head
-    r.interleaved, r.blocked = bool(interleaved), bool(blocked)
-    _tables(r, cos, sin)
-    _indices(r, n, row_pos, row_seq, None, lens_out)
+    r = _lib.PagedRowsStruct(
+        at, at + n_head * D * 4, at + (n_head + K) * D * 4,
+        on_device(q_out, "q_out", _lib.F32), None, _index(row_seq, "row_seq", n),
+        _index(row_pos, "row_pos", n),
+        None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        cos_t, sin_t, ld, D, ld, D, ld, D, n_head * D, D, _lib.F32, n, n_head, rotary,
+        n_pos, bool(interleaved), bool(blocked))
     _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
     return q_out
 
@@ -266,7 +257,6 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
     if len(row_pos.shape) != 1:
         raise ValueError(f"row_pos must be 1D, got {tuple(row_pos.shape)}")
     n = int(row_pos.shape[0])
-    r = _lib.PagedRowsStruct()
     if (row_stride is None) != (head_stride is None):
         raise ValueError("row_stride and head_stride go together")
     if row_stride is None:
@@ -279,15 +269,17 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
         sk, sv = strides(k), strides(v)
         if sk[2] != 1 or sv[2] != 1:
             raise ValueError("the last axis of k and v must be contiguous")
-        r.k_row_stride, r.k_head_stride = sk[0], sk[1]
-        r.v_row_stride, r.v_head_stride = sv[0], sv[1]
     else:
-        r.k_row_stride = r.v_row_stride = int(row_stride)
-        r.k_head_stride = r.v_head_stride = int(head_stride)
-    r.k, r.v = k.data_ptr(), v.data_ptr()
-    r.src_dtype, r.rows, r.interleaved = code, n, bool(interleaved)
-    _tables(r, cos, sin)
-    _indices(r, n, row_pos, row_seq, row_src, lens_out)
+        sk = sv = (int(row_stride), int(head_stride))
+    require_gpu(k, "k")
+    require_gpu(v, "v")
+    cos_t, sin_t, n_pos, rotary = _tables(cos, sin)
+    r = _lib.PagedRowsStruct(
+        None, k.data_ptr(), v.data_ptr(), None, _index(row_src, "row_src", n),
+        _index(row_seq, "row_seq", n), _index(row_pos, "row_pos", n),
+        None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        cos_t, sin_t, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0, code, n, 0, rotary, n_pos,
+        bool(interleaved), 0)
     _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
 
 
