@@ -381,8 +381,9 @@ int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
  * (beam within the group) and out_tokens, all (groups, k). A beam with
  * done[row] != 0 (done may be NULL) has one candidate, (pad_token,
  * scores[row]). NaN candidates, and all of a beam whose score is +inf, count
- * as -inf. 1 <= k <= 64, k <= vocab,
- * beams <= 32. Scratch: tllm_beam_workspace bytes, zero-filled once; a call
+ * as -inf. out_done (groups, k), may be NULL: 1 for a candidate whose beam is
+ * done or whose token is eos_token (-1: none), else 0. 1 <= k <= 64,
+ * k <= vocab, beams <= 32. Scratch: tllm_beam_workspace bytes, zero-filled once; a call
  * that overlaps another on the GPU needs its own. The reference selects
  * greedily or by sampling (smollm2_triton/model.py:566-584).
  */
@@ -390,8 +391,8 @@ int tllm_beam_workspace(int groups, int beams, int vocab, int k, size_t *bytes);
 int tllm_beam_select(const float *logits, long ld, const float *scores,
                      const int32_t *done, int pad_token, int groups, int beams,
                      int vocab, int k, float *out_scores, int32_t *out_parents,
-                     int32_t *out_tokens, void *workspace, size_t workspace_bytes,
-                     tllm_stream_t stream);
+                     int32_t *out_tokens, int eos_token, int32_t *out_done,
+                     void *workspace, size_t workspace_bytes, tllm_stream_t stream);
 
 /*
  * Page tables after a selection step: beam i of group g continues beam

@@ -42,7 +42,7 @@ struct AttnParams {
   float *part_ml;        // (rows, n_y, max_splits, G, 2)
   int *counters;         // (rows, n_y)
   int *err;
-  int rows, group, n_gsub, g_tile, n_y;   // heads per KV head, sub-groups, heads per CTA
+  int rows, row0, group, n_gsub, g_tile, n_y;   // heads per KV head, sub-groups, heads per CTA
   int chunk, max_splits, tile;
   int window, sinks;
   float qscale;          // sm_scale * log2(e)
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kGenWarps * 32)
   constexpr int U = NV == 1 ? 4 : 2;
   extern __shared__ __align__(16) float smem_f[];
   __shared__ int s_flag;
-  const int row = blockIdx.z, y = blockIdx.y, split = blockIdx.x;
+  const int row = p.row0 + blockIdx.z, y = blockIdx.y, split = blockIdx.x;
   RowSpan x = row_keys(p, row, split);
   split_row(p, x, split, x.s + x.len - x.a);   // the visible keys, in order
   if (split >= x.n_splits) return;
@@ -1437,8 +1437,7 @@ extern "C" int tllm_paged_attention(
   const int n_y = n_kv * n_gsub;
   const int tile = mma ? (D == 128 ? Tile<128>::KT : Tile<64>::KT)
                        : kGenWarps * (nv == 1 ? 4 : 2) * (32 / lpr);
-  TLLM_CHECK_ARG(n_y <= 65535 && rows <= 65535, "grid too large: %d rows, %d head groups",
-                 rows, n_y);
+  TLLM_CHECK_ARG(n_y <= 65535, "%d head groups", n_y);
 
   const long cap = (long)kv->table_cols * kv->page_size;
   long most = max_len > 0 && max_len < cap ? max_len : cap;
@@ -1458,6 +1457,7 @@ extern "C" int tllm_paged_attention(
   int chunk = 0;
   long splits = 1, ctas = 1;
   const long blocks = (rows + kRowBlock - 1) / kRowBlock;
+  TLLM_CHECK_ARG(blocks <= 65535, "%d rows", rows);
   MmaKern kern = nullptr;
   size_t one, count;
   if (mma) {
@@ -1520,6 +1520,7 @@ extern "C" int tllm_paged_attention(
   p.err = device_error_ptr();
   TLLM_CHECK_ARG(p.err, "device error word unavailable");
   p.rows = rows;
+  p.row0 = 0;
   p.group = group;
   p.n_gsub = n_gsub;
   p.g_tile = g_tile;
@@ -1543,8 +1544,11 @@ extern "C" int tllm_paged_attention(
                          (int)slots_first));
     return TLLM_OK;
   }
-  const dim3 grid((unsigned)splits, n_y, rows);
-  return kv->kv_dtype == TLLM_BF16
-             ? launch_rows_t<__nv_bfloat16>(p, lpr, nv, grid, st)
-             : launch_rows_t<float>(p, lpr, nv, grid, st);
+  for (p.row0 = 0; p.row0 < rows; p.row0 += 65535) {   // (a grid's third axis)
+    const dim3 grid((unsigned)splits, n_y, rows - p.row0 < 65535 ? rows - p.row0 : 65535);
+    rc = kv->kv_dtype == TLLM_BF16 ? launch_rows_t<__nv_bfloat16>(p, lpr, nv, grid, st)
+                                   : launch_rows_t<float>(p, lpr, nv, grid, st);
+    if (rc) return rc;
+  }
+  return TLLM_OK;
 }

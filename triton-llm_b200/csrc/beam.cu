@@ -59,7 +59,8 @@ struct BeamParams {
   int pad, groups, beams, vocab, k;
   int chunks, chunk;    // parts of a row, their logits (whole steps)
   float *out_scores;
-  int *out_parents, *out_tokens;
+  int *out_parents, *out_tokens, *out_done;
+  int eos;
   int *counters;        // (groups)
   float2 *stats;        // (rows, chunks): max, sum of exponentials
   uint64_t *lists;      // (rows, chunks, k)
@@ -466,6 +467,9 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     p.out_scores[(size_t)group * k + tid] = key_value(s_top[tid]);
     p.out_parents[(size_t)group * k + tid] = at / p.vocab;
     p.out_tokens[(size_t)group * k + tid] = at % p.vocab;
+    if (p.out_done)
+      p.out_done[(size_t)group * k + tid] =
+          s_done[at / p.vocab] || (int)(at % p.vocab) == p.eos;
   }
 }
 
@@ -574,8 +578,9 @@ extern "C" int tllm_beam_workspace(int groups, int beams, int vocab, int k, size
 extern "C" int tllm_beam_select(const float *logits, long ld, const float *scores,
                                 const int32_t *done, int pad_token, int groups, int beams,
                                 int vocab, int k, float *out_scores, int32_t *out_parents,
-                                int32_t *out_tokens, void *workspace,
-                                size_t workspace_bytes, tllm_stream_t stream) {
+                                int32_t *out_tokens, int eos_token, int32_t *out_done,
+                                void *workspace, size_t workspace_bytes,
+                                tllm_stream_t stream) {
   TLLM_INJECT("launch");
   size_t need = 0;
   int rc = tllm_beam_workspace(groups, beams, vocab, k, &need);
@@ -602,6 +607,8 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   p.out_scores = out_scores;
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;
+  p.eos = eos_token;
+  p.out_done = out_done;
   char *w = static_cast<char *>(workspace);
   p.counters = reinterpret_cast<int *>(w);
   w += kCounterBytes;

@@ -196,24 +196,12 @@ class LlamaSession:
         self.act_planes = 2 if act_dtype == "split" else 1
         self.B = int(batch)
         self.S = int(max_seq)
-        if self.S > wts.max_pos:
-            raise ValueError(f"max_seq ({self.S}) exceeds the RoPE table "
-                             f"({wts.max_pos} positions)")
-        B, S, Hkv, D = self.B, self.S, wts.Hkv, wts.D
+        self.cos, self.sin = self._rope_tables()
+        B = self.B
         # KV cache precision follows the weights unless given ("float32" keeps
         # the reference's fp32 cache under bf16 weights)
         self.kv_bf16 = wts.bf16 if kv_dtype is None else kv_dtype in ("bfloat16", "bf16")
-        kvdt = "bfloat16" if self.kv_bf16 else np.float32
-        per_layer = 2 * B * Hkv * S * D
-        self.kv_arena = gpu.zeros((wts.L * per_layer,), kvdt)
-        esz = 2 if self.kv_bf16 else 4
-        self.kv = []
-        for i in range(wts.L):
-            k = gpu.sub_view(self.kv_arena, (2 * i) * (per_layer // 2) * esz,
-                             (B, Hkv, S, D))
-            v = gpu.sub_view(self.kv_arena, (2 * i + 1) * (per_layer // 2) * esz,
-                             (B, Hkv, S, D))
-            self.kv.append((k, v))
+        self._cache_buffers()
         self.pos = gpu.zeros((B,), np.int32)     # next position of each sequence
         self.lens = gpu.zeros((B,), np.int32)    # keys attended in the current step
         self.ids = gpu.zeros((B,), np.int32)     # tokens fed to the next step
@@ -221,8 +209,6 @@ class LlamaSession:
         self.row_seq = gpu.to_device(np.arange(B, dtype=np.int32))
         self._p2p = bool(p2p)
         self._buffers(B)
-        self.attn_ws = DecodeWorkspace(B, wts.H, Hkv, D, S,
-                                       _lib.BF16 if self.kv_bf16 else _lib.F32)
         self.lin_ws = LinearWorkspace(wts.linear_shapes(B))
         self._prefill_rows = 0
         self._p_blocks, self._p_nblocks = None, 0
@@ -233,6 +219,32 @@ class LlamaSession:
         # last known on the host: plans the split-KV sizes of small batches
         # (tllm_gqa_rows_hint); 0 = unknown
         self._keys_hint = 0
+
+    def _rope_tables(self):
+        """cos and sin of every position the session may reach."""
+        if self.S > self.w.max_pos:
+            raise ValueError(f"max_seq ({self.S}) exceeds the RoPE table "
+                             f"({self.w.max_pos} positions)")
+        return self.w.cos, self.w.sin
+
+    def _cache_buffers(self):
+        """The KV caches (B, n_kv_head, max_seq, head_dim) of all layers, one
+        arena, and the attention's scratch."""
+        w = self.w
+        B, S, Hkv, D = self.B, self.S, w.Hkv, w.D
+        per_layer = 2 * B * Hkv * S * D
+        self.kv_arena = gpu.zeros((w.L * per_layer,),
+                                  "bfloat16" if self.kv_bf16 else np.float32)
+        esz = 2 if self.kv_bf16 else 4
+        self.kv = []
+        for i in range(w.L):
+            k = gpu.sub_view(self.kv_arena, (2 * i) * (per_layer // 2) * esz,
+                             (B, Hkv, S, D))
+            v = gpu.sub_view(self.kv_arena, (2 * i + 1) * (per_layer // 2) * esz,
+                             (B, Hkv, S, D))
+            self.kv.append((k, v))
+        self.attn_ws = DecodeWorkspace(B, w.H, Hkv, D, S,
+                                       _lib.BF16 if self.kv_bf16 else _lib.F32)
 
     def _act(self, rows, cols):
         """A projection-input buffer: bf16 operand format for bf16 weights,
@@ -309,7 +321,6 @@ class LlamaSession:
         layer's first, or the final norm)."""
         w = self.w
         L = w.layers[i]
-        k, v = self.kv[i]
         ss = self.ss if decode else self.p_ss
         fold_ln1 = None
         if part is not None and i > 0:
@@ -320,21 +331,8 @@ class LlamaSession:
             fold_ln1 = FoldedNorm(L["ln1"], x, ss, w.n, w.eps, M, w.F)
         else:
             rms_norm_rows(h, L["ln1"], x, M, w.eps)
-        linear(x, L["qkv"], op=_lib.EPI_QKV, ws=ws, M=M, fold_in=fold_ln1, qkv=dict(
-            cos=w.cos, sin=w.sin, row_seq=row_seq, row_pos=row_pos, q_out=q,
-            k_cache=k, v_cache=v, n_head=w.H, n_kv_head=w.Hkv, head_dim=w.D,
-            lens_out=lens if decode else None))
-        # decode: row b reads its own sequence for lens[b] keys (set by the
-        # QKV epilogue); prefill: row r reads its sequence's causal prefix,
-        # in blocks of 64 rows (tllm_gqa_prefill) where the cache allows
-        if not decode and self._p_blocks is not None:
-            gqa_prefill(q, k, v, self._p_blocks, self._p_nblocks, attn, w.H,
-                        w.H * w.D, w.D, w.H * w.D, w.D)
-        else:
-            gqa_rows(q, k, v, row_seq, lens if decode else row_len, attn, M, w.H,
-                     w.H * w.D, w.D, w.H * w.D, w.D,
-                     self.S if decode else (max_len or self.S), workspace=attn_ws,
-                     keys_hint=self._keys_hint if decode else 0)
+        self._project_qkv(i, M, x, q, row_seq, row_pos, lens, ws, decode, fold_ln1)
+        self._attend(i, M, q, attn, row_seq, lens, decode, attn_ws, row_len, max_len)
         if part is None and decode and self.mlp_ws is not None:
             _mlp.mlp_block(attn, L["o"], h, L["ln2"], x, L["gu"], act, L["down"], M,
                            w.eps, self.mlp_ws)
@@ -363,6 +361,31 @@ class LlamaSession:
             linear(act, L["down"], out_dev=h, op=_lib.EPI_RESID, resid_dev=h, ws=ws, M=M)
         else:
             self._reduce(act, L["down"], part, M, ws)
+
+    def _project_qkv(self, i, M, x, q, row_seq, row_pos, lens, ws, decode, fold_in):
+        """q of M rows (rotated) and their k, v in layer i's cache."""
+        w = self.w
+        k, v = self.kv[i]
+        linear(x, w.layers[i]["qkv"], op=_lib.EPI_QKV, ws=ws, M=M, fold_in=fold_in, qkv=dict(
+            cos=self.cos, sin=self.sin, row_seq=row_seq, row_pos=row_pos, q_out=q,
+            k_cache=k, v_cache=v, n_head=w.H, n_kv_head=w.Hkv, head_dim=w.D,
+            lens_out=lens if decode else None))
+
+    def _attend(self, i, M, q, attn, row_seq, lens, decode, attn_ws, row_len, max_len):
+        """Attention of M rows over layer i's cache. Decode: row b reads its
+        own sequence for lens[b] keys (set by the QKV epilogue); prefill: row r
+        reads its sequence's causal prefix, in blocks of 64 rows
+        (tllm_gqa_prefill) where the cache allows."""
+        w = self.w
+        k, v = self.kv[i]
+        if not decode and self._p_blocks is not None:
+            gqa_prefill(q, k, v, self._p_blocks, self._p_nblocks, attn, w.H,
+                        w.H * w.D, w.D, w.H * w.D, w.D)
+        else:
+            gqa_rows(q, k, v, row_seq, lens if decode else row_len, attn, M, w.H,
+                     w.H * w.D, w.D, w.H * w.D, w.D,
+                     self.S if decode else (max_len or self.S), workspace=attn_ws,
+                     keys_hint=self._keys_hint if decode else 0)
 
     def _next_norm(self, i, x, ss, decode, M):
         """The folded norm after layer i's down projection: the next layer's
@@ -409,19 +432,8 @@ class LlamaSession:
         else:
             self._norm_add(h, part, w.norm, x, M)
 
-    def prefill(self, prompts, all_logits=False, slots=None):
-        """Run the prompts through the model into cache sequences ``slots``
-        (default 0..len(prompts)-1).
-
-        Every such sequence restarts at position 0. Returns the logits of the
-        last prompt token of each prompt (host, (n, V)), or of every prompt
-        token when ``all_logits`` (host, (sum(len), V)). Afterwards ``ids``
-        holds the greedy next token of each prompt's sequence and ``pos`` the
-        prompt lengths, ready for ``decode_step``. Without ``slots`` the other
-        sequences are reset to position 0; with ``slots`` they keep their
-        state (a serving loop admitting requests into free slots).
-        """
-        w = self.w
+    def _check_prompts(self, prompts, slots):
+        """(prompts, slots, lengths, whether the other sequences stay)."""
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
         nseq = len(prompts)
         if nseq > self.B:
@@ -438,12 +450,33 @@ class LlamaSession:
             raise ValueError("every prompt needs at least one token")
         if lens.max() > self.S:
             raise ValueError(f"prompt of {lens.max()} tokens exceeds max_seq {self.S}")
+        return prompts, slots, lens, keep
+
+    def _prompt_rows(self, seq, pos):
+        """Called with the sequences and positions of a prefill's rows."""
+
+    def prefill(self, prompts, all_logits=False, slots=None):
+        """Run the prompts through the model into cache sequences ``slots``
+        (default 0..len(prompts)-1).
+
+        Every such sequence restarts at position 0. Returns the logits of the
+        last prompt token of each prompt (host, (n, V)), or of every prompt
+        token when ``all_logits`` (host, (sum(len), V)). Afterwards ``ids``
+        holds the greedy next token of each prompt's sequence and ``pos`` the
+        prompt lengths, ready for ``decode_step``. Without ``slots`` the other
+        sequences are reset to position 0; with ``slots`` they keep their
+        state (a serving loop admitting requests into free slots).
+        """
+        w = self.w
+        prompts, slots, lens, keep = self._check_prompts(prompts, slots)
+        nseq = len(prompts)
         M = int(lens.sum())
         if M > self._prefill_rows:
             self._prefill_buffers(M, 256 << 20)
         ids = np.concatenate(prompts)
         seq = np.repeat(slots, lens)
         pos = np.concatenate([np.arange(n, dtype=np.int32) for n in lens])
+        self._prompt_rows(seq, pos)
         self.p_ids.from_numpy(np.pad(ids, (0, self._prefill_rows - M)))
         self.p_seq.from_numpy(np.pad(seq, (0, self._prefill_rows - M)))
         self.p_pos.from_numpy(np.pad(pos, (0, self._prefill_rows - M)))

@@ -10,7 +10,9 @@ the GPU: the KV cache is written and read in place (the reference copies the
 whole prefix between host and device in every layer, model.py:301-308), and
 decode steps sample on the device, greedy or temperature / top-k.
 
-``generate_batch`` adds ragged-batch greedy generation over many prompts.
+``generate_batch`` adds ragged-batch greedy generation over many prompts,
+``generate_paged`` the same over a paged cache (sliding windows, scaled rotary
+positions) and ``generate_beam`` beam search.
 """
 
 from __future__ import annotations
@@ -289,6 +291,52 @@ class SmolLM2ForCausalLM:
                 g = g[: g.index(eos_token_id) + 1]
             out.append(np.concatenate([p, np.array(g, np.int32)]))
         return out
+
+    def generate_paged(self, prompts, max_new_tokens: int = 20,
+                       eos_token_id: int | None = None, use_graph: bool = True, **session):
+        """``generate_batch`` over a paged KV cache. ``session``: arguments of
+        ``PagedSession`` -- page_size, n_pages, window and sinks (a sliding
+        window with a few first tokens that stay visible), rope_scaling (contexts
+        past the model's own, ``scaled_cos_sin``)."""
+        from .paged import PagedSession
+        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        longest = max(len(p) for p in prompts) + max_new_tokens
+        if longest > self.config.max_position_embeddings and not session.get("rope_scaling"):
+            raise ValueError(f"{longest} tokens exceed max_position_embeddings "
+                             f"({self.config.max_position_embeddings})")
+        self._init_gpu_weights()
+        sess = PagedSession(self.dev, len(prompts), longest, kv_dtype=self._kv_dtype,
+                            act_dtype=self._act_dtype, **session)
+        logits = sess.prefill(prompts)
+        gen = [[int(np.argmax(row))] for row in logits]
+        if use_graph and max_new_tokens > 1:
+            sess.capture()
+        for _ in range(max_new_tokens - 1):
+            sess.step()
+            for row, t in zip(gen, sess.ids.to_numpy()):
+                row.append(int(t))
+        out = []
+        for p, g in zip(prompts, gen):
+            if eos_token_id is not None and eos_token_id in g:
+                g = g[: g.index(eos_token_id) + 1]
+            out.append(np.concatenate([p, np.array(g, np.int32)]))
+        return out
+
+    def generate_beam(self, prompts, beams: int = 4, max_new_tokens: int = 20,
+                      eos_token_id: int | None = None, length_penalty: float = 0.0,
+                      **session):
+        """Beam search over a paged KV cache (``beam_search``): for every prompt
+        its ``beams`` best continuations as (generated tokens, score)."""
+        from .paged import beam_search
+        for p in prompts:
+            n = len(np.asarray(p).reshape(-1)) + max_new_tokens
+            if n > self.config.max_position_embeddings and not session.get("rope_scaling"):
+                raise ValueError(f"{n} tokens exceed max_position_embeddings "
+                                 f"({self.config.max_position_embeddings})")
+        self._init_gpu_weights()
+        return beam_search(self.dev, prompts, beams, max_new_tokens, eos_token_id,
+                           length_penalty, kv_dtype=self._kv_dtype,
+                           act_dtype=self._act_dtype, **session)
 
     # ------------------------------------------------------------------
     def _embed(self, token_ids: np.ndarray) -> np.ndarray:

@@ -103,8 +103,8 @@ SIGNATURES: dict[str, list] = {
     "tllm_page_copy": [_vp, _l, _i, _l, _i, _i, _l, _i, _i, _vp, _vp, _vp, _i, _vp],
     # beam search
     "tllm_beam_workspace": [_i, _i, _i, _i, _psz],
-    "tllm_beam_select": [_vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz,
-                         _vp],
+    "tllm_beam_select": [_vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp,
+                         _vp, _sz, _vp],
     "tllm_beam_reorder": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp],
     # projections
     "tllm_linear_workspace": [_i, _i, _i, _psz, _psz],

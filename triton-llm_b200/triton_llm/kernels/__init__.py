@@ -18,7 +18,8 @@ from .linear import Linear, LinearWorkspace, linear
 from .paged import (PagedKV, PagedWorkspace, page_copy, paged_append, paged_attention,
                     paged_write)
 from .rms_norm import rms_norm
-from .rope import precompute_cos_sin, precompute_cos_sin_device, apply_rope
+from .rope import (apply_rope, precompute_cos_sin, precompute_cos_sin_device,
+                   scaled_cos_sin)
 from .softmax import softmax
 from .swiglu import swiglu
 
@@ -57,4 +58,5 @@ __all__ = [
     "BeamWorkspace",
     "beam_select",
     "beam_reorder",
+    "scaled_cos_sin",
 ]

@@ -29,7 +29,7 @@ class BeamWorkspace:
 
 
 def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
-                pad_token=0, workspace=None, stream=None):
+                pad_token=0, out_done=None, eos_token=-1, workspace=None, stream=None):
     """The k best continuations of every group of beams.
 
     logits   (groups * beams, vocab) float32, rows contiguous
@@ -41,6 +41,8 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
              the lower token; k <= 64
     done     (groups, beams) or (groups * beams,) int32 or None: a beam with a
              value != 0 has one candidate, ``pad_token`` at its own score
+    out_done (groups, k) int32 or None: whether the candidate's beam is done or
+             its token is ``eos_token``
     """
     if len(scores.shape) != 2 or len(logits.shape) != 2:
         raise ValueError(f"scores and logits must be 2D, got {tuple(scores.shape)}, "
@@ -79,7 +81,9 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
                                gpu.current_device(), groups, beams, vocab, k)
     _lib.call("tllm_beam_select", logits.data_ptr(), sl[0] if groups * beams > 1 else 0,
               args[0], flags, int(pad_token), groups, beams, vocab, k, args[1], args[2],
-              args[3], workspace.ptr, workspace.nbytes, stream)
+              args[3], int(eos_token),
+              None if out_done is None else on_device(out_done, "out_done", _lib.I32, shape),
+              workspace.ptr, workspace.nbytes, stream)
 
 
 def beam_reorder(parents, lens, table, table_out, copy_src, copy_dst, copy_fill, *,

@@ -107,18 +107,20 @@ def _workspace(make, *key):
 
 def _out_args(out, rows, n_head, head_dim):
     """(address, dtype code, plane rows, row stride, head stride) of an
-    attention output: fp32 or bf16 (rows, n_head, head_dim), or an operand
-    buffer (``gpu.act_empty``) of at least n_head * head_dim columns."""
-    if type(out) is gpu.DeviceTensor and out.is_split:
-        planes, prows, cols = out.shape
-        if prows < rows or cols < n_head * head_dim:
-            raise ValueError(f"out holds {prows} rows of {cols}, {rows} of "
-                             f"{n_head * head_dim} needed")
-        return (out.data_ptr(), _lib.SPLIT if planes == 2 else _lib.BF16, prows, cols,
-                head_dim)
+    attention output: fp32 or bf16 (rows, n_head, head_dim), or a buffer of at
+    least so many rows and n_head * head_dim columns: fp32 2D, or in an operand
+    format (``gpu.act_empty``)."""
     code = dtype_code(out, "out")
     if code == _lib.I32:
         raise ValueError("out must be float32 or bfloat16")
+    if type(out) is gpu.DeviceTensor and (out.is_split or len(out.shape) == 2):
+        prows, cols = out.shape[-2:]
+        if prows < rows or cols < n_head * head_dim:
+            raise ValueError(f"out holds {prows} rows of {cols}, {rows} of "
+                             f"{n_head * head_dim} needed")
+        if out.is_split and out.shape[0] == 2:
+            code = _lib.SPLIT
+        return out.data_ptr(), code, prows, cols, head_dim
     ptr = on_device(out, "out", None, (rows, n_head, head_dim))
     return ptr, code, rows, n_head * head_dim, head_dim
 
@@ -130,7 +132,8 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     kv        PagedKV
     q         (rows, n_head, head_dim) float32, the last axis contiguous
     row_len   (rows,) int32 on the device: keys before and with the row's token
-    out       (rows, n_head, head_dim) float32 or bfloat16, or an operand buffer
+    out       (rows, n_head, head_dim) float32 or bfloat16, or a buffer of at least
+              rows x (n_head * head_dim): fp32, or in an operand format
     row_seq   (rows,) int32 on the device: the rows' sequences (None: row r is
               sequence r); rows may share a sequence
     max_len, keys_hint
