@@ -135,56 +135,80 @@ __device__ void finish_split(const AttnParams &p, const RowSpan &x, int row, int
   }
   if (single) return;
 
-  __threadfence();
   __syncthreads();
   if (tid == 0) {
     int *ctr = p.counters + (size_t)row * p.n_y + y;
-    const int ticket = atomicAdd(ctr, 1);
-    *s_flag = ticket == x.n_splits - 1;
+    __threadfence();   // (of all writes that the barrier has ordered before)
+    *s_flag = atomicAdd(ctr, 1) == x.n_splits - 1;
     if (*s_flag) *ctr = 0;   // all other CTAs of this (row, y) took theirs
+    __threadfence();
   }
   __syncthreads();
   if (!*s_flag) return;
-  __threadfence();
 
+  // The statistics (one split per lane) and the first kJoin values of this
+  // thread's first output are on the way together; later ones come in batches
+  // whose size does not depend on the number of splits.
+  constexpr int kJoin = 8;
   const size_t base = ((size_t)row * p.n_y + y) * p.max_splits;
-  float *sw = smem;   // [G][max_splits] weights of the splits
+  const float *acc = p.part_acc + base * p.g_tile * D;
+  const size_t step = (size_t)p.g_tile * D;
+  float v[kJoin];
+  auto load = [&](int s0, int i) {
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k)
+      v[k] = __ldcg(acc + (size_t)min(s0 + k, x.n_splits - 1) * step + i);
+  };
+  if (tid < G * D) load(0, tid);
+  float *sw = smem;   // [G][kMaxSplits] weights of the splits
+  const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + base * p.g_tile;
   for (int g = warp; g < G; g += THREADS / 32) {
-    float mx = -INFINITY;
-    for (int s = lane; s < x.n_splits; s += 32)
-      mx = fmaxf(mx, __ldcg(&p.part_ml[((base + s) * p.g_tile + g) * 2]));
+    auto stats = [&](int s) {
+      return s < x.n_splits ? __ldcg(ml + (size_t)s * p.g_tile + g)
+                            : make_float2(-INFINITY, 0.f);
+    };
+    const float2 own = stats(lane);
+    float mx = own.x, den = 0.f;
+    for (int s = lane + 32; s < x.n_splits; s += 32) mx = fmaxf(mx, stats(s).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-    float den = 0.f;
-    for (int s = lane; s < x.n_splits; s += 32) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
-          &p.part_ml[((base + s) * p.g_tile + g) * 2]));
-      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
-      sw[g * kMaxSplits + s] = f;
-      den = fmaf(ml.y, f, den);
-    }
+    auto weigh = [&](int s, float2 m) {
+      const float f = m.x == -INFINITY ? 0.f : fast_exp2(m.x - mx);
+      if (s < x.n_splits) sw[g * kMaxSplits + s] = f;
+      den = fmaf(m.y, f, den);
+    };
+    weigh(lane, own);
+    for (int s = lane + 32; s < x.n_splits; s += 32) weigh(s, stats(s));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(~0u, den, o);
     const float inv = den == 0.f ? 0.f : 1.f / den;
+    __syncwarp();
     for (int s = lane; s < x.n_splits; s += 32) sw[g * kMaxSplits + s] *= inv;
   }
   __syncthreads();
   for (int i = tid; i < G * D; i += THREADS) {
     const int g = i / D;
     float o = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < x.n_splits; ++s)
-      o = fmaf(sw[g * kMaxSplits + s], __ldcg(&p.part_acc[(base + s) * p.g_tile * D + i]), o);
+    for (int s0 = 0; s0 < x.n_splits; s0 += kJoin) {
+      if (i != tid || s0 > 0) load(s0, i);
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k)
+        if (s0 + k < x.n_splits) o = fmaf(sw[g * kMaxSplits + s0 + k], v[k], o);
+    }
     store_out(p, (size_t)row * p.o_sr + (size_t)(head0 + g) * p.o_sh + (i - g * D), o);
   }
 }
 
 // --------------------------------------------------------------------------
 // Every page size, layout, cache type and head_dim: CUDA cores, loads straight
-// from the pages. LPR lanes (a power of two) share a key, each holding NV
-// 16-byte units of it; a warp takes KPW = U * 32 / LPR keys at a time with all
-// their K and V loads in flight. Each group of LPR lanes keeps its own running
-// maximum and sums over its keys, joined at the end.
+// from the pages. LPR lanes (8, 16 or 32) share a key, each holding NV 16-byte
+// units of it; a warp takes U * 32 / LPR keys at a time with all their K and V
+// loads in flight and their pages looked up one step ahead. The U x G partial
+// products of a lane are summed over the LPR lanes by halving: a lane passes
+// on half of its sums and keeps the other half in every step, so that 16 sums
+// over 32 lanes cost 16 shuffles, not 80, and end in one lane each, which keeps
+// the running maximum and sum of its head. Each group of LPR lanes has its own
+// over its keys; they are joined at the end.
 // --------------------------------------------------------------------------
 constexpr int kGenWarps = 8;
 
@@ -204,14 +228,21 @@ template <> struct Unit<__nv_bfloat16> {
   }
 };
 
-template <typename T, int G, int NV>
+// Keys of a group of lanes whose loads are in flight together, as far as the
+// registers go.
+__host__ __device__ constexpr int units_deep(int NV) { return NV > 1 ? 2 : 4; }
+
+template <typename T, int G, int NV, int LPR>
 __global__ void __launch_bounds__(kGenWarps * 32)
-    paged_rows_kernel(const AttnParams p, const int LPR) {
+    paged_rows_kernel(const AttnParams p) {
   griddep_launch();
   griddep_wait();
   using UT = Unit<T>;
   constexpr int E = UT::N;
-  constexpr int U = NV == 1 ? 4 : 2;
+  constexpr int U = units_deep(NV), N = U * G;
+  constexpr int R = N > LPR ? N / LPR : 1;   // sums that a lane ends up with
+  constexpr int rpw = 32 / LPR;              // groups of lanes
+  static_assert(U <= LPR, "a lane's sums are of one key");
   extern __shared__ __align__(16) float smem_f[];
   __shared__ int s_flag;
   const int row = p.row0 + blockIdx.z, y = blockIdx.y, split = blockIdx.x;
@@ -225,16 +256,14 @@ __global__ void __launch_bounds__(kGenWarps * 32)
   const int D = p.kv.head_dim;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = D / E;
-  const int rl = lane / LPR, cl = lane % LPR, rpw = 32 / LPR;
+  const int rl = lane / LPR, cl = lane % LPR;
   const T *kp = static_cast<const T *>(p.kv.k);
   const T *vp = static_cast<const T *>(p.kv.v);
   const int *table = p.kv.table + (size_t)x.seq * p.kv.table_stride;
 
-  float q[G][NV * E], acc[G][NV * E], m[G], l[G];
+  float q[G][NV * E], acc[G][NV * E];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = cl + v * LPR;
@@ -253,43 +282,70 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 #pragma unroll
     for (int e = 0; e < NV * E; ++e) acc[g][e] = 0.f;
   }
+  // Sum n = u * G + g (key u, head g) ends in the lane of each group that has
+  // lane bit o_k set where n has bit half_k, o_k = LPR / 2, LPR / 4, .. and
+  // half_k = N / 2, N / 4, ..; with R > 1 a lane has R neighbours.
+  int n0 = 0;
+#pragma unroll
+  for (int o = LPR / 2, half = N / 2; o > 0 && half >= R && half > 0; o >>= 1, half >>= 1)
+    if (cl & o) n0 += half;
+  const int my_u = n0 / G;
+  auto holder = [&](int n) {   // lane of sum n in this lane's group
+    int at = rl * LPR;
+#pragma unroll
+    for (int o = LPR / 2, half = N / 2; o > 0 && half >= R && half > 0; o >>= 1, half >>= 1)
+      if (n & half) at += o;
+    return at;
+  };
+  float m[R], l[R];   // of heads n0 % G + i; l of this lane's keys only
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
 
   const int step = kGenWarps * U * rpw;
   bool bad = false;
-  for (int i0 = x.begin + warp * U * rpw; i0 < x.end; i0 += step) {
+  // page of key i (-1: none, or out of range); looked up one step ahead
+  auto lookup = [&](int i) {
+    if (i >= x.end) return -1;
+    const int page = table[p.kv.column(i < x.s ? i : i - x.s + x.a)];
+    if (page >= 0 && page < p.kv.n_pages) return page;
+    bad = true;
+    return -1;
+  };
+  int next[U];
+  const int first = x.begin + warp * U * rpw;
+#pragma unroll
+  for (int u = 0; u < U; ++u) next[u] = lookup(first + u * rpw + rl);
+  for (int i0 = first; i0 < x.end; i0 += step) {
     uint4 kr[U][NV], vr[U][NV];
-    bool ok[U];
+    bool mine = false;   // whether the row sees this lane's key
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * rpw + rl;
-      ok[u] = i < x.end;
-      int page = 0, slot = 0;
-      if (ok[u]) {
-        const int pos = i < x.s ? i : i - x.s + x.a;
-        const int col = p.kv.column(pos);
-        slot = pos - col * p.kv.page_size;
-        page = table[col];
-        if (page < 0 || page >= p.kv.n_pages) {
-          ok[u] = false;
-          bad = true;
-        }
-      }
-      const size_t at = ok[u] ? p.kv.offset(page, kvh, slot) : 0;
+      const int pos = i < x.s ? i : i - x.s + x.a;
+      const bool ok = next[u] >= 0;
+      if (u == my_u) mine = ok;
+      const size_t at =
+          ok ? p.kv.offset(next[u], kvh, pos - p.kv.column(pos) * p.kv.page_size) : 0;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = cl + v * LPR;
         kr[u][v] = vr[u][v] = make_uint4(0, 0, 0, 0);
-        if (ok[u] && c < units) {
+        if (ok && c < units) {
           kr[u][v] = ld_stream(kp + at + c * E);
           vr[u][v] = ld_stream(vp + at + c * E);
         }
       }
     }
-    float sc[U][G];
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = lookup(i0 + step + u * rpw + rl);
+    float sc[N];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) sc[u][g] = 0.f;
+      for (int g = 0; g < G; ++g) sc[u * G + g] = 0.f;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float f[E];
@@ -297,36 +353,56 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int e = 0; e < E; ++e) sc[u][g] = fmaf(q[g][v * E + e], f[e], sc[u][g]);
+          for (int e = 0; e < E; ++e)
+            sc[u * G + g] = fmaf(q[g][v * E + e], f[e], sc[u * G + g]);
       }
     }
-    for (int o = 1; o < LPR; o <<= 1)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int o = LPR / 2, half = N / 2; o > 0; o >>= 1, half >>= 1) {
+      if (half >= R && half > 0) {
+        const bool upper = cl & o;
 #pragma unroll
-        for (int g = 0; g < G; ++g) sc[u][g] += __shfl_xor_sync(~0u, sc[u][g], o);
+        for (int i = 0; i < half; ++i) {
+          const float give = upper ? sc[i] : sc[i + half];
+          const float keep = upper ? sc[i + half] : sc[i];
+          sc[i] = keep + __shfl_xor_sync(~0u, give, o);
+        }
+      } else {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float mn = m[g];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!ok[u]) sc[u][g] = -INFINITY;
-        mn = fmaxf(mn, sc[u][g]);
+        for (int i = 0; i < R; ++i) sc[i] += __shfl_xor_sync(~0u, sc[i], o);
       }
+    }
+    float alpha[R];
+    bool moved = false;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (!mine) sc[i] = -INFINITY;
+      // maximum over the group's keys: the lanes that differ in the bits of u
+      float mn = fmaxf(m[i], sc[i]);
+#pragma unroll
+      for (int o = LPR / 2, k = U; k > 1; o >>= 1, k >>= 1)
+        mn = fmaxf(mn, __shfl_xor_sync(~0u, mn, o));
       const float base = mn == -INFINITY ? 0.f : mn;
-      const float alpha = fast_exp2(m[g] - base);   // 0 while m is -inf
-      m[g] = mn;
-      l[g] *= alpha;
+      alpha[i] = fast_exp2(m[i] - base);   // 0 while m is -inf
+      moved |= mn != m[i];
+      m[i] = mn;
+      sc[i] = fast_exp2(sc[i] - base);
+      l[i] = fmaf(l[i], alpha[i], sc[i]);
+    }
+    if (__any_sync(~0u, moved)) {
 #pragma unroll
-      for (int e = 0; e < NV * E; ++e) acc[g][e] *= alpha;
+      for (int g = 0; g < G; ++g) {
+        const float f = __shfl_sync(~0u, alpha[g & (R - 1)], holder(g));
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        sc[u][g] = fast_exp2(sc[u][g] - base);
-        l[g] += sc[u][g];
+        for (int e = 0; e < NV * E; ++e) acc[g][e] *= f;
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      float w[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        w[g] = __shfl_sync(~0u, sc[(u * G + g) & (R - 1)], holder(u * G + g));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float f[E];
@@ -335,21 +411,35 @@ __global__ void __launch_bounds__(kGenWarps * 32)
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            acc[g][v * E + e] = fmaf(sc[u][g], f[e], acc[g][v * E + e]);
+            acc[g][v * E + e] = fmaf(w[g], f[e], acc[g][v * E + e]);
       }
+    }
   }
   if (bad) atomicOr(p.err, DEV_ERR_PAGE);
 
+  // every lane's view of all heads: maximum, and the sum over the group's keys
+  float mg[G], lg[G];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int o = LPR / 2, k = U; k > 1; o >>= 1, k >>= 1)
+      l[i] += __shfl_xor_sync(~0u, l[i], o);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    mg[g] = __shfl_sync(~0u, m[g & (R - 1)], holder(g));
+    lg[g] = __shfl_sync(~0u, l[g & (R - 1)], holder(g));
+  }
   // join the groups of lanes of this warp
+#pragma unroll
   for (int o = LPR; o < 32; o <<= 1)
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float mo = __shfl_xor_sync(~0u, m[g], o);
-      const float mn = fmaxf(m[g], mo);
+      const float mo = __shfl_xor_sync(~0u, mg[g], o);
+      const float mn = fmaxf(mg[g], mo);
       const float base = mn == -INFINITY ? 0.f : mn;
-      const float f0 = fast_exp2(m[g] - base), f1 = fast_exp2(mo - base);
-      m[g] = mn;
-      l[g] = l[g] * f0 + __shfl_xor_sync(~0u, l[g], o) * f1;
+      const float f0 = fast_exp2(mg[g] - base), f1 = fast_exp2(mo - base);
+      mg[g] = mn;
+      lg[g] = lg[g] * f0 + __shfl_xor_sync(~0u, lg[g], o) * f1;
 #pragma unroll
       for (int e = 0; e < NV * E; ++e)
         acc[g][e] = acc[g][e] * f0 + __shfl_xor_sync(~0u, acc[g][e], o) * f1;
@@ -370,8 +460,8 @@ __global__ void __launch_bounds__(kGenWarps * 32)
             w_acc[(warp * Gn + g) * D + c * E + e] = acc[g][v * E + e];
       }
       if (cl == 0) {
-        w_m[warp * Gn + g] = m[g];
-        w_l[warp * Gn + g] = l[g];
+        w_m[warp * Gn + g] = mg[g];
+        w_l[warp * Gn + g] = lg[g];
       }
     }
   }
@@ -1271,38 +1361,44 @@ bool mma_takes(const tllm_paged_kv *kv, const PagedView &w) {
          (kv->n_pages == 1 || kv->page_stride > 0);
 }
 
-template <typename T, int G, int NV>
-int launch_rows(const AttnParams &p, int lpr, dim3 grid, cudaStream_t st) {
+template <typename T, int G, int NV, int LPR>
+int launch_rows(const AttnParams &p, dim3 grid, cudaStream_t st) {
   const int D = p.kv.head_dim;
   size_t smem = (size_t)kGenWarps * G * (D + 2) * sizeof(float);
   const size_t sw = (size_t)G * kMaxSplits * sizeof(float);
   if (sw > smem) smem = sw;
-  auto kern = paged_rows_kernel<T, G, NV>;
+  auto kern = paged_rows_kernel<T, G, NV, LPR>;
   if (smem > 48 * 1024)
     TLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)smem));
-  TLLM_CUDA(launch_pdl(kern, grid, dim3(kGenWarps * 32), smem, st, p, lpr));
+  TLLM_CUDA(launch_pdl(kern, grid, dim3(kGenWarps * 32), smem, st, p));
   return TLLM_OK;
 }
 
-template <typename T, int NV>
-int launch_rows_g(const AttnParams &p, int lpr, dim3 grid, cudaStream_t st) {
-  if (p.g_tile == 1) return launch_rows<T, 1, NV>(p, lpr, grid, st);
-  if (p.g_tile == 2) return launch_rows<T, 2, NV>(p, lpr, grid, st);
-  if (p.g_tile <= 4) return launch_rows<T, 4, NV>(p, lpr, grid, st);
-  if constexpr (NV * Unit<T>::N <= 8) return launch_rows<T, 8, NV>(p, lpr, grid, st);
+template <typename T, int NV, int LPR>
+int launch_rows_g(const AttnParams &p, dim3 grid, cudaStream_t st) {
+  if (p.g_tile == 1) return launch_rows<T, 1, NV, LPR>(p, grid, st);
+  if (p.g_tile == 2) return launch_rows<T, 2, NV, LPR>(p, grid, st);
+  if (p.g_tile <= 4) return launch_rows<T, 4, NV, LPR>(p, grid, st);
+  if constexpr (NV * Unit<T>::N <= 8) return launch_rows<T, 8, NV, LPR>(p, grid, st);
   set_error("group tile %d not built", p.g_tile);
   return TLLM_ERR_UNSUPPORTED;
 }
 
 template <typename T>
 int launch_rows_t(const AttnParams &p, int lpr, int nv, dim3 grid, cudaStream_t st) {
-  if (nv == 1) return launch_rows_g<T, 1>(p, lpr, grid, st);
-  if (nv == 2) return launch_rows_g<T, 2>(p, lpr, grid, st);
-  if constexpr (Unit<T>::N == 4) return launch_rows_g<T, 4>(p, lpr, grid, st);
+  if (lpr == 8) return launch_rows_g<T, 1, 8>(p, grid, st);
+  if (lpr == 16) return launch_rows_g<T, 1, 16>(p, grid, st);
+  if (nv == 1) return launch_rows_g<T, 1, 32>(p, grid, st);
+  if (nv == 2) return launch_rows_g<T, 2, 32>(p, grid, st);
+  if constexpr (Unit<T>::N == 4) return launch_rows_g<T, 4, 32>(p, grid, st);
   set_error("head_dim %d not built", p.kv.head_dim);
   return TLLM_ERR_UNSUPPORTED;
 }
+
+// A split of fewer keys costs more than it saves (6 rows of 12 heads of 64 fp32,
+// 17 to 1003 keys: 13.1 us with 64, 10.6 with 128, 15.3 with 256).
+constexpr int kMinKeys = 128;
 
 // Keys per split, a multiple of `tile`, for `pairs` (row, head group) pairs
 // of at most max_keys keys and about `keys` in all rows.
@@ -1310,7 +1406,7 @@ int plan_chunk(int tile, long rows, int n_y, long keys, long max_keys, long slot
   const long tiles = (max_keys + tile - 1) / tile;
   long c = (keys * n_y / tile + slots - 1) / slots;   // one CTA per slot
   if (rows * n_y >= slots || c > 32) c = c < 32 ? 32 : c;
-  if (c < 2) c = 2;
+  if (c * tile < kMinKeys) c = (kMinKeys + tile - 1) / tile;
   const long least = (tiles + kMaxSplits - 1) / kMaxSplits;
   if (c < least) c = least;
   if (c > tiles) c = tiles > 0 ? tiles : 1;
@@ -1426,7 +1522,7 @@ extern "C" int tllm_paged_attention(
   const int group = n_head / n_kv;
   const bool mma = mma_takes(kv, p.kv);
   const int units = D / vec;
-  int lpr = 1;
+  int lpr = 8;
   while (lpr < units && lpr < 32) lpr <<= 1;
   int nv = (units + lpr - 1) / lpr;
   if (nv == 3) nv = 4;
@@ -1436,7 +1532,7 @@ extern "C" int tllm_paged_attention(
   const int g_tile = mma ? g_even : g_even <= 2 ? g_even : g_even <= 4 ? 4 : 8;
   const int n_y = n_kv * n_gsub;
   const int tile = mma ? (D == 128 ? Tile<128>::KT : Tile<64>::KT)
-                       : kGenWarps * (nv == 1 ? 4 : 2) * (32 / lpr);
+                       : kGenWarps * units_deep(nv) * (32 / lpr);
   TLLM_CHECK_ARG(n_y <= 65535, "%d head groups", n_y);
 
   const long cap = (long)kv->table_cols * kv->page_size;

@@ -131,15 +131,15 @@ __device__ __forceinline__ void store4(uint16_t *p, float4 v) {
   *reinterpret_cast<uint2 *>(p) = r;
 }
 
-// Heads of whole 8-value units on 16-byte rows: one thread takes kUnits units
-// of two runs of four values (a pair's two sides, or eight neighbours), with
-// all its loads issued before the row's page is known. One CTA per row: a row
+// Heads of whole 8-value units on 16-byte rows: one thread takes U units of two
+// runs of four values (a pair's two sides, or eight neighbours), with all its
+// loads issued before the row's page is known. U = 4 for many rows, bound by
+// HBM (12001 rows of 24 / 8 heads of 128: 77 us, 0.89 of its bandwidth; with 2,
+// 81, with 8, 91), U = 2 for few, bound by latency (64 rows: 2.8 us, with 4, 3.4). One CTA per row: a row
 // moves a few KB, and 12 or more CTAs of an SM cover the chain of loads
 // position -> page -> store. HBM-bound: 12001 rows of 24 + 8 + 8 heads of 128
 // read 246 MB and write 197 MB.
-constexpr int kUnits = 4;
-
-template <typename S, typename T>
+template <typename S, typename T, int kUnits>
 __global__ void __launch_bounds__(512)
     append_units_kernel(const __grid_constant__ AppendParams p) {
   griddep_launch();
@@ -218,9 +218,9 @@ __global__ void __launch_bounds__(512)
   }
 }
 
-// Whether every run of four values that the call touches is aligned, and a
-// row fits one CTA.
-bool append_in_units(const AppendParams &p) {
+// Units of a thread, or 0 where a run of four values that the call touches may
+// not be aligned, or a row does not fit one CTA.
+int append_units(const AppendParams &p) {
   const tllm_paged_rows &in = p.in;
   const int src = in.src_dtype == TLLM_F32 ? 4 : 2;
   long strides = in.k_row_stride | in.k_head_stride | in.v_row_stride | in.v_head_stride |
@@ -235,17 +235,18 @@ bool append_in_units(const AppendParams &p) {
   if (in.cos_t)
     ok = ok && ((uintptr_t)in.cos_t | (uintptr_t)in.sin_t) % 16 == 0 && in.rotary_dim % 8 == 0;
   const long units = ((in.q ? in.n_head : 0) + 2L * p.kv.n_kv) * (p.kv.head_dim / 8);
-  return ok && strides % 4 == 0 && p.kv.head_dim % 8 == 0 && units <= 512 * kUnits;
+  if (!ok || strides % 4 || p.kv.head_dim % 8 || units > 512 * 4) return 0;
+  return in.rows <= 4 * sm_count() && units <= 512 * 2 ? 2 : 4;
 }
 
 template <typename S, typename T>
 int launch_append(const AppendParams &p, cudaStream_t st) {
   const int D = p.kv.head_dim, rot = p.in.cos_t ? p.in.rotary_dim : 0;
   const long heads = (p.in.q ? p.in.n_head : 0) + 2L * p.kv.n_kv;
-  if (append_in_units(p)) {
-    const long threads = (heads * (D / 8) + kUnits - 1) / kUnits;
-    TLLM_CUDA(launch_pdl(append_units_kernel<S, T>, dim3(p.in.rows),
-                         dim3((unsigned)((threads + 31) / 32 * 32)), 0, st, p));
+  if (const int units = append_units(p)) {
+    const long threads = (heads * (D / 8) + units - 1) / units;
+    TLLM_CUDA(launch_pdl(units == 2 ? append_units_kernel<S, T, 2> : append_units_kernel<S, T, 4>,
+                         dim3(p.in.rows), dim3((unsigned)((threads + 31) / 32 * 32)), 0, st, p));
     return TLLM_OK;
   }
   const long items = heads * (D - rot / 2);
@@ -266,9 +267,10 @@ struct CopyParams {
 };
 
 // One CTA per (copy, plane). A warp takes pieces of kDeep units per lane of a
-// run, all loaded before the first is stored: 8 warps x 32 lanes x 8 units of
-// 16 bytes keep 32 KB of a CTA in flight.
-constexpr int kCopyWarps = 8, kDeep = 8;
+// run, all loaded before the first is stored: 8 warps x 32 lanes x 16 units of
+// 16 bytes keep 64 KB of a CTA in flight (8 units: forking beams 27.4 us, 16:
+// 26.4; compaction is at the copy bandwidth with either).
+constexpr int kCopyWarps = 8, kDeep = 16;
 
 template <typename U>
 __global__ void __launch_bounds__(kCopyWarps * 32) page_copy_kernel(const CopyParams p) {
