@@ -648,3 +648,29 @@ def test_operators_take_torch_tensors():
     gpu.synchronize()
     want = attend(cache, q.cpu().numpy(), [0, 1], lens)
     assert head_error(out.cpu().numpy().astype(np.float64), want) < F32_TOL
+
+
+@pytest.mark.parametrize("V,k", [(40000, 8), (40000, 64), (128256, 16), (9000, 33)])
+def test_beam_select_clustered_values(V, k):
+    """Large values where they crowd one thread's, warp's or step's share: runs,
+    strides of the kernel's step and sorted rows; equal values across them."""
+    rng = np.random.default_rng(V + k)
+    base = rng.standard_normal((8, V)).astype(np.float32)
+    rows = [np.sort(base[0]), np.sort(base[1])[::-1].copy()]
+    for stride in (4096, 1024, 128, 512):
+        x = base[len(rows)].copy()
+        at = np.arange(stride // 2, V, stride)
+        x[at] = 20 + rng.permutation(len(at)).astype(np.float32) / 8
+        rows.append(x)
+    x = base[6].copy()
+    x[777:777 + 300] = 9 + np.arange(300, dtype=np.float32) / 16
+    rows.append(x)
+    x = np.round(base[7] * 2) / 2           # many equal ones
+    x[:V // 2] = -np.inf
+    rows.append(x)
+    logits = np.stack(rows)
+    # one row a group, so that every row's own order shows
+    s, p, t = run_select(logits, np.zeros((8, 1), np.float32), k)
+    ws, wp, wt = select(logits, np.zeros((8, 1), np.float32), k)
+    assert np.abs(s - ws).max() < 2.0 ** -14
+    assert (t == wt).all()

@@ -9,11 +9,14 @@
 // group to finish joins them. Each logit is read once.
 //
 // Values carry their index in a 64-bit code, so all are distinct and ties are
-// in order. A warp reads 512 values at a time, the next 512 on the way, and
-// lists those above the best bound that a warp of the CTA has found so far (a
-// key that k others reach, so the k largest do too); after the first steps
-// hardly any is, and a value costs a maximum, an exponential and a share of a
-// comparison. Warps meet once, at the end of their part.
+// in order. A thread reads its share of the part with the next 16 values on the
+// way, keeps the maximum and the sum, and remembers its two best steps (of 16
+// values) and the largest value outside them. The k-th largest of the threads'
+// own maxima is a key that the part's k largest reach; the few threads that
+// reach it read those steps again (from L2) and list what does. Bound by HBM
+// while it reads (9 us of 25 for 16 x 8 beams over 128256 tokens, 66 MB), then
+// by the latency of a few dependent passes; a list of candidates kept up during
+// the reading took 31 us, k rounds of maxima over all values 121.
 #include <cmath>
 
 #include "mma_sync.cuh"
@@ -28,9 +31,8 @@ constexpr int kBeamWarps = 8;
 constexpr int kBeamThreads = kBeamWarps * 32;
 constexpr int kPerLane = 16;                          // logits of a lane in one step
 constexpr int kStep = kBeamThreads * kPerLane;        // logits of a CTA in one step
-constexpr int kListed = 128;                          // keys of a warp's list, >= kMaxK + 32
 constexpr int kCtasPerSm = 4;                         // parts are cut for so many
-constexpr int kBatch = 8;                             // listed candidates of a thread
+constexpr int kBatch = 4;                             // listed candidates of a thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxRows = 65535;
 // the groups' tickets lie at the front of the workspace whatever its shape, so
@@ -103,47 +105,30 @@ __device__ __forceinline__ uint64_t block_bound(uint64_t best, int k, uint64_t *
   return bound;
 }
 
-// A warp's list of keys in shared memory, n of them, cut down to its k largest
-// in order: every key goes to the place that the number of larger ones gives.
-// All lanes; returns the new n.
-template <int kSlots>
-__device__ __forceinline__ void cut_slots(uint64_t *list, int n, int k) {
+// The k largest of the warp's 32 keys (all of them for k >= 16) into out, where
+// 32 places are this warp's; returns their number.
+__device__ __forceinline__ int warp_largest(uint64_t key, int k, uint64_t *out) {
   const int lane = threadIdx.x & 31;
-  uint64_t key[kSlots];
-  int rank[kSlots] = {};
-#pragma unroll
-  for (int q = 0; q < kSlots; ++q) key[q] = q * 32 + lane < n ? list[q * 32 + lane] : 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const uint64_t other = list[j];
-#pragma unroll
-    for (int q = 0; q < kSlots; ++q) rank[q] += other > key[q];
+  if (k >= 16) {
+    out[lane] = key;
+    return 32;
   }
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < kSlots; ++q)
-    if (key[q] && rank[q] < k) list[rank[q]] = key[q];
-}
-__device__ __noinline__ int cut_list(uint64_t *list, int n, int k) {
-  __syncwarp();
-  if (n <= 32)
-    cut_slots<1>(list, n, k);
-  else
-    cut_slots<kListed / 32>(list, n, k);
-  __syncwarp();
-  return min(n, k);
-}
-
-// Number of keys larger than `key` in the warps' lists.
-__device__ __forceinline__ int rank_of(const uint64_t *lists, const int *counts, uint64_t key) {
-  int rank = 0;
-  for (int w = 0; w < kBeamWarps; ++w) {
-    const uint64_t *other = lists + w * kListed;
-    const int n = counts[w];
-#pragma unroll 4
-    for (int q = 0; q < n; ++q) rank += other[q] > key;
+  uint32_t left = (uint32_t)(key >> 32);
+  for (int i = 0; i < k; ++i) {
+    const uint32_t top = __reduce_max_sync(~0u, left);
+    if (top == 0) {   // no keys left
+      out[i] = 0;
+      continue;
+    }
+    // equal values: the lower index first
+    const uint32_t tie = left == top ? (uint32_t)key : 0;
+    const uint32_t low = __reduce_max_sync(~0u, tie);
+    if (left == top && tie == low) {
+      out[i] = key;
+      left = 0;
+    }
   }
-  return rank;
+  return k;
 }
 
 __device__ __forceinline__ void keep(uint64_t key, uint64_t *list, int *n) {
@@ -168,12 +153,12 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
   griddep_launch();
   griddep_wait();
   constexpr int kKeys = kBatch * kBeamThreads + kMaxK;
-  static_assert(kBeamWarps * kListed <= kKeys, "the warps' lists use the same memory");
+  static_assert(kBeamWarps * 32 <= kKeys, "the threads' keys use the same memory");
   __shared__ uint64_t s_list[kKeys];
   __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
   __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
-  __shared__ int s_n, s_count[kBeamWarps], s_last;
+  __shared__ int s_n, s_last;
   __shared__ float s_base[kMaxBeams], s_lse[kMaxBeams];
   __shared__ int s_done[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
@@ -182,6 +167,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
 
   if (!(p.done && p.done[row])) {
     const float *x = p.logits + (size_t)row * p.ld;
+    const int begin = chunk * p.chunk + warp * 32 * kPerLane;
     const int end = min(p.vocab, (chunk + 1) * p.chunk);
     // value i of this lane in a step: token t0 + at(i), ascending in i
     auto at = [&](int i) {
@@ -191,7 +177,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       if (kVec && t0 + 32 * kPerLane <= end) {
 #pragma unroll
         for (int i = 0; i < kPerLane; i += 4) {
-          const float4 f = __ldcs(reinterpret_cast<const float4 *>(x + t0 + at(i)));
+          const float4 f = __ldg(reinterpret_cast<const float4 *>(x + t0 + at(i)));
           v[i] = f.x;
           v[i + 1] = f.y;
           v[i + 2] = f.z;
@@ -200,85 +186,14 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       } else {
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i)
-          v[i] = t0 + at(i) < end ? __ldcs(x + t0 + at(i)) : -INFINITY;
+          v[i] = t0 + at(i) < end ? __ldg(x + t0 + at(i)) : -INFINITY;
       }
     };
-    uint64_t *list = s_list + warp * kListed;
-    int n = 0;
-    uint64_t bound = 0;      // keys below it are out
-    float least = -INFINITY; // its value
-    float m = -INFINITY, s = 0.f;   // of this lane's values
-    int t0 = chunk * p.chunk + warp * 32 * kPerLane;
-    auto raise = [&](uint64_t to) {
-      bound = to;
-      least = key_value(to);
-      if (lane == 0) atomicMax(&s_bound, to);
-    };
-    auto follow = [&]() {   // the best bound of the CTA's warps
-      const uint64_t others = *(volatile unsigned long long *)&s_bound;
-      if (others > bound) {
-        bound = others;
-        least = key_value(others);
-      }
-    };
-    // lists the values that reach the bound
-    auto scan = [&](const float (&v)[kPerLane], float top) {
-      if (!__any_sync(~0u, top >= least)) return;
-      uint32_t hits = 0;
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i)
-        if (v[i] >= least) hits |= 1u << i;
-      if (n + (int)__reduce_add_sync(~0u, __popc(hits)) <= kListed) {
-        int *count = &s_count[warp];
-        if (lane == 0) *count = n;
-        __syncwarp();
-        auto add = [&](float x, int i) {
-          const uint64_t key = rank_key(x, (uint32_t)(t0 + at(i)));
-          if (key >= bound && t0 + at(i) < end) list[atomicAdd(count, 1)] = key;
-        };
-        if (__any_sync(~0u, hits & (hits - 1))) {
-          if (hits) {
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i)
-              if (hits >> i & 1) add(v[i], i);
-          }
-        } else if (hits) {
-          add(top, __ffs(hits) - 1);   // a lane's only one is its largest
-        }
-        __syncwarp();
-        n = *count;
-        __syncwarp();
-      } else {
-        // long runs of equal or rising values: in order, cutting the list
-        for (int i = 0; i < kPerLane; ++i) {
-          const int t = t0 + at(i);
-          uint64_t key = 0;
-          if (hits >> i & 1 && t < end) {
-            float x = 0.f;   // v[i], without a copy of v in memory
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) x = j == i ? v[j] : x;
-            key = rank_key(x, (uint32_t)t);
-          }
-          uint32_t in = __ballot_sync(~0u, key && key >= bound);
-          if (!in) continue;
-          if (n + __popc(in) > kListed) {
-            n = cut_list(list, n, k);
-            // (a full list holds more than k; its k-th itself is listed)
-            if (list[k - 1] >= bound) raise(list[k - 1]);
-            in = __ballot_sync(~0u, key && key >= bound && key != list[k - 1]);
-          }
-          if (in >> lane & 1) list[n + __popc(in & ((1u << lane) - 1))] = key;
-          n += __popc(in);
-        }
-      }
-      // a tighter bound once the list has grown
-      if (n >= 2 * k && n > 20) {
-        n = cut_list(list, n, k);
-        if (list[k - 1] > bound) raise(list[k - 1]);
-      }
-    };
-    // maximum and sum of exponentials; returns the largest of v
-    auto sum_up = [&](const float (&v)[kPerLane]) {
+    // maxima of the best step, the second and the others
+    float m = -INFINITY, m2 = -INFINITY, other = -INFINITY;
+    float s = 0.f;                            // sum of 2^((v - m) log2 e)
+    int best = begin, second = begin;
+    auto sum_up = [&](const float (&v)[kPerLane], int t0) {
       float top = v[0];
 #pragma unroll
       for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, v[i]);
@@ -288,51 +203,41 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2(fmaf(v[i], kLog2e, -zero));
       s = s * fast_exp2(fmaf(m, kLog2e, -zero)) + ((add[0] + add[1]) + (add[2] + add[3]));
-      m = mn;
-      return top;
+      if (t0 == begin) {
+        m = top;
+        return;
+      }
+      const bool up = top > m, up2 = top > m2 || (second == begin && best == begin);
+      other = fmaxf(other, up || up2 ? m2 : top);
+      m2 = up ? m : up2 ? top : m2;
+      second = up ? best : up2 ? t0 : second;
+      m = up ? top : m;
+      best = up ? t0 : best;
     };
     // two steps' values are in registers, one in use and one on the way
-    float va[kPerLane], vb[kPerLane];
-    load(t0, va);
-    load(t0 + kStep, vb);
-    if (tid == 0) s_bound = 0;
-    __syncthreads();
     {
-      // the first step: k lanes' own maxima bound the k largest; all warps'
-      // bounds, then the k-th largest of what they have listed
-      const float top = sum_up(va);
-      int first = 0;
+      float va[kPerLane], vb[kPerLane];
+      int t0 = begin;
+      load(t0, va);
+      while (t0 < end) {
+        load(t0 + kStep, vb);
+        sum_up(va, t0);
+        t0 += kStep;
+        if (t0 >= end) break;
+        load(t0 + kStep, va);
+        sum_up(vb, t0);
+        t0 += kStep;
+      }
+    }
+    // this thread's largest key
+    float v[kPerLane];
+    load(best, v);
+    int first = kPerLane;
 #pragma unroll
-      for (int i = kPerLane - 1; i >= 0; --i) first = va[i] == top ? at(i) : first;
-      if (top == -INFINITY) first = at(0);
-      if (k <= 32) {
-        const uint64_t own =
-            warp_bound(t0 + first < end ? rank_key(top, (uint32_t)(t0 + first)) : 0, k);
-        if (own) raise(own);
-      }
-      __syncthreads();
-      follow();
-      scan(va, top);
-      t0 += kStep;
-      if (p.chunk > 2 * kStep) {
-        if (lane == 0) s_count[warp] = n;
-        __syncthreads();
-        for (int i = lane; i < n; i += 32)
-          if (rank_of(s_list, s_count, list[i]) == k - 1) atomicMax(&s_bound, list[i]);
-        __syncthreads();
-      }
-    }
-    while (t0 < end) {
-      load(t0 + kStep, va);
-      follow();
-      scan(vb, sum_up(vb));
-      t0 += kStep;
-      if (t0 >= end) break;
-      load(t0 + kStep, vb);
-      follow();
-      scan(va, sum_up(va));
-      t0 += kStep;
-    }
+    for (int i = kPerLane - 1; i >= 0; --i)
+      if (v[i] == m || (m == -INFINITY && i == 0)) first = i;
+    const bool any = first < kPerLane && best + at(first) < end;
+    const uint64_t mine = any ? rank_key(m, (uint32_t)(best + at(first))) : 0;
     float mm = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
@@ -342,19 +247,91 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     if (lane == 0) {
       s_m[warp] = mm;
       s_s[warp] = s;
-      s_count[warp] = n;
+    }
+    // the k-th largest of all threads' keys (0: fewer than k have one)
+    const int per = warp_largest(mine, k, s_list + warp * 32);
+    if (tid == 0) {
+      s_bound = 0;
+      s_n = 0;
     }
     __syncthreads();
-    // the part's k largest of what its warps have listed
-    uint64_t *out = p.lists + ((size_t)row * p.chunks + chunk) * k;
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) total += s_count[w];
-    for (int i = lane; i < n; i += 32) {
-      const int rank = rank_of(s_list, s_count, list[i]);
-      if (rank < k) out[rank] = list[i];
+    // (four lanes a key, each against two warps' keys)
+    for (int w = warp; w < per; w += kBeamWarps) {
+      const uint64_t key = s_list[(lane >> 2) * 32 + w];
+      int rank = 0;
+#pragma unroll 4
+      for (int q = 0; q < per; ++q) {
+        rank += s_list[(lane & 3) * 64 + q] > key;
+        rank += s_list[(lane & 3) * 64 + 32 + q] > key;
+      }
+      rank += __shfl_xor_sync(~0u, rank, 1);
+      rank += __shfl_xor_sync(~0u, rank, 2);
+      if (rank == k - 1 && key) s_bound = key;
     }
-    for (int i = total + tid; i < k; i += kBeamThreads) out[i] = 0;   // a short last part
+    __syncthreads();
+    const uint64_t bound = s_bound;
+    const float least = bound ? key_value(bound) : -INFINITY;
+    // list the values that reach it; a thread's other steps only if their
+    // largest value may (equal ones do not where the step starts past the
+    // bound's index)
+    if (mine >= bound && any) {
+      auto list = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+          if (!(v[i] >= least) || t0 + at(i) >= end) continue;
+          const uint64_t key = rank_key(v[i], (uint32_t)(t0 + at(i)));
+          if (key < bound) continue;
+          const int to = atomicAdd(&s_n, 1);
+          if (to < kKeys) s_list[to] = key;
+        }
+      };
+      auto may = [&](float top, int t) {
+        return !bound || top > least || (top == least && t <= (int)key_index(bound));
+      };
+      list(best);
+      if (second != best && may(m2, second)) {
+        load(second, v);
+        list(second);
+      }
+      if (may(other, begin)) {
+#pragma unroll 1
+        for (int t = begin; t < end; t += kStep) {
+          if (t == best || t == second) continue;
+          if (!may(other, t)) break;
+          load(t, v);
+          list(t);
+        }
+      }
+    }
+    __syncthreads();
+    uint64_t *out = p.lists + ((size_t)row * p.chunks + chunk) * k;
+    const int n = s_n;
+    if (n <= kKeys) {
+      rank_keys(s_list, n, k, [&](int rank, uint64_t key) { out[rank] = key; });
+      for (int i = n + tid; i < k; i += kBeamThreads) out[i] = 0;   // a short last part
+    } else {
+      // more values above the bound than the list holds (they all lie in the
+      // same threads' shares): k rounds of the largest below the last
+      uint64_t last = ~0ull;
+      for (int j = 0; j < k; ++j) {
+        uint64_t top = 0;
+        for (int t = begin; t < end; t += kStep) {
+          load(t, v);
+#pragma unroll
+          for (int i = 0; i < kPerLane; ++i) {
+            const uint64_t key = t + at(i) < end ? rank_key(v[i], (uint32_t)(t + at(i))) : 0;
+            if (v[i] == v[i] && key < last && key > top) top = key;
+          }
+        }
+        __syncthreads();
+        warp_largest(top, 1, s_warp + warp);
+        __syncthreads();
+        last = 0;
+#pragma unroll
+        for (int w = 0; w < kBeamWarps; ++w) last = s_warp[w] > last ? s_warp[w] : last;
+        if (tid == 0) out[j] = last;
+      }
+    }
     if (tid == 0) {
       float all = -INFINITY, ss = 0.f;
 #pragma unroll
@@ -459,8 +436,10 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     rank_keys(s_list, found, k, [&](int rank, uint64_t code) { s_top[rank] = code; });
     kept = min(found, k);
     __syncthreads();
-    if (tid == 0) s_n = 0;
-    __syncthreads();
+    if (i0 + kBatch * kBeamThreads < n) {
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+    }
   }
   if (tid < k) {
     const uint32_t at = key_index(s_top[tid]);
