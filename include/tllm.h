@@ -318,8 +318,9 @@ int tllm_paged_attention(const tllm_paged_kv *kv, const float *q,
  * plain order. lens_out (may be NULL): raised to row_pos + 1 at the row's
  * sequence where it is lower (rows may come in any order).
  * Strides in elements. A row whose position is outside the table's capacity
- * or n_pos, or whose sequence or page is out of range, is skipped and sets
- * bit 32 of the device error word. Two rows must not name the same token.
+ * or n_pos, or whose sequence, page or source row is out of range, is skipped
+ * and sets bit 32 of the device error word. Two rows must not name the same
+ * token.
  * Replaces, for pages, triton_llm/kernels/rope.py:153-222 and the cache write
  * of smollm2_triton/model.py:296-308.
  */
@@ -345,7 +346,7 @@ typedef struct {
   int n_pos;
   int interleaved;
   int blocked;
-  int reserved;           /* 0 */
+  int src_rows;           /* rows of q, k and v, bounds row_src (0: not checked) */
 } tllm_paged_rows;
 int tllm_paged_append(const tllm_paged_kv *kv, const tllm_paged_rows *rows,
                       tllm_stream_t stream);

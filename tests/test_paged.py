@@ -157,6 +157,9 @@ def test_append_refusals(kw, msg):
     ((3, 2, 64), (2, 2, 64), (3,), {}, "v has 2 rows"),
     ((3, 2, 64), (3, 2, 64), (3,), dict(row_stride=64), "go together"),
     ((3, 2, 64), (3, 2, 64), (3, 1), {}, "1D"),
+    ((3, 2, 64), (3, 2, 64), (4,), dict(row_stride=128, head_stride=64), "4 rows of 3 source"),
+    ((1, 1, 64), (3, 2, 64), (3,), dict(row_stride=128, head_stride=64), "no row"),
+    ((3, 2, 64), (3, 2, 64), (3,), dict(row_stride=0, head_stride=64), "row_stride"),
 ])
 def test_write_refusals(k, v, pos, kw, msg):
     with pytest.raises(ValueError, match=msg):

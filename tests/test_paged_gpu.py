@@ -447,6 +447,21 @@ def test_write_from_a_contiguous_cache(src_dtype, dtype):
         assert (got == want).all()
 
 
+@pytest.mark.parametrize("P", [16, 7])
+def test_write_skips_source_rows_out_of_range(P):
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((3, 2, 64)).astype(np.float32)
+    zero = np.zeros((4, 2, P, 64), np.float32)
+    kv = PagedKV(gpu.to_device(zero), gpu.to_device(zero), i32([[0, 1], [2, 3]]))
+    gpu.device_error(reset=True)
+    paged_write(kv, gpu.to_device(x), gpu.to_device(x), i32([0, 1, 2, 3]),
+                row_seq=i32([0, 0, 1, 1]), row_src=i32([2, 3, -1, 0]))
+    assert gpu.device_error() == 32
+    want = zero.copy()
+    want[0, :, 0], want[2, :, 3] = x[2], x[0]
+    assert (kv.k.to_numpy() == want).all() and (kv.v.to_numpy() == want).all()
+
+
 # -- page copies ------------------------------------------------------------
 @pytest.mark.parametrize("dtype,shape,slots_first", [
     ("bf16", (4, 20, 3, 16, 64), False), ("f32", (2, 20, 8, 5, 128), False),

@@ -30,6 +30,10 @@ __device__ __forceinline__ int source_dim(int d, int D, int blocked) {
   return d < half ? (d >> 3) * 16 + (d & 7) : ((d - half) >> 3) * 16 + 8 + ((d - half) & 7);
 }
 
+__device__ __forceinline__ bool source_ok(const AppendParams &p, int src) {
+  return src >= 0 && (p.in.src_rows == 0 || src < p.in.src_rows);
+}
+
 // Row `row` of the call: cache row index, position, page, slot; false (and an
 // error bit) where an index is out of range.
 struct AppendRow {
@@ -39,8 +43,9 @@ struct AppendRow {
 __device__ __forceinline__ bool append_row(const AppendParams &p, int row, AppendRow *r) {
   r->seq = p.in.row_seq ? p.in.row_seq[row] : row;
   r->pos = p.in.row_pos[row];
-  r->src = p.in.row_src ? p.in.row_src[row] : row;
-  bool ok = r->seq >= 0 && r->seq < p.kv.n_seq && r->pos >= 0 &&
+  const int src = p.in.row_src ? p.in.row_src[row] : row;
+  r->src = src;
+  bool ok = source_ok(p, src) && r->seq >= 0 && r->seq < p.kv.n_seq && r->pos >= 0 &&
             r->pos < p.kv.table_cols * p.kv.page_size &&
             (!p.in.cos_t || r->pos < p.in.n_pos);
   if (ok) {
@@ -148,7 +153,8 @@ __global__ void __launch_bounds__(512)
   const int D = p.kv.head_dim, H = p.in.q ? p.in.n_head : 0, K = p.kv.n_kv;
   const int rot = p.in.cos_t ? p.in.rotary_dim : 0, half = rot >> 1;
   const unsigned per = D >> 3, n = (H + 2 * K) * per;
-  const size_t from = p.in.row_src ? p.in.row_src[row] : row;
+  const int src_row = p.in.row_src ? p.in.row_src[row] : row;
+  const size_t from = source_ok(p, src_row) ? src_row : 0;   // (else skipped below)
   float4 x[kUnits], y[kUnits];
   // runs a and b of unit u of a head
   auto runs = [&](int head, int u, int *a, int *b) {
@@ -316,7 +322,10 @@ extern "C" int tllm_paged_append(const tllm_paged_kv *kv, const tllm_paged_rows 
   if (rc) return rc;
   TLLM_CHECK_ARG(in, "rows is NULL");
   const int D = kv->head_dim;
-  TLLM_CHECK_ARG(in->rows >= 0, "rows (%d) must be >= 0", in->rows);
+  TLLM_CHECK_ARG(in->rows >= 0 && in->src_rows >= 0, "rows (%d) and src_rows (%d) must be >= 0",
+                 in->rows, in->src_rows);
+  TLLM_CHECK_ARG(in->row_src || in->src_rows == 0 || in->rows <= in->src_rows,
+                 "%d rows of %d source rows", in->rows, in->src_rows);
   TLLM_CHECK_ARG(in->src_dtype == TLLM_F32 || in->src_dtype == TLLM_BF16,
                  "src_dtype must be F32 or BF16");
   TLLM_CHECK_ARG(!in->q || in->n_head > 0, "n_head (%d) must be > 0", in->n_head);

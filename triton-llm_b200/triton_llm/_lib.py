@@ -177,7 +177,7 @@ class PagedRowsStruct(ctypes.Structure):
                 ("k_row_stride", _l), ("k_head_stride", _l), ("v_row_stride", _l),
                 ("v_head_stride", _l), ("q_out_row_stride", _l), ("q_out_head_stride", _l),
                 ("src_dtype", _i), ("rows", _i), ("n_head", _i), ("rotary_dim", _i),
-                ("n_pos", _i), ("interleaved", _i), ("blocked", _i), ("reserved", _i)]
+                ("n_pos", _i), ("interleaved", _i), ("blocked", _i), ("src_rows", _i)]
 
 
 EL_SWIGLU, EL_ADD, EL_GELU = 0, 1, 2

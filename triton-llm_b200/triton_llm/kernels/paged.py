@@ -17,6 +17,7 @@ to be ordered by the caller.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 
@@ -143,7 +144,8 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
               window > 0: a row sees its last ``window`` keys and the first
               ``sinks`` ones; pages outside them are not read
     workspace PagedWorkspace, needed with ``stream``; without one the library
-              stream's own is used
+              stream's own is used (made by the first call of a shape: before a
+              graph capture, not in it)
 
     A row without a visible key gives zeros. Returns ``out``.
     """
@@ -237,7 +239,7 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
         _index(row_pos, "row_pos", n),
         None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
         cos_t, sin_t, ld, D, ld, D, ld, D, n_head * D, D, _lib.F32, n, n_head, rotary,
-        n_pos, bool(interleaved), bool(blocked))
+        n_pos, bool(interleaved), bool(blocked), int(qkv.shape[0]))
     _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
     return q_out
 
@@ -272,8 +274,17 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
         sk, sv = strides(k), strides(v)
         if sk[2] != 1 or sv[2] != 1:
             raise ValueError("the last axis of k and v must be contiguous")
+        src_rows = min(int(k.shape[0]), int(v.shape[0]))
     else:
         sk = sv = (int(row_stride), int(head_stride))
+        if sk[0] < 1 or sk[1] < 0:
+            raise ValueError(f"row_stride ({sk[0]}) must be >= 1, head_stride ({sk[1]}) >= 0")
+        for t, name in ((k, "k"), (v, "v")):
+            on_device(t, name)
+        values = min(math.prod(k.shape), math.prod(v.shape))
+        src_rows = max(0, values - (kv.n_kv_head - 1) * sk[1] - kv.head_dim + sk[0]) // sk[0]
+        if n and src_rows == 0:
+            raise ValueError("k and v hold no row of these strides")
     require_gpu(k, "k")
     require_gpu(v, "v")
     cos_t, sin_t, n_pos, rotary = _tables(cos, sin)
@@ -282,7 +293,7 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
         _index(row_seq, "row_seq", n), _index(row_pos, "row_pos", n),
         None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
         cos_t, sin_t, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0, code, n, 0, rotary, n_pos,
-        bool(interleaved), 0)
+        bool(interleaved), 0, src_rows)
     _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
 
 
