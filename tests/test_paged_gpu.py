@@ -387,6 +387,28 @@ def test_append(H, K, D, rot, P, blocked, slots_first, interleaved, dtype):
     assert lens.to_numpy().tolist() == [3, P + 1, 42, 3 * P]
 
 
+def test_append_many_rows():
+    """72 MB of results (stored as streams), neighbouring pairs, half a head."""
+    H, K, D, P, R = 24, 8, 128, 16, 3531
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((R, H + 2 * K, D), dtype=np.float32)
+    pages = rng.permutation(R // P + 1).reshape(1, -1).astype(np.int32)
+    zero = np.zeros((R // P + 1, K, P, D), np.float32)
+    kv = PagedKV(up(zero, "bf16"), up(zero, "bf16"), i32(pages))
+    cos, sin = tables(R, 64)
+    qo, pos = gpu.allocate((R, H, D), np.float32), np.arange(R)
+    paged_append(kv, gpu.to_device(x.reshape(R, -1)), i32(pos), qo, gpu.to_device(cos),
+                 gpu.to_device(sin), n_head=H, row_seq=i32(np.zeros(R)), interleaved=True)
+    norm = np.abs(x).max() * np.sqrt(2)
+    want = rotate(x[:, :H + K], cos, sin, True)
+    assert np.abs(qo.to_numpy() - want[:, :H]).max() <= 3 * 2.0 ** -24 * norm
+    page, slot = pages[0, pos // P], pos % P
+    k, v = gpu.to_host(kv.k)[page, :, slot], gpu.to_host(kv.v)[page, :, slot]
+    assert (np.abs(k - want[:, H:]) <= 2.0 ** -8 * np.abs(want[:, H:]) + 3 * 2.0 ** -24
+            * norm).all()
+    assert (v == bf16(x[:, H + K:])).all()
+
+
 def test_append_in_place_and_bad_rows():
     """q rotated in place; rows with a bad index are skipped and reported."""
     H, K, D, P, R = 4, 2, 64, 16, 6

@@ -12,6 +12,7 @@ namespace {
 struct AppendParams {
   PagedView kv;
   tllm_paged_rows in;
+  bool stream;   // the results do not stay in L2
   int *err;
 };
 
@@ -126,24 +127,30 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
   const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(p));
   return make_float4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y));
 }
-__device__ __forceinline__ void store4(float *p, float4 v) {
-  *reinterpret_cast<float4 *>(p) = v;
+// (`stream`: not kept in L2)
+__device__ __forceinline__ void store4(float *p, float4 v, bool stream) {
+  if (stream)
+    __stcs(reinterpret_cast<float4 *>(p), v);
+  else
+    *reinterpret_cast<float4 *>(p) = v;
 }
-__device__ __forceinline__ void store4(uint16_t *p, float4 v) {
+__device__ __forceinline__ void store4(uint16_t *p, float4 v, bool stream) {
   uint2 r;
   r.x = (uint32_t)f32_to_bf16_bits(v.x) | (uint32_t)f32_to_bf16_bits(v.y) << 16;
   r.y = (uint32_t)f32_to_bf16_bits(v.z) | (uint32_t)f32_to_bf16_bits(v.w) << 16;
-  *reinterpret_cast<uint2 *>(p) = r;
+  if (stream)
+    __stcs(reinterpret_cast<uint2 *>(p), r);
+  else
+    *reinterpret_cast<uint2 *>(p) = r;
 }
 
 // Heads of whole 8-value units on 16-byte rows: one thread takes U units of two
 // runs of four values (a pair's two sides, or eight neighbours), with all its
-// loads issued before the row's page is known. U = 4 for many rows, bound by
-// HBM (12001 rows of 24 / 8 heads of 128: 77 us, 0.89 of its bandwidth; with 2,
-// 81, with 8, 91), U = 2 for few, bound by latency (64 rows: 2.8 us, with 4, 3.4). One CTA per row: a row
-// moves a few KB, and 12 or more CTAs of an SM cover the chain of loads
-// position -> page -> store. HBM-bound: 12001 rows of 24 + 8 + 8 heads of 128
-// read 246 MB and write 197 MB.
+// loads issued before the row's page is known. U = 4 for many rows, bound by HBM
+// (12001 rows of 24 / 8 heads of 128: 73 us, 0.94 of its bandwidth; with 2 or 8
+// units 4 and 17 % more), U = 2 for few, bound by latency (64 rows: 2.8 us, with
+// 4, 3.4). One CTA per row: a row moves a few KB, and 12 or more CTAs of an SM
+// cover the chain of loads position -> page -> store.
 template <typename S, typename T, int kUnits>
 __global__ void __launch_bounds__(512)
     append_units_kernel(const __grid_constant__ AppendParams p) {
@@ -212,14 +219,14 @@ __global__ void __launch_bounds__(512)
     if (head < H) {
       float *to = p.in.q_out + (size_t)row * p.in.q_out_row_stride +
                   (size_t)head * p.in.q_out_head_stride;
-      store4(to + a, x[i]);
-      store4(to + b, y[i]);
+      store4(to + a, x[i], p.stream);
+      store4(to + b, y[i], p.stream);
     } else {
       const bool is_v = head >= H + K;
       T *to = static_cast<T *>(is_v ? p.kv.v : p.kv.k) +
               p.kv.offset(r.page, head - H - (is_v ? K : 0), r.slot);
-      store4(to + a, x[i]);
-      store4(to + b, y[i]);
+      store4(to + a, x[i], p.stream);
+      store4(to + b, y[i], p.stream);
     }
   }
 }
@@ -246,11 +253,15 @@ int append_units(const AppendParams &p) {
 }
 
 template <typename S, typename T>
-int launch_append(const AppendParams &p, cudaStream_t st) {
+int launch_append(AppendParams &p, cudaStream_t st) {
   const int D = p.kv.head_dim, rot = p.in.cos_t ? p.in.rotary_dim : 0;
   const long heads = (p.in.q ? p.in.n_head : 0) + 2L * p.kv.n_kv;
   if (const int units = append_units(p)) {
     const long threads = (heads * (D / 8) + units - 1) / units;
+    // Results of about the size of L2 (126 MB) would only push one another out:
+    // past half of it they are stored as streams (12001 rows, 197 MB: 78 -> 73
+    // us); smaller ones stay for the attention that reads them next.
+    p.stream = (long)p.in.rows * D * (heads * 4L) > 64L << 20;
     TLLM_CUDA(launch_pdl(units == 2 ? append_units_kernel<S, T, 2> : append_units_kernel<S, T, 4>,
                          dim3(p.in.rows), dim3((unsigned)((threads + 31) / 32 * 32)), 0, st, p));
     return TLLM_OK;
