@@ -669,13 +669,14 @@ __device__ __noinline__ void join_parts(const AttnParams &p, size_t base, int n,
   for (int j = 0; j < kMost; ++j) r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < n; i0 += batch) {
     const int m = min(batch, n - i0);
-    for (int i = tid; i < m * cols; i += THREADS) {
-      const int part = i / cols;
-      const float4 *from =
-          acc + part_slot(base + i0 + part, i0 + part == 0) * step + (i - part * cols);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + i)),
-                   "l"(from)
-                   : "memory");
+    for (int k = warp; k < m; k += THREADS / 32) {   // (a warp per part)
+      const float4 *from = acc + part_slot(base + i0 + k, i0 + k == 0) * step;
+      const uint32_t to = smem_u32(ring + k * cols);
+#pragma unroll 1
+      for (int c = tid & 31; c < cols; c += 32)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + c * 16),
+                     "l"(from + c)
+                     : "memory");
     }
     if (i0 == 0) {
       for (int h = warp; h < G; h += THREADS / 32) {
