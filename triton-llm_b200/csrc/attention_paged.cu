@@ -494,6 +494,7 @@ constexpr int kStages = 3;
 constexpr int kRowBlock = 512;   // rows that share one axis (and one grid row)
 constexpr int kMaxPerSm = 2;     // CTAs that the shared memory lets an SM hold
 constexpr int kSegs = 2;         // segments announced to the consumers
+constexpr int kSegTiles = 2;     // tiles that a CTA reads in the time of a segment's end
 constexpr int kMinTiles = 2;     // least tiles of a share
 constexpr int kJoinTiles = 4;    // tiles that a CTA reads in the time of a join
 
@@ -573,10 +574,13 @@ __device__ __forceinline__ PageSpan page_span(const AttnParams &p, int len, int 
   return g;
 }
 
-// The tiles of all (row, head group) pairs, in that order, are one axis, cut
-// into equal shares, one for each CTA. The part of a pair that lies in one
-// share is a segment: a share holds the end of one pair, some whole ones and
-// the start of another. (Short intervals at the end of the shares, for the CTAs
+// The tiles of all (row, head group) pairs, in that order, are one axis, with
+// kSegTiles idle places after each pair for the time that its end takes (32 rows
+// of 100 to 2048 keys, 32 heads of 64: 87.7 us without them, 56.6 with one place,
+// 53.6 with two, 54.2 with three). It is cut into equal
+// shares, one for each CTA. The part of a pair that lies in one share is a
+// segment: a share holds the end of one pair, some whole ones and the start of
+// another. (Short intervals at the end of the shares, for the CTAs
 // that are done first, balance the SMs' bandwidth, but every further segment
 // costs its CTA about 2 us and its pair's join 0.15 us: 64 x 24/8/128 took 200
 // us with them and 192 without, one row of 131071 keys 93 and 96.)
@@ -805,7 +809,8 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   }
   griddep_wait();
 
-  // ---- tiles of every row, summed up (a row without keys has one, empty)
+  // ---- places of every row's pairs, summed up (a row without keys has a tile,
+  // empty)
   const int per = (nrows + T::THREADS - 1) / T::THREADS;
   int sum = 0, most = 0;
   for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
@@ -822,11 +827,11 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     }
     if (len < 0) len = 0;
     int xs, xa;
-    const int nt = max(1, (page_span(p, len, &xs, &xa).n + KT - 1) / KT);
+    const int places = max(1, (page_span(p, len, &xs, &xa).n + KT - 1) / KT) + kSegTiles;
     s_len[i] = len;
-    s_cum[i] = nt;
-    sum += nt;
-    most = max(most, nt);
+    s_cum[i] = places;
+    sum += places;
+    most = max(most, places);
   }
   int scan = sum;
 #pragma unroll
@@ -848,9 +853,9 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     most = max(most, s_warp[1][w]);
   }
   for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
-    const int nt = s_cum[i];
+    const int places = s_cum[i];
     s_cum[i] = before;
-    before += nt;
+    before += places;
   }
   if (tid == 0) s_cum[nrows] = total;
   __syncthreads();
@@ -860,7 +865,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   const int ncta = gridDim.x;
   const long work = (long)total * p.n_y;
   int share = (int)((work + ncta - 1) / ncta);
-  if (share < kMinTiles) share = kMinTiles;
+  if (share < kMinTiles + kSegTiles) share = kMinTiles + kSegTiles;
   const bool whole_pairs = (long)nrows * p.n_y <= ncta && most <= share + kJoinTiles;
   const size_t base = (size_t)blockIdx.y * ncta;   // of the shares
   const int P = p.kv.page_size, box = min(P, KT);   // slots of one load
@@ -927,13 +932,14 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         }
       }
     };
+    auto tiles_of = [&](int row) { return s_cum[row + 1] - s_cum[row] - kSegTiles; };
     Segment g;
     if (whole_pairs) {
       if (blockIdx.x < nrows * p.n_y) {
         g.row = blockIdx.x / p.n_y;
         g.y = blockIdx.x - g.row * p.n_y;
         g.t0 = 0;
-        g.t1 = s_cum[g.row + 1] - s_cum[g.row];
+        g.t1 = tiles_of(g.row);
         g.parts = 1;
         stream(g);
       }
@@ -946,22 +952,24 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         if ((long)s_cum[mid] * p.n_y <= w) lo = mid; else hi = mid;
       }
       g.row = lo;
-      int nt = s_cum[lo + 1] - s_cum[lo];
+      int nt = tiles_of(lo);
       const int rem = (int)(w - (long)s_cum[lo] * p.n_y);
-      g.y = rem / nt;
-      g.t0 = rem - g.y * nt;
+      g.y = rem / (nt + kSegTiles);
+      g.t0 = rem - g.y * (nt + kSegTiles);
       while (w < w1 && !failed) {
-        g.t1 = (int)min((long)nt, g.t0 + w1 - w);
-        const long begin = w - g.t0;
-        g.first = (int)(begin / share);
-        g.parts = (int)((begin + nt - 1) / share) - g.first + 1;
-        stream(g);
-        w += g.t1 - g.t0;
+        const long begin = w - g.t0;   // of the pair
+        if (g.t0 < nt) {
+          g.t1 = (int)min((long)nt, g.t0 + w1 - w);
+          g.first = (int)(begin / share);
+          g.parts = (int)((begin + nt - 1) / share) - g.first + 1;
+          stream(g);
+        }
+        w = begin + nt + kSegTiles;
         g.t0 = 0;
         if (++g.y == p.n_y) {
           g.y = 0;
           ++g.row;
-          if (g.row < nrows) nt = s_cum[g.row + 1] - s_cum[g.row];
+          if (g.row < nrows) nt = tiles_of(g.row);
         }
       }
     }
