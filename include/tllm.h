@@ -291,15 +291,28 @@ typedef struct {
 int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_head,
                                    int head_dim, size_t *partial_bytes,
                                    size_t *counter_bytes);
-int tllm_paged_attention(const tllm_paged_kv *kv, const float *q,
-                         long q_row_stride, long q_head_stride,
-                         const int32_t *row_seq, const int32_t *row_len,
-                         void *out, int out_dtype, long out_plane_rows,
-                         long out_row_stride, long out_head_stride, int rows,
-                         int n_head, int max_len, long keys_hint, int window,
-                         int sinks, float sm_scale, void *partial,
-                         size_t partial_bytes, int32_t *counters,
-                         size_t counter_bytes, tllm_stream_t stream);
+typedef struct {
+  const float *q;
+  const int32_t *row_seq;  /* or NULL */
+  const int32_t *row_len;
+  void *out;
+  void *partial;
+  int32_t *counters;
+  size_t partial_bytes, counter_bytes;
+  long q_row_stride, q_head_stride;
+  long out_plane_rows, out_row_stride, out_head_stride;
+  long keys_hint;
+  int out_dtype;           /* F32, BF16 or SPLIT */
+  int rows;
+  int n_head;
+  int max_len;
+  int window;
+  int sinks;
+  float sm_scale;          /* <= 0: 1/sqrt(head_dim) */
+  int reserved;            /* 0 */
+} tllm_paged_attn;
+int tllm_paged_attention(const tllm_paged_kv *kv, const tllm_paged_attn *args,
+                         tllm_stream_t stream);
 
 /*
  * New tokens into a paged cache, with rotary positions. Row r of q

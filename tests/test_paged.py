@@ -38,7 +38,7 @@ class Fake:
 
 
 class Scratch:
-    partial = counters = None
+    partial = counters = 0
     partial_bytes = counter_bytes = 0
 
 

@@ -1489,17 +1489,24 @@ extern "C" int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_hea
   return TLLM_OK;
 }
 
-extern "C" int tllm_paged_attention(
-    const tllm_paged_kv *kv, const float *q, long q_row_stride, long q_head_stride,
-    const int32_t *row_seq, const int32_t *row_len, void *out, int out_dtype,
-    long out_plane_rows, long out_row_stride, long out_head_stride, int rows,
-    int n_head, int max_len, long keys_hint, int window, int sinks, float sm_scale,
-    void *partial, size_t partial_bytes, int32_t *counters, size_t counter_bytes,
-    tllm_stream_t stream) {
+extern "C" int tllm_paged_attention(const tllm_paged_kv *kv, const tllm_paged_attn *a,
+                                    tllm_stream_t stream) {
   TLLM_INJECT("launch");
   AttnParams p;
   int rc = paged_view(kv, &p.kv);
   if (rc) return rc;
+  TLLM_CHECK_ARG(a, "args is NULL");
+  const float *q = a->q;
+  void *out = a->out, *partial = a->partial;
+  const int32_t *row_seq = a->row_seq, *row_len = a->row_len;
+  int32_t *counters = a->counters;
+  const size_t partial_bytes = a->partial_bytes, counter_bytes = a->counter_bytes;
+  const long q_row_stride = a->q_row_stride, q_head_stride = a->q_head_stride;
+  const long out_plane_rows = a->out_plane_rows, out_row_stride = a->out_row_stride;
+  const long out_head_stride = a->out_head_stride, keys_hint = a->keys_hint;
+  const int out_dtype = a->out_dtype, rows = a->rows, n_head = a->n_head;
+  const int max_len = a->max_len, window = a->window, sinks = a->sinks;
+  float sm_scale = a->sm_scale;
   const int D = kv->head_dim, n_kv = kv->n_kv_head, P = kv->page_size;
   TLLM_CHECK_ARG(rows >= 0 && n_head > 0, "invalid rows %d / n_head %d", rows, n_head);
   TLLM_CHECK_ARG(n_head % n_kv == 0, "n_head (%d) must be divisible by n_kv_head (%d)",

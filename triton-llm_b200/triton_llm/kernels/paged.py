@@ -163,7 +163,7 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     if n_head % kv.n_kv_head:
         raise ValueError(f"n_head ({n_head}) must be divisible by n_kv_head ({kv.n_kv_head})")
     lens = on_device(row_len, "row_len", _lib.I32, (rows,))
-    seq = None if row_seq is None else on_device(row_seq, "row_seq", _lib.I32, (rows,))
+    seq = 0 if row_seq is None else on_device(row_seq, "row_seq", _lib.I32, (rows,))
     if workspace is None:
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
@@ -173,17 +173,18 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
         workspace = _workspace(
             lambda: PagedWorkspace(n, n_head, kv.n_kv_head, kv.head_dim),
             "attention", kv.device, n, n_head, kv.n_kv_head, kv.head_dim)
-    _lib.call("tllm_paged_attention", kv._ref, q.data_ptr(), sq[0], sq[1], seq, lens, o[0],
-              o[1], o[2], o[3], o[4], rows, n_head, int(max_len), int(keys_hint),
-              int(window), int(sinks), float(sm_scale or 0.0), workspace.partial,
-              workspace.partial_bytes, workspace.counters, workspace.counter_bytes, stream)
+    _lib.call("tllm_paged_attention", kv._ref, _lib.PAGED_ATTN.pack(
+        q.data_ptr(), seq, lens, o[0], workspace.partial, workspace.counters,
+        workspace.partial_bytes, workspace.counter_bytes, sq[0], sq[1], o[2], o[3], o[4],
+        int(keys_hint), o[1], rows, n_head, int(max_len), int(window), int(sinks),
+        float(sm_scale or 0.0), 0), stream)
     return out
 
 
 def _tables(cos, sin):
     """(cos, sin, positions, rotary values) of rotary tables, zeros for none."""
     if cos is None and sin is None:
-        return None, None, 0, 0
+        return 0, 0, 0, 0
     if cos is None or sin is None:
         raise ValueError("cos and sin go together")
     shape = cos.shape
@@ -195,7 +196,7 @@ def _tables(cos, sin):
 
 
 def _index(t, name, n):
-    return None if t is None else on_device(t, name, _lib.I32, (n,))
+    return 0 if t is None else on_device(t, name, _lib.I32, (n,))
 
 
 def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq=None,
@@ -233,14 +234,14 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
         raise ValueError(f"q_out must be ({n}, {n_head}, {D}), got {tuple(shape)}")
     cos_t, sin_t, n_pos, rotary = _tables(cos, sin)
     at = qkv.data_ptr()
-    r = _lib.PagedRowsStruct(
+    r = _lib.PAGED_ROWS.pack(
         at, at + n_head * D * 4, at + (n_head + K) * D * 4,
-        on_device(q_out, "q_out", _lib.F32), None, _index(row_seq, "row_seq", n),
+        on_device(q_out, "q_out", _lib.F32), 0, _index(row_seq, "row_seq", n),
         _index(row_pos, "row_pos", n),
-        None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        0 if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
         cos_t, sin_t, ld, D, ld, D, ld, D, n_head * D, D, _lib.F32, n, n_head, rotary,
         n_pos, bool(interleaved), bool(blocked), int(qkv.shape[0]))
-    _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
+    _lib.call("tllm_paged_append", kv._ref, r, stream)
     return q_out
 
 
@@ -288,13 +289,13 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
     require_gpu(k, "k")
     require_gpu(v, "v")
     cos_t, sin_t, n_pos, rotary = _tables(cos, sin)
-    r = _lib.PagedRowsStruct(
-        None, k.data_ptr(), v.data_ptr(), None, _index(row_src, "row_src", n),
+    r = _lib.PAGED_ROWS.pack(
+        0, k.data_ptr(), v.data_ptr(), 0, _index(row_src, "row_src", n),
         _index(row_seq, "row_seq", n), _index(row_pos, "row_pos", n),
-        None if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        0 if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
         cos_t, sin_t, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0, code, n, 0, rotary, n_pos,
         bool(interleaved), 0, src_rows)
-    _lib.call("tllm_paged_append", kv._ref, ctypes.addressof(r), stream)
+    _lib.call("tllm_paged_append", kv._ref, r, stream)
 
 
 def page_copy(arena, src, dst, fill=None, slots_first=False, stream=None):
