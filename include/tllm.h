@@ -402,11 +402,22 @@ int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
  * greedily or by sampling (smollm2_triton/model.py:566-584).
  */
 int tllm_beam_workspace(int groups, int beams, int vocab, int k, size_t *bytes);
-int tllm_beam_select(const float *logits, long ld, const float *scores,
-                     const int32_t *done, int pad_token, int groups, int beams,
-                     int vocab, int k, float *out_scores, int32_t *out_parents,
-                     int32_t *out_tokens, int eos_token, int32_t *out_done,
-                     void *workspace, size_t workspace_bytes, tllm_stream_t stream);
+typedef struct {
+  const float *logits;
+  const float *scores;
+  const int32_t *done;      /* or NULL */
+  float *out_scores;
+  int32_t *out_parents;
+  int32_t *out_tokens;
+  int32_t *out_done;        /* or NULL */
+  void *workspace;
+  size_t workspace_bytes;
+  long ld;
+  int groups, beams, vocab, k;
+  int pad_token;
+  int eos_token;            /* -1: none */
+} tllm_beam_step;
+int tllm_beam_select(const tllm_beam_step *step, tllm_stream_t stream);
 
 /*
  * Page tables after a selection step: beam i of group g continues beam
@@ -424,11 +435,15 @@ int tllm_beam_select(const float *logits, long ld, const float *scores,
  * table_in. Parents or lengths out of range leave their group's tables as
  * they were, name no copies and set bit 32 of the device error word.
  */
-int tllm_beam_reorder(const int32_t *parents, const int32_t *lens,
-                      const int32_t *table_in, int32_t *table_out, int groups,
-                      int beams, int table_cols, int page_size,
-                      int32_t *copy_src, int32_t *copy_dst, int32_t *copy_fill,
-                      tllm_stream_t stream);
+typedef struct {
+  const int32_t *parents;   /* (groups, beams) */
+  const int32_t *lens;      /* (groups * beams) */
+  const int32_t *table_in;  /* (groups * beams, table_cols) */
+  int32_t *table_out;
+  int32_t *copy_src, *copy_dst, *copy_fill;   /* (groups * beams) each */
+  int groups, beams, table_cols, page_size;
+} tllm_beam_tables;
+int tllm_beam_reorder(const tllm_beam_tables *tables, tllm_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Projections (GEMM with fused epilogues)                                   */

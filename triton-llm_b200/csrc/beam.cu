@@ -554,13 +554,18 @@ extern "C" int tllm_beam_workspace(int groups, int beams, int vocab, int k, size
   return TLLM_OK;
 }
 
-extern "C" int tllm_beam_select(const float *logits, long ld, const float *scores,
-                                const int32_t *done, int pad_token, int groups, int beams,
-                                int vocab, int k, float *out_scores, int32_t *out_parents,
-                                int32_t *out_tokens, int eos_token, int32_t *out_done,
-                                void *workspace, size_t workspace_bytes,
-                                tllm_stream_t stream) {
+extern "C" int tllm_beam_select(const tllm_beam_step *step, tllm_stream_t stream) {
   TLLM_INJECT("launch");
+  TLLM_CHECK_ARG(step, "step is NULL");
+  const float *logits = step->logits, *scores = step->scores;
+  const int32_t *done = step->done;
+  float *out_scores = step->out_scores;
+  int32_t *out_parents = step->out_parents, *out_tokens = step->out_tokens;
+  void *workspace = step->workspace;
+  const size_t workspace_bytes = step->workspace_bytes;
+  const long ld = step->ld;
+  const int groups = step->groups, beams = step->beams, vocab = step->vocab, k = step->k;
+  const int pad_token = step->pad_token;
   size_t need = 0;
   int rc = tllm_beam_workspace(groups, beams, vocab, k, &need);
   if (rc) return rc;
@@ -586,8 +591,8 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   p.out_scores = out_scores;
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;
-  p.eos = eos_token;
-  p.out_done = out_done;
+  p.eos = step->eos_token;
+  p.out_done = step->out_done;
   char *w = static_cast<char *>(workspace);
   p.counters = reinterpret_cast<int *>(w);
   w += kCounterBytes;
@@ -601,31 +606,30 @@ extern "C" int tllm_beam_select(const float *logits, long ld, const float *score
   return TLLM_OK;
 }
 
-extern "C" int tllm_beam_reorder(const int32_t *parents, const int32_t *lens,
-                                 const int32_t *table_in, int32_t *table_out, int groups,
-                                 int beams, int table_cols, int page_size,
-                                 int32_t *copy_src, int32_t *copy_dst, int32_t *copy_fill,
-                                 tllm_stream_t stream) {
+extern "C" int tllm_beam_reorder(const tllm_beam_tables *t, tllm_stream_t stream) {
   TLLM_INJECT("launch");
+  TLLM_CHECK_ARG(t, "tables is NULL");
+  const int groups = t->groups, beams = t->beams, table_cols = t->table_cols;
+  const int page_size = t->page_size;
   TLLM_CHECK_ARG(groups >= 0 && beams >= 1 && beams <= kMaxBeams,
                  "groups (%d) must be >= 0 and beams (%d) in [1, %d]", groups, beams, kMaxBeams);
   TLLM_CHECK_ARG(table_cols >= 0 && page_size >= 1, "invalid table: %d columns of %d slots",
                  table_cols, page_size);
   if (groups == 0) return TLLM_OK;
-  TLLM_CHECK_ARG(parents && lens && copy_src && copy_dst && copy_fill &&
-                     (table_cols == 0 || (table_in && table_out)),
+  TLLM_CHECK_ARG(t->parents && t->lens && t->copy_src && t->copy_dst && t->copy_fill &&
+                     (table_cols == 0 || (t->table_in && t->table_out)),
                  "NULL pointer");
   ReorderParams p;
-  p.parents = parents;
-  p.lens = lens;
-  p.table_in = table_in;
-  p.table_out = table_out;
+  p.parents = t->parents;
+  p.lens = t->lens;
+  p.table_in = t->table_in;
+  p.table_out = t->table_out;
   p.beams = beams;
   p.cols = table_cols;
   p.page_size = page_size;
-  p.copy_src = copy_src;
-  p.copy_dst = copy_dst;
-  p.copy_fill = copy_fill;
+  p.copy_src = t->copy_src;
+  p.copy_dst = t->copy_dst;
+  p.copy_fill = t->copy_fill;
   p.err = device_error_ptr();
   TLLM_CHECK_ARG(p.err, "device error word unavailable");
   const int threads = table_cols >= 256 ? 256 : (table_cols + 31) / 32 * 32 > 32

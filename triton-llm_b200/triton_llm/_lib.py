@@ -103,9 +103,8 @@ SIGNATURES: dict[str, list] = {
     "tllm_page_copy": [_vp, _l, _i, _l, _i, _i, _l, _i, _i, _vp, _vp, _vp, _i, _vp],
     # beam search
     "tllm_beam_workspace": [_i, _i, _i, _i, _psz],
-    "tllm_beam_select": [_vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp,
-                         _vp, _sz, _vp],
-    "tllm_beam_reorder": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp],
+    "tllm_beam_select": [_vp, _vp],
+    "tllm_beam_reorder": [_vp, _vp],
     # projections
     "tllm_linear_workspace": [_i, _i, _i, _psz, _psz],
     "tllm_linear_plan": [_i, _i, _i, _i, _pi],
@@ -184,6 +183,8 @@ class PagedRowsStruct(ctypes.Structure):
 # of the time that filling a ctypes structure, or passing its fields, does
 PAGED_ATTN = struct.Struct("@6P2N6l6ifi")   # tllm_paged_attn
 PAGED_ROWS = struct.Struct("@10P8l8i")      # tllm_paged_rows
+BEAM_STEP = struct.Struct("@8PNl6i")        # tllm_beam_step
+BEAM_TABLES = struct.Struct("@7P4i")        # tllm_beam_tables
 
 EL_SWIGLU, EL_ADD, EL_GELU = 0, 1, 2
 

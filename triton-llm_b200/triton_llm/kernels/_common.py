@@ -57,21 +57,22 @@ def require_gpu(t, name):
 
 def on_device(t, name, code=None, shape=None):
     """Address of a contiguous device tensor, its type and shape checked."""
-    if code is not None and _CODES.get(t.dtype) != code and dtype_code(t, name) != code:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected {_WORDS[code]}")
-    if shape is not None and t.shape != shape and tuple(t.shape) != shape:
+    if type(t) is not _Device:
+        try:
+            if ((code is None or _CODES[t.dtype] == code)
+                    and (shape is None or t.shape == shape) and t.is_cuda
+                    and t.is_contiguous()):
+                return t.data_ptr()
+        except (AttributeError, KeyError):
+            pass
+    if code is not None and dtype_code(t, name) != code:
+        raise ValueError(f"{name} has dtype {'bfloat16' if getattr(t, 'is_bf16', 0) else t.dtype}"
+                         f", expected {_WORDS[code]}")
+    if shape is not None and tuple(t.shape) != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if type(t) is _Device:
-        if t.is_bf16 and code is not None and code != _lib.BF16:
-            raise ValueError(f"{name} has dtype bfloat16, expected {_WORDS[code]}")
-        return t.ptr.value
-    try:
-        if t.is_cuda and t.is_contiguous():
-            return t.data_ptr()
-    except AttributeError:
-        pass
     require_gpu(t, name)
-    contiguous = getattr(t, "is_contiguous", None)
-    if contiguous is not None and not contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    if type(t) is not _Device:
+        contiguous = getattr(t, "is_contiguous", None)
+        if contiguous is not None and not contiguous():
+            raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()

@@ -8,6 +8,7 @@ Tensors and streams as in ``triton_llm.kernels.paged``.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 
@@ -44,46 +45,41 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     out_done (groups, k) int32 or None: whether the candidate's beam is done or
              its token is ``eos_token``
     """
-    if len(scores.shape) != 2 or len(logits.shape) != 2:
-        raise ValueError(f"scores and logits must be 2D, got {tuple(scores.shape)}, "
-                         f"{tuple(logits.shape)}")
-    groups, beams = int(scores.shape[0]), int(scores.shape[1])
-    if logits.shape[0] != groups * beams:
-        raise ValueError(f"logits have {logits.shape[0]} rows, {groups} groups of {beams} "
-                         "beams")
+    shape, rows = tuple(scores.shape), tuple(logits.shape)
+    if len(shape) != 2 or len(rows) != 2:
+        raise ValueError(f"scores and logits must be 2D, got {shape}, {rows}")
+    groups, beams = shape
+    n, vocab = rows
+    if n != groups * beams:
+        raise ValueError(f"logits have {n} rows, {groups} groups of {beams} beams")
     if dtype_code(logits, "logits") != _lib.F32:
         raise ValueError(f"logits must be float32, got {logits.dtype}")
-    sl = strides(logits)
-    vocab = int(logits.shape[1])
-    if sl[1] != 1 and vocab > 1:
+    ld, one = strides(logits)
+    if one != 1 and vocab > 1:
         raise ValueError("rows of logits must be contiguous")
     require_gpu(logits, "logits")
-    if len(out_scores.shape) != 2 or out_scores.shape[0] != groups:
-        raise ValueError(f"out_scores must be ({groups}, k), got {tuple(out_scores.shape)}")
-    shape = tuple(out_scores.shape)
-    k = int(shape[1])
-    flags = None
+    out = tuple(out_scores.shape)
+    if len(out) != 2 or out[0] != groups:
+        raise ValueError(f"out_scores must be ({groups}, k), got {out}")
+    k = out[1]
+    flags = 0
     if done is not None:
         flags = on_device(done, "done", _lib.I32)
-        n = 1
-        for s in done.shape:
-            n *= int(s)
-        if n != groups * beams:
-            raise ValueError(f"done has {n} values for {groups * beams} beams")
-    args = (on_device(scores, "scores", _lib.F32),
-            on_device(out_scores, "out_scores", _lib.F32),
-            on_device(out_parents, "out_parents", _lib.I32, shape),
-            on_device(out_tokens, "out_tokens", _lib.I32, shape))
+        if math.prod(done.shape) != n:
+            raise ValueError(f"done has {math.prod(done.shape)} values for {n} beams")
     if workspace is None:
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
         workspace = _workspace(lambda: BeamWorkspace(groups, beams, vocab, k), "beam",
                                gpu.current_device(), groups, beams, vocab, k)
-    _lib.call("tllm_beam_select", logits.data_ptr(), sl[0] if groups * beams > 1 else 0,
-              args[0], flags, int(pad_token), groups, beams, vocab, k, args[1], args[2],
-              args[3], int(eos_token),
-              None if out_done is None else on_device(out_done, "out_done", _lib.I32, shape),
-              workspace.ptr, workspace.nbytes, stream)
+    _lib.call("tllm_beam_select", _lib.BEAM_STEP.pack(
+        logits.data_ptr(), on_device(scores, "scores", _lib.F32), flags,
+        on_device(out_scores, "out_scores", _lib.F32),
+        on_device(out_parents, "out_parents", _lib.I32, out),
+        on_device(out_tokens, "out_tokens", _lib.I32, out),
+        0 if out_done is None else on_device(out_done, "out_done", _lib.I32, out),
+        workspace.ptr, workspace.nbytes, ld if n > 1 else 0, groups, beams, vocab, k,
+        int(pad_token), int(eos_token)), stream)
 
 
 def beam_reorder(parents, lens, table, table_out, copy_src, copy_dst, copy_fill, *,
@@ -100,18 +96,17 @@ def beam_reorder(parents, lens, table, table_out, copy_src, copy_dst, copy_fill,
              step needs; none where src == dst or src < 0
     Every beam has to own the page that it is filling and those after it.
     """
-    if len(parents.shape) != 2 or len(table.shape) != 2:
-        raise ValueError(f"parents and table must be 2D, got {tuple(parents.shape)}, "
-                         f"{tuple(table.shape)}")
-    groups, beams = int(parents.shape[0]), int(parents.shape[1])
-    n = groups * beams
-    if table.shape[0] != n:
-        raise ValueError(f"table has {table.shape[0]} rows for {n} beams")
-    shape = tuple(table.shape)
-    _lib.call("tllm_beam_reorder", on_device(parents, "parents", _lib.I32),
-              on_device(lens, "lens", _lib.I32, (n,)), on_device(table, "table", _lib.I32),
-              on_device(table_out, "table_out", _lib.I32, shape), groups, beams,
-              int(shape[1]), int(page_size),
-              on_device(copy_src, "copy_src", _lib.I32, (n,)),
-              on_device(copy_dst, "copy_dst", _lib.I32, (n,)),
-              on_device(copy_fill, "copy_fill", _lib.I32, (n,)), stream)
+    shape, rows = tuple(parents.shape), tuple(table.shape)
+    if len(shape) != 2 or len(rows) != 2:
+        raise ValueError(f"parents and table must be 2D, got {shape}, {rows}")
+    n = shape[0] * shape[1]
+    if rows[0] != n:
+        raise ValueError(f"table has {rows[0]} rows for {n} beams")
+    _lib.call("tllm_beam_reorder", _lib.BEAM_TABLES.pack(
+        on_device(parents, "parents", _lib.I32), on_device(lens, "lens", _lib.I32, (n,)),
+        on_device(table, "table", _lib.I32),
+        on_device(table_out, "table_out", _lib.I32, rows),
+        on_device(copy_src, "copy_src", _lib.I32, (n,)),
+        on_device(copy_dst, "copy_dst", _lib.I32, (n,)),
+        on_device(copy_fill, "copy_fill", _lib.I32, (n,)), shape[0], shape[1], rows[1],
+        int(page_size)), stream)
