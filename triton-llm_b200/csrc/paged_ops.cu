@@ -1,6 +1,7 @@
 // Writing and moving the pages of a paged KV cache, for sm_100a: new tokens
 // with rotary positions (tllm_paged_append) and page copies over the planes of
 // an arena (tllm_page_copy).
+#include "mma_sync.cuh"
 #include "paged.cuh"
 
 namespace tllm {
@@ -135,9 +136,7 @@ __device__ __forceinline__ void store4(float *p, float4 v, bool stream) {
     *reinterpret_cast<float4 *>(p) = v;
 }
 __device__ __forceinline__ void store4(uint16_t *p, float4 v, bool stream) {
-  uint2 r;
-  r.x = (uint32_t)f32_to_bf16_bits(v.x) | (uint32_t)f32_to_bf16_bits(v.y) << 16;
-  r.y = (uint32_t)f32_to_bf16_bits(v.z) | (uint32_t)f32_to_bf16_bits(v.w) << 16;
+  const uint2 r = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   if (stream)
     __stcs(reinterpret_cast<uint2 *>(p), r);
   else
@@ -163,6 +162,7 @@ __global__ void __launch_bounds__(512)
   const int src_row = p.in.row_src ? p.in.row_src[row] : row;
   const size_t from = source_ok(p, src_row) ? src_row : 0;   // (else skipped below)
   float4 x[kUnits], y[kUnits];
+  int heads[kUnits], at_a[kUnits], at_b[kUnits];   // (head * 2 + whether it turns)
   // runs a and b of unit u of a head
   auto runs = [&](int head, int u, int *a, int *b) {
     const bool turned = head < H + K && u < rot >> 3;
@@ -176,7 +176,9 @@ __global__ void __launch_bounds__(512)
     if (at >= n) continue;
     const int head = at / per, u = at - head * per;
     int a, b;
-    runs(head, u, &a, &b);
+    heads[i] = head * 2 + runs(head, u, &a, &b);
+    at_a[i] = a;
+    at_b[i] = b;
     const S *src;
     if (head < H)
       src = static_cast<const S *>(p.in.q) + from * p.in.q_row_stride +
@@ -197,10 +199,9 @@ __global__ void __launch_bounds__(512)
   for (int i = 0; i < kUnits; ++i) {
     const unsigned at = threadIdx.x + i * blockDim.x;
     if (at >= n) continue;
-    const int head = at / per, u = at - head * per;
-    int a, b;
-    if (runs(head, u, &a, &b)) {
-      const size_t t = (size_t)r.pos * half + 4 * u;
+    const int head = heads[i] >> 1, a = at_a[i], b = at_b[i];
+    if (heads[i] & 1) {
+      const size_t t = (size_t)r.pos * half + (p.in.interleaved ? a >> 1 : a);
       const float4 c = __ldg(reinterpret_cast<const float4 *>(p.in.cos_t + t));
       const float4 s = __ldg(reinterpret_cast<const float4 *>(p.in.sin_t + t));
       const float4 v = x[i], w = y[i];
