@@ -284,6 +284,31 @@ def test_attention_offsets_past_32_bits():
     assert head_error(o.to_numpy().astype(np.float64), want) < F32_TOL
 
 
+def test_attention_of_a_table_near_its_largest():
+    """Two sequences that may have 2^30 - 2^20 tokens; rows in more than one
+    block of the kernel."""
+    K, P, D, cols, R = 1, 1 << 20, 64, 1023, 600
+    rng = np.random.default_rng(41)
+    kv = [gpu.allocate((2, K, P, D), "bfloat16") for _ in range(2)]
+    host = bf16(rng.standard_normal((2, 300, D)).astype(np.float32))   # page 1's first tokens
+    for t, h in zip(kv, host):
+        gpu.copy_d2d(gpu.sub_view(t, P * D * 2, (300, D)), gpu.to_device_bf16(h))
+    table = np.full((2, cols), -1, np.int32)
+    table[1, 0] = 1
+    lens = rng.integers(0, 301, R)
+    q = rng.standard_normal((R, 5, D)).astype(np.float32)
+    o = gpu.allocate(q.shape, np.float32)
+    paged_attention(PagedKV(*kv, i32(table)), gpu.to_device(q), i32(lens), o,
+                    row_seq=i32(np.ones(R)))
+    k, v = host.astype(np.float64)
+    s = q.astype(np.float64) @ k.T / 8.0
+    s[np.broadcast_to(np.arange(300) >= lens[:, None, None], s.shape)] = -np.inf
+    w = np.exp(s - np.maximum(s.max(-1, keepdims=True), -1e30))
+    want = w @ v / np.maximum(w.sum(-1, keepdims=True), 1e-30)
+    assert head_error(o.to_numpy().astype(np.float64), want) < F32_TOL
+    assert gpu.device_error() == 0
+
+
 def test_attention_repeats_and_other_streams():
     """The same bits on every call, in a graph and on another stream."""
     from triton_llm import _lib

@@ -483,8 +483,11 @@ __global__ void __launch_bounds__(kGenWarps * 32)
 // terms leave 2.5e-6 of each value, which the result then shows. A tile's
 // O^T is added to the running one by ordinary fp32 additions: the tensor
 // core's own additions round towards zero, and a chain of them over a long
-// row loses 1e-5 (measured over 20011 keys). The work is bound by HBM: at head_dim 128 a tile is 32 KB, 1400 cycles of an SM's share
-// of 6.4 TB/s.
+// row loses 1e-5 (measured over 20011 keys). The work is bound by HBM: a tile is
+// 32 KB, 1400 cycles of an SM's share of 6.4 TB/s. Measured in a graph: 64 rows of
+// 24/8/128 with 1024 to 8192 keys 191 us (6.35 TB/s), one of 131071 keys 90 (5.95),
+// 8 of 1024 to 8192 keys 33 (4.55), 48 of 15/5/64 over 1028 keys of a window 17.5
+// (3.4: the first tile and the last write take as long as the stream).
 //
 // The tiles run over the row's pages: with a window, the pages of the first
 // tokens and then those from the window's first page on (all pages where the
@@ -496,6 +499,7 @@ constexpr int kMaxPerSm = 2;     // CTAs that the shared memory lets an SM hold
 constexpr int kSegs = 2;         // segments announced to the consumers
 constexpr int kSegTiles = 2;     // tiles that a CTA reads in the time of a segment's end
 constexpr int kMinTiles = 2;     // least tiles of a share
+constexpr int kJobWaits = 1024;  // waits of the joining warp
 constexpr int kJoinTiles = 4;    // tiles that a CTA reads in the time of a join
 
 template <int D>
@@ -780,8 +784,8 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   __shared__ uint32_t s_bad[kStages];                 // bad pages of a stage's tile
   __shared__ Segment s_seg[kSegs];
   __shared__ Job s_job;
-  __shared__ int s_cum[kRowBlock + 1], s_len[kRowBlock];
-  __shared__ int s_warp[2][NCW + 2], s_last;
+  __shared__ long s_cum[kRowBlock + 1], s_warp[NCW + 2];   // (512 x 2^24 places)
+  __shared__ int s_len[kRowBlock], s_most[NCW + 2], s_last;
   __shared__ volatile int s_fail;
   __shared__ float s_m[NCW][16], s_l[NCW][16];
   const int row0 = blockIdx.y * kRowBlock, nrows = min(kRowBlock, p.rows - row0);
@@ -812,7 +816,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   // ---- places of every row's pairs, summed up (a row without keys has a tile,
   // empty)
   const int per = (nrows + T::THREADS - 1) / T::THREADS;
-  int sum = 0, most = 0;
+  int sum = 0, most = 0;   // (a warp's 96 rows: below 2^31)
   for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
     int len = p.row_len[row0 + i];
     const int cap = p.kv.table_cols * p.kv.page_size;
@@ -841,19 +845,19 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     most = max(most, __shfl_xor_sync(~0u, most, o));
   }
   if (lane == 31) {
-    s_warp[0][warp] = scan;
-    s_warp[1][warp] = most;
+    s_warp[warp] = scan;
+    s_most[warp] = most;
   }
   __syncthreads();
-  int before = scan - sum, total = 0;
+  long before = scan - sum, total = 0;
 #pragma unroll
   for (int w = 0; w < NCW + 2; ++w) {
-    if (w < warp) before += s_warp[0][w];
-    total += s_warp[0][w];
-    most = max(most, s_warp[1][w]);
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
+    most = max(most, s_most[w]);
   }
   for (int i = tid * per; i < min(nrows, (tid + 1) * per); ++i) {
-    const int places = s_cum[i];
+    const long places = s_cum[i];
     s_cum[i] = before;
     before += places;
   }
@@ -863,8 +867,8 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
   // ---- shares. Where every pair can have a CTA of its own and sharing would
   // save less than kJoinTiles, pairs stay whole: joining costs about as much.
   const int ncta = gridDim.x;
-  const long work = (long)total * p.n_y;
-  int share = (int)((work + ncta - 1) / ncta);
+  const long work = total * p.n_y;
+  long share = (work + ncta - 1) / ncta;
   if (share < kMinTiles + kSegTiles) share = kMinTiles + kSegTiles;
   const bool whole_pairs = (long)nrows * p.n_y <= ncta && most <= share + kJoinTiles;
   const size_t base = (size_t)blockIdx.y * ncta;   // of the shares
@@ -932,7 +936,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         }
       }
     };
-    auto tiles_of = [&](int row) { return s_cum[row + 1] - s_cum[row] - kSegTiles; };
+    auto tiles_of = [&](int row) { return (int)(s_cum[row + 1] - s_cum[row]) - kSegTiles; };
     Segment g;
     if (whole_pairs) {
       if (blockIdx.x < nrows * p.n_y) {
@@ -944,18 +948,18 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
         stream(g);
       }
     } else {
-      long w = (long)blockIdx.x * share;
+      long w = blockIdx.x * share;
       const long w1 = min(w + share, work);
       int lo = 0, hi = nrows;   // s_cum[lo] * n_y <= w < s_cum[hi] * n_y
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if ((long)s_cum[mid] * p.n_y <= w) lo = mid; else hi = mid;
+        if (s_cum[mid] * p.n_y <= w) lo = mid; else hi = mid;
       }
       g.row = lo;
       int nt = tiles_of(lo);
-      const int rem = (int)(w - (long)s_cum[lo] * p.n_y);
-      g.y = rem / (nt + kSegTiles);
-      g.t0 = rem - g.y * (nt + kSegTiles);
+      const long rem = w - s_cum[lo] * p.n_y;
+      g.y = (int)(rem / (nt + kSegTiles));
+      g.t0 = (int)(rem - (long)g.y * (nt + kSegTiles));
       while (w < w1 && !failed) {
         const long begin = w - g.t0;   // of the pair
         if (g.t0 < nt) {
@@ -998,9 +1002,17 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     return last;
   };
   if (warp == NCW + 1) {
-    // ---- joining warp
+    // ---- joining warp (its wait lasts as long as the CTA's first segment, whose
+    // own waits are bounded)
     for (int jobs = 0;; ++jobs) {
-      if (!__all_sync(~0u, wait_phase(job_full, jobs & 1, &s_fail))) return;
+      bool told = false;
+      for (int n = 0; n < kJobWaits && !told && !s_fail; ++n)
+        told = __all_sync(~0u, wait_phase(job_full, jobs & 1, &s_fail));
+      if (!told) {
+        if (lane == 0 && !s_fail) atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+        s_fail = 1;
+        return;
+      }
       const Job job = s_job;
       __syncwarp();
       if (lane == 0) arrive(job_empty);

@@ -382,7 +382,7 @@ extern "C" int tllm_page_copy(void *arena, long plane_stride, int planes, long p
                      page_size >= 1 && row_bytes >= 1 && n_copies >= 0,
                  "invalid arena: %d planes, %d pages of %d runs of %d slots of %d bytes, %d copies",
                  planes, n_pages, heads, page_size, row_bytes, n_copies);
-  TLLM_CHECK_ARG((long)page_size * row_bytes < (1L << 31), "a run of a page must be below 2 GiB");
+  TLLM_CHECK_ARG((long)page_size * row_bytes <= (1L << 30), "a run of a page must be at most 1 GiB");
   TLLM_CHECK_ARG(plane_stride >= 0 && page_stride >= 0 && run_stride >= 0, "negative stride");
   if (planes == 0 || heads == 0 || n_copies == 0) return TLLM_OK;
   TLLM_CHECK_ARG(arena && src && dst, "NULL pointer");
