@@ -143,6 +143,7 @@ def append(qkv=(3, 8 * 64), pos=(3,), q_out=(3, 4, 64), cos=(10, 32), sin=(10, 3
     (dict(cos=(10, 33), sin=(10, 33)), "rotary_dim"),
     (dict(cos=(0, 32), sin=(0, 32)), "n_pos"),
     (dict(rows=4), "4 rows of a qkv of 3"),
+    (dict(lens_out=Fake((2,), "int32")), "lens_out has shape"),
     (dict(qkv=(4, 8 * 64), pos=(4,), q_out=(4, 4, 64)), "4 rows for a table of 3"),
     (dict(cache=kv(D=72), qkv=(3, 8 * 72), q_out=(3, 4, 72), cos=None, sin=None,
           blocked=True), "blocked"),

@@ -145,10 +145,10 @@ def test_fork_compact_release():
             s.compact()
     s.release([2, 3])
     s.release([1])
-    assert s.pool.used == 4                 # one page for every idle slot
-    for _ in range(20):                     # idle slots stay within theirs
+    assert s.pool.used == 0
+    for _ in range(20):                     # idle slots take none
         s.step()
-    assert s.pool.used == 4
+    assert s.pool.used == 0
 
 
 def test_slots_and_page_limits():
@@ -160,8 +160,8 @@ def test_slots_and_page_limits():
     s.prefill([p], slots=[0])
     with pytest.raises(RuntimeError, match="out of pages"):
         s.prefill([p], slots=[1])
-    s.step()
-    s.step()
+    for _ in range(18):                     # up to position 48 = 3 pages of 16
+        s.step()
     with pytest.raises(RuntimeError, match="out of pages"):
         s.step()
     for kw in (dict(page_size=0), dict(sinks=2), dict(window=-1)):
@@ -169,6 +169,48 @@ def test_slots_and_page_limits():
             PagedSession(m.dev, 2, 64, **kw)
     with pytest.raises(ValueError, match="fork"):
         s.fork(1, [0])
+    with pytest.raises(ValueError, match="fork"):
+        s.fork(0, [2])
+    with pytest.raises(ValueError, match="slots"):
+        s.release([-1])
+
+
+def test_sequences_survive_when_pages_run_out():
+    """A prompt, a fork or a step that finds too few pages leaves the other
+    sequences as they were: they go on as if it had not been tried."""
+    from smollm2_triton.paged import PagedSession
+    m, _ = model(dtype="bfloat16")
+    m._init_gpu_weights()
+    a, b = prompts_of(inputs.SMOL_TINY, [21, 30])
+    want = run(PagedSession(m.dev, 1, 96, page_size=8), [a], 30)[:, 0]
+    s = PagedSession(m.dev, 4, 96, page_size=8, n_pages=8)
+    got = [s.prefill([a], slots=[1])[0]]    # 3 pages
+
+    def step(n):
+        for _ in range(n):
+            s.step()
+            got.append(s.logits.to_numpy()[1])
+    s.prefill([b], slots=[2])               # 4 pages, 1 is left
+    step(1)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        s.fork(1, [0, 3])                   # needs two
+    with pytest.raises(RuntimeError, match="out of pages"):
+        s.prefill([b], slots=[0])
+    step(1)                                 # (slot 2 is at 32 = 4 pages, slot 1 at 23)
+    s.fork(1, [3])                          # shares 2 pages, the last free one is its own
+    assert s.pool.free == 0
+    with pytest.raises(RuntimeError, match="out of pages"):
+        s.step()                            # slot 2 needs a fifth page
+    with pytest.raises(RuntimeError, match="out of pages"):
+        s.prefill([b], slots=[0])           # (nothing to give back)
+    s.release([3])                          # of its pages one comes free
+    assert s.pool.free == 1
+    s.release([2])
+    step(28)
+    assert s.pool.used == 7                 # 51 tokens
+    got = np.stack(got)
+    assert np.abs(got - want).max() < 1e-4 * np.abs(want).max()
+    assert (got.argmax(-1) == want.argmax(-1)).all()
 
 
 def test_rope_scaling_reaches_past_the_models_window():

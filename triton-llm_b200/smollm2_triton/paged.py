@@ -45,7 +45,9 @@ class PagedSession(LlamaSession):
     rope_scaling  see ``scaled_cos_sin``: positions past the model's window
 
     The other arguments are LlamaSession's. ``step`` (or ``decode_step``)
-    advances every slot that holds a sequence; the others run idle.
+    advances every slot that holds a sequence; the others run idle, on one page
+    past the pool's that they share. Where pages run out, the slots that were to
+    get some hold no sequence afterwards; the others are as they were.
     """
 
     def __init__(self, wts: LlamaWeights, batch: int, max_seq: int, page_size: int = 64,
@@ -73,10 +75,11 @@ class PagedSession(LlamaSession):
 
     def _cache_buffers(self):
         w = self.w
-        shape = (2 * w.L, self.n_pages, w.Hkv, self.P, w.D)
+        shape = (2 * w.L, self.n_pages + 1, w.Hkv, self.P, w.D)   # (the last: idle slots)
         self.arena = gpu.allocate(shape, "bfloat16" if self.kv_bf16 else np.float32)
         self.pool = PagePool(self.n_pages)
         self._table = np.full((self.B, self.cols), -1, np.int32)
+        self._table[:, 0] = self.n_pages
         self.table = gpu.to_device(self._table)
         plane = self.arena.nbytes // (2 * w.L)
         self.pages = [PagedKV(gpu.sub_view(self.arena, 2 * i * plane, shape[1:]),
@@ -89,26 +92,41 @@ class PagedSession(LlamaSession):
         self._capturing = False
         self.qkv = gpu.allocate((self.B, (w.H + 2 * w.Hkv) * w.D), np.float32)
         self.attn_ws = PagedWorkspace(self.B, w.H, w.Hkv, w.D)
-        for b in range(self.B):                   # an idle slot writes somewhere
-            self._table[b, 0] = self.pool.take(1)[0]
-        self._upload()
 
     def _upload(self):
         self.table.from_numpy(self._table)
 
     # -- pages ------------------------------------------------------------
-    def _set_pages(self, slot: int, tokens: int):
-        """Gives the slot fresh pages for ``tokens`` positions."""
-        row = self._table[slot]
-        self.pool.release(row[row >= 0])
-        row[:] = -1
-        n = max(1, -(-tokens // self.P))
-        try:
-            row[:n] = self.pool.take(n)
-        except RuntimeError:
-            row[0] = self.pool.take(1)[0]
-            self._live[slot] = False
-            raise
+    def _drop(self, row, which) -> None:
+        """Gives back the pages of these columns of a table row."""
+        pages = row[which & (row >= 0)]
+        self.pool.release(pages[pages < self.n_pages])
+        row[which] = -1
+
+    def _idle(self, slots) -> None:
+        """Slots without a sequence: no pages of the pool, position 0."""
+        for b in slots:
+            self._drop(self._table[b], np.ones(self.cols, bool))
+            self._table[b, 0] = self.n_pages
+            self._live[b], self._pos[b] = False, 0
+
+    def _set_pages(self, slots, tokens):
+        """Fresh pages for new sequences of these lengths."""
+        self._idle(slots)
+        need = [max(1, -(-int(n) // self.P)) for n in tokens]
+        if sum(need) > self.pool.free:
+            self._upload_all()
+            self.pool.take(sum(need))   # (raises)
+        for b, n in zip(slots, need):
+            self._table[b, :n] = self.pool.take(n)
+            self._live[b] = True
+        self._upload()
+
+    def _upload_all(self):
+        self._upload()
+        # (idle slots' positions are theirs, not the last prefill's)
+        for t in (self.pos, self.lens):
+            t.from_numpy(self._pos.astype(np.int32))
 
     def _outside(self, length: int) -> np.ndarray:
         """Columns whose tokens a row of this length does not see."""
@@ -120,8 +138,7 @@ class PagedSession(LlamaSession):
             return False
         row = self._table[slot]
         old = self._outside(length) & (row >= 0)
-        self.pool.release(row[old])
-        row[old] = -1
+        self._drop(row, old)
         return bool(old.any())
 
     def _advance(self):
@@ -134,27 +151,27 @@ class PagedSession(LlamaSession):
             raise ValueError(f"a sequence has reached max_seq ({self.S})")
         if idle.any():
             self._pos[idle] = 0
-            self.pos.from_numpy(self._pos.astype(np.int32))
-            self.lens.from_numpy(self._pos.astype(np.int32))
+            self._upload_all()
         changed = False
-        for b in np.flatnonzero(self._live & (self._pos % self.P == 0)):
-            changed |= self._drop_outside(b, int(self._pos[b]) + 1)
-            if self._table[b, self._pos[b] // self.P] < 0:
-                self._table[b, self._pos[b] // self.P] = self.pool.take(1)[0]
-                changed = True
-        if changed:
-            self._upload()
+        try:
+            for b in np.flatnonzero(self._live & (self._pos % self.P == 0)):
+                changed |= self._drop_outside(b, int(self._pos[b]) + 1)
+                if self._table[b, self._pos[b] // self.P] < 0:
+                    self._table[b, self._pos[b] // self.P] = self.pool.take(1)[0]
+                    changed = True
+        finally:   # (a caller may release a slot and go on where pages ran out)
+            if changed:
+                self._upload()
         self._keys_hint = int(self._pos[self._live].sum()) + self.B
         self._pos += 1
 
     def release(self, slots) -> None:
         """Ends the sequences in ``slots`` and frees their pages."""
-        for b in np.asarray(slots, np.int64).reshape(-1):
-            self._set_pages(int(b), 0)
-            self._live[b], self._pos[b] = False, 0
-        self._upload()
-        self.pos.from_numpy(self._pos.astype(np.int32))
-        self.lens.from_numpy(self._pos.astype(np.int32))
+        slots = [int(b) for b in np.asarray(slots, np.int64).reshape(-1)]
+        if not all(0 <= b < self.B for b in slots):
+            raise ValueError(f"slots {slots} are not all in the batch of {self.B}")
+        self._idle(slots)
+        self._upload_all()
 
     def fork(self, src: int, dst, reserve: int = 0) -> None:
         """Continues the sequence of slot ``src`` in the slots ``dst`` as well:
@@ -162,31 +179,33 @@ class PagedSession(LlamaSession):
         ``reserve``: tokens that every one of them, ``src`` too, gets its own
         pages for ahead of time."""
         dst = [int(d) for d in np.asarray(dst, np.int64).reshape(-1)]
-        if not self._live[src] or src in dst or len(set(dst)) != len(dst):
+        if not all(0 <= b < self.B for b in [src, *dst]) or not self._live[src] or \
+                src in dst or len(set(dst)) != len(dst):
             raise ValueError(f"cannot fork slot {src} into {dst}")
         pos = int(self._pos[src])
         full, part = divmod(pos, self.P)
         last = min(self.cols, max(full + (part > 0), -(-(pos + reserve) // self.P)))
+        self._idle(dst)
+        more = np.flatnonzero(self._table[src, full:last] < 0) + full
+        need = len(dst) * (last - full) + len(more)
+        if need > self.pool.free:
+            self._upload_all()
+            self.pool.take(need)   # (raises)
         copies = []
+        shared = self._table[src, :full]
         for d in dst:
-            old = self._table[d][self._table[d] >= 0]
-            self.pool.release(old)
-            self._table[d] = -1
-            shared = self._table[src, :full]
             self.pool.share(shared[shared >= 0])
+            self._table[d, 0] = -1
             self._table[d, :full] = shared
             self._table[d, full:last] = self.pool.take(last - full)
             if part:
                 copies.append((self._table[src, full], self._table[d, full], part))
             self._live[d], self._pos[d] = True, pos
-        more = self._table[src, full:last] < 0
-        self._table[src, full:last][more] = self.pool.take(int(more.sum()))
-        self._upload()
+        self._table[src, more] = self.pool.take(len(more))
+        self._upload_all()
         if copies:
             c = np.array(copies, np.int32).T.copy()
             page_copy(self.arena, *[gpu.to_device(x) for x in c])
-        for t in (self.pos, self.lens):
-            t.from_numpy(self._pos.astype(np.int32))
         ids = self.ids.to_numpy()
         ids[dst] = ids[src]
         self.ids.from_numpy(ids)
@@ -197,7 +216,8 @@ class PagedSession(LlamaSession):
         src, dst, where = self.pool.compact()
         if len(src):
             page_copy(self.arena, gpu.to_device(src), gpu.to_device(dst))
-            self._table = np.where(self._table >= 0, where[self._table], -1).astype(np.int32)
+            where = np.append(where, [self.n_pages, -1])   # the idle slots' page, none
+            self._table = where[self._table].astype(np.int32)
             self._upload()
         return len(src)
 
@@ -242,34 +262,30 @@ class PagedSession(LlamaSession):
         if self._fixed:
             raise RuntimeError("the session's pages are reserved by a beam search")
         if not keep:
-            self.release(np.setdiff1d(np.arange(self.B), at))
-        for b, n in zip(at, lens):
-            self._live[b] = True
-            self._set_pages(int(b), int(n))
-        self._upload()
+            self._idle(np.setdiff1d(np.arange(self.B), at))
+        self._set_pages(at, lens)
         w = self.w
         shape = (self.B, w.Hkv, int(lens.max()), w.D)
         dt = "bfloat16" if self.kv_bf16 else np.float32
-        self.kv = [(gpu.allocate(shape, dt), gpu.allocate(shape, dt))] * w.L
         try:
+            self.kv = [(gpu.allocate(shape, dt), gpu.allocate(shape, dt))] * w.L
             out = super().prefill(prompts, all_logits, slots)
+        except BaseException:
+            self.release(at)
+            raise
         finally:
             self.kv, self._p_src = None, None
         self._pos[at] = lens
         for b, n in zip(at, lens):
             self._drop_outside(int(b), int(n) + 1)
-        self._upload()
-        # (idle slots' positions are theirs, not the last prefill's)
-        self.pos.from_numpy(self._pos.astype(np.int32))
-        self.lens.from_numpy(self._pos.astype(np.int32))
+        self._upload_all()
         return out
 
     def set_state(self, pos, ids):
         """Sequences of these lengths with whatever their pages hold."""
         pos = np.asarray(pos, np.int64)
+        self._set_pages(range(len(pos)), pos)
         for b, n in enumerate(pos):
-            self._live[b] = True
-            self._set_pages(b, int(n))
             self._drop_outside(b, int(n) + 1)
         self._pos[:] = pos
         self._upload()
@@ -320,7 +336,7 @@ def beam_search(wts: LlamaWeights, prompts, beams: int, max_new_tokens: int,
     # a prompt's full pages once, and every beam's own from there on
     own = sum(len(p) // P + W * (-(-(len(p) + max_new_tokens) // P) - len(p) // P)
               for p in prompts)
-    session.setdefault("n_pages", own + 2 * G * W)
+    session.setdefault("n_pages", own)
     s = PagedSession(wts, G * W, longest, **session)
     first = np.arange(G) * W
     s.prefill(prompts, slots=first)

@@ -238,7 +238,7 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
         at, at + n_head * D * 4, at + (n_head + K) * D * 4,
         on_device(q_out, "q_out", _lib.F32), 0, _index(row_seq, "row_seq", n),
         _index(row_pos, "row_pos", n),
-        0 if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        _index(lens_out, "lens_out", kv.n_seq),
         cos_t, sin_t, ld, D, ld, D, ld, D, n_head * D, D, _lib.F32, n, n_head, rotary,
         n_pos, bool(interleaved), bool(blocked), int(qkv.shape[0]))
     _lib.call("tllm_paged_append", kv._ref, r, stream)
@@ -292,7 +292,7 @@ def paged_write(kv, k, v, row_pos, row_seq=None, row_src=None, cos=None, sin=Non
     r = _lib.PAGED_ROWS.pack(
         0, k.data_ptr(), v.data_ptr(), 0, _index(row_src, "row_src", n),
         _index(row_seq, "row_seq", n), _index(row_pos, "row_pos", n),
-        0 if lens_out is None else on_device(lens_out, "lens_out", _lib.I32),
+        _index(lens_out, "lens_out", kv.n_seq),
         cos_t, sin_t, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0, code, n, 0, rotary, n_pos,
         bool(interleaved), 0, src_rows)
     _lib.call("tllm_paged_append", kv._ref, r, stream)
