@@ -41,8 +41,11 @@ def dtype_code(t, name="tensor"):
 
 def strides(t):
     """Element strides of a device tensor (a DeviceTensor is contiguous)."""
-    if type(t) is not _Device and hasattr(t, "stride"):
-        return tuple(t.stride())
+    if type(t) is not _Device:
+        try:
+            return t.stride()
+        except AttributeError:
+            pass
     out, n = [], 1
     for s in reversed(t.shape):
         out.append(n)
@@ -76,3 +79,9 @@ def on_device(t, name, code=None, shape=None):
         if contiguous is not None and not contiguous():
             raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
+
+
+def device_of(t):
+    """GPU index of a device tensor (a DeviceTensor is on the current one)."""
+    index = None if type(t) is _Device else getattr(t, "get_device", None)
+    return gpu.current_device() if index is None else index()

@@ -13,7 +13,7 @@ import math
 import numpy as np
 
 from triton_llm import gpu, _lib
-from ._common import dtype_code, on_device, require_gpu, strides
+from ._common import device_of, dtype_code, on_device, require_gpu, strides
 from .paged import _workspace
 
 
@@ -45,9 +45,9 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     out_done (groups, k) int32 or None: whether the candidate's beam is done or
              its token is ``eos_token``
     """
-    shape, rows = tuple(scores.shape), tuple(logits.shape)
+    shape, rows = scores.shape, logits.shape
     if len(shape) != 2 or len(rows) != 2:
-        raise ValueError(f"scores and logits must be 2D, got {shape}, {rows}")
+        raise ValueError(f"scores and logits must be 2D, got {tuple(shape)}, {tuple(rows)}")
     groups, beams = shape
     n, vocab = rows
     if n != groups * beams:
@@ -58,20 +58,20 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     if one != 1 and vocab > 1:
         raise ValueError("rows of logits must be contiguous")
     require_gpu(logits, "logits")
-    out = tuple(out_scores.shape)
+    out = out_scores.shape
     if len(out) != 2 or out[0] != groups:
-        raise ValueError(f"out_scores must be ({groups}, k), got {out}")
+        raise ValueError(f"out_scores must be ({groups}, k), got {tuple(out)}")
     k = out[1]
     flags = 0
     if done is not None:
         flags = on_device(done, "done", _lib.I32)
-        if math.prod(done.shape) != n:
+        if done.shape != shape and math.prod(done.shape) != n:
             raise ValueError(f"done has {math.prod(done.shape)} values for {n} beams")
     if workspace is None:
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
         workspace = _workspace(lambda: BeamWorkspace(groups, beams, vocab, k), "beam",
-                               gpu.current_device(), groups, beams, vocab, k)
+                               device_of(logits), groups, beams, vocab, k)
     _lib.call("tllm_beam_select", _lib.BEAM_STEP.pack(
         logits.data_ptr(), on_device(scores, "scores", _lib.F32), flags,
         on_device(out_scores, "out_scores", _lib.F32),
@@ -96,10 +96,11 @@ def beam_reorder(parents, lens, table, table_out, copy_src, copy_dst, copy_fill,
              step needs; none where src == dst or src < 0
     Every beam has to own the page that it is filling and those after it.
     """
-    shape, rows = tuple(parents.shape), tuple(table.shape)
+    shape, rows = parents.shape, table.shape
     if len(shape) != 2 or len(rows) != 2:
-        raise ValueError(f"parents and table must be 2D, got {shape}, {rows}")
-    n = shape[0] * shape[1]
+        raise ValueError(f"parents and table must be 2D, got {tuple(shape)}, {tuple(rows)}")
+    groups, beams = shape
+    n = groups * beams
     if rows[0] != n:
         raise ValueError(f"table has {rows[0]} rows for {n} beams")
     _lib.call("tllm_beam_reorder", _lib.BEAM_TABLES.pack(
@@ -108,5 +109,5 @@ def beam_reorder(parents, lens, table, table_out, copy_src, copy_dst, copy_fill,
         on_device(table_out, "table_out", _lib.I32, rows),
         on_device(copy_src, "copy_src", _lib.I32, (n,)),
         on_device(copy_dst, "copy_dst", _lib.I32, (n,)),
-        on_device(copy_fill, "copy_fill", _lib.I32, (n,)), shape[0], shape[1], rows[1],
+        on_device(copy_fill, "copy_fill", _lib.I32, (n,)), groups, beams, rows[1],
         int(page_size)), stream)

@@ -152,7 +152,7 @@ def paged_attention(kv, q, row_len, out, row_seq=None, max_len=0, keys_hint=0, w
     shape = q.shape
     if len(shape) != 3 or shape[2] != kv.head_dim:
         raise ValueError(f"q must be (rows, n_head, {kv.head_dim}), got {tuple(shape)}")
-    rows, n_head = int(shape[0]), int(shape[1])
+    rows, n_head, _ = shape
     if dtype_code(q, "q") != _lib.F32:
         raise ValueError(f"q must be float32, got {q.dtype}")
     sq = strides(q)
@@ -188,11 +188,11 @@ def _tables(cos, sin):
     if cos is None or sin is None:
         raise ValueError("cos and sin go together")
     shape = cos.shape
-    if len(shape) != 2 or tuple(sin.shape) != tuple(shape):
+    if len(shape) != 2 or sin.shape != shape:
         raise ValueError(f"cos and sin must be 2D with the same shape, got "
                          f"{tuple(shape)} and {tuple(sin.shape)}")
-    return (on_device(cos, "cos", _lib.F32), on_device(sin, "sin", _lib.F32),
-            int(shape[0]), 2 * int(shape[1]))
+    n_pos, half = shape
+    return on_device(cos, "cos", _lib.F32), on_device(sin, "sin", _lib.F32), n_pos, 2 * half
 
 
 def _index(t, name, n):
@@ -220,15 +220,16 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
     shape, cols = qkv.shape, (n_head + 2 * K) * D
     if len(shape) != 2 or shape[1] != cols:
         raise ValueError(f"qkv must be (rows, {cols}), got {tuple(shape)}")
+    src_rows = shape[0]
     if dtype_code(qkv, "qkv") != _lib.F32:
         raise ValueError(f"qkv must be float32, got {qkv.dtype}")
     ld, one = strides(qkv)
     if one != 1:
         raise ValueError("rows of qkv must be contiguous")
     require_gpu(qkv, "qkv")
-    n = int(shape[0]) if rows is None else int(rows)
-    if n > shape[0]:
-        raise ValueError(f"{n} rows of a qkv of {shape[0]}")
+    n = src_rows if rows is None else int(rows)
+    if n > src_rows:
+        raise ValueError(f"{n} rows of a qkv of {src_rows}")
     shape = q_out.shape
     if len(shape) != 3 or shape[0] < n or shape[1] != n_head or shape[2] != D:
         raise ValueError(f"q_out must be ({n}, {n_head}, {D}), got {tuple(shape)}")
@@ -236,11 +237,12 @@ def paged_append(kv, qkv, row_pos, q_out, cos=None, sin=None, *, n_head, row_seq
     at = qkv.data_ptr()
     r = _lib.PAGED_ROWS.pack(
         at, at + n_head * D * 4, at + (n_head + K) * D * 4,
-        on_device(q_out, "q_out", _lib.F32), 0, _index(row_seq, "row_seq", n),
-        _index(row_pos, "row_pos", n),
-        _index(lens_out, "lens_out", kv.n_seq),
+        on_device(q_out, "q_out", _lib.F32), 0,
+        0 if row_seq is None else on_device(row_seq, "row_seq", _lib.I32, (n,)),
+        on_device(row_pos, "row_pos", _lib.I32, (n,)),
+        0 if lens_out is None else on_device(lens_out, "lens_out", _lib.I32, (kv.n_seq,)),
         cos_t, sin_t, ld, D, ld, D, ld, D, n_head * D, D, _lib.F32, n, n_head, rotary,
-        n_pos, bool(interleaved), bool(blocked), int(qkv.shape[0]))
+        n_pos, bool(interleaved), bool(blocked), src_rows)
     _lib.call("tllm_paged_append", kv._ref, r, stream)
     return q_out
 
