@@ -587,7 +587,8 @@ __device__ __forceinline__ PageSpan page_span(const AttnParams &p, int len, int 
 // another. (Short intervals at the end of the shares, for the CTAs
 // that are done first, balance the SMs' bandwidth, but every further segment
 // costs its CTA about 2 us and its pair's join 0.15 us: 64 x 24/8/128 took 200
-// us with them and 192 without, one row of 131071 keys 93 and 96.)
+// us with two of 7 tiles, 203 with four of 3 and 192 without; one row of 131071
+// keys 93.5, 116 and 96, and 90 without them since.)
 struct Segment {
   int row, y;      // row of this block of rows, head group; row < 0: no more
   int t0, t1;      // tiles of the pair
