@@ -1,0 +1,123 @@
+"""Beam selection on a B200 where its numbers and its paths are hardest: many
+steps of one thread, large logits, masks of the type's lowest value, scores that
+collapse in fp32, row strides.
+
+Oracle: base + ((x - max) - log(sum exp(x - max))) in 64 bits, which keeps the
+logarithm beside a maximum of 1e38 too. Tolerance 2^-16 for scores below 64: a
+sum of up to 160 fp32 additions of positive terms is off by less than 160 * 2^-24
+= 2^-16.7 of itself, a term by 2^-22 of the exponential and 15 * 2^-23 of its
+argument (terms further below the maximum do not count), the subtraction and the
+logarithm by 2^-21. Scores near the type's lowest value are off by their own
+rounding, 2^-23.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from triton_llm import gpu
+from triton_llm.kernels import beam_select
+
+pytestmark = pytest.mark.gpu
+
+LOWEST = np.finfo(np.float32).min
+# more rows than a GPU has places for CTAs: a row is not cut into parts, and a
+# thread reads a step of 4096 logits of it after another
+MANY = 600
+
+
+def candidates(logits, scores, done=None, pad=0):
+    """(groups, beams * vocab) candidate scores in 64 bits."""
+    G, W = scores.shape
+    x = logits.astype(np.float64).reshape(G, W, -1)
+    m = x.max(axis=2, keepdims=True)
+    lp = (x - m) - np.log(np.exp(x - m).sum(axis=2, keepdims=True))
+    c = scores[:, :, None].astype(np.float64) + lp
+    if done is not None:
+        for g, b in np.argwhere(done != 0):
+            c[g, b] = -np.inf
+            c[g, b, pad] = scores[g, b]
+    return c.reshape(G, -1)
+
+
+def best(c, k, vocab):
+    """The k best, ties to the lowest index."""
+    at = np.argsort(-c, axis=1, kind="stable")[:, :k]
+    return np.take_along_axis(c, at, 1), at // vocab, at % vocab
+
+
+def run(logits, scores, k, done=None, pad=0):
+    G = scores.shape[0]
+    s, p, t = (gpu.allocate((G, k), d) for d in (np.float32, np.int32, np.int32))
+    beam_select(logits if hasattr(logits, "data_ptr") else gpu.to_device(logits),
+                gpu.to_device(scores), s, p, t,
+                done=None if done is None else gpu.to_device(done.astype(np.int32)),
+                pad_token=pad)
+    return s.to_numpy(), p.to_numpy(), t.to_numpy()
+
+
+def many(rows):
+    """The rows again and again, MANY of them."""
+    return np.ascontiguousarray(np.resize(rows, (MANY, rows.shape[1])))
+
+
+@pytest.mark.parametrize("V", [128256, 50257])
+def test_large_logits_in_many_steps(V):
+    """32 (or 13) steps a thread: the running sum keeps its precision whatever
+    the logits' size."""
+    rng = np.random.default_rng(V)
+    rows = (rng.standard_normal((8, V)) * 3).astype(np.float32)
+    rows += np.array([0, 10, -20, 100, -100, 1000, -1000, 4000], np.float32)[:, None]
+    zero = np.zeros((MANY, 1), np.float32)
+    s, _, t = run(many(rows), zero, 8)
+    ws, _, wt = best(candidates(rows, zero[:8]), 8, V)
+    assert (t == np.resize(wt, t.shape)).all()
+    assert np.abs(s - np.resize(ws, s.shape)).max() < 2.0 ** -16
+
+
+def masked_rows(V):
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((10, V)).astype(np.float32)
+    x[0, :V // 2] = LOWEST               # a range of tokens, whole steps of it
+    x[1, 1:] = LOWEST                    # all but one
+    x[2, :-1] = LOWEST
+    x[3, ::2] = LOWEST
+    x[4] = LOWEST                        # all: the tokens are equally likely
+    x[5, :] = LOWEST / 2
+    x[5, 77] = LOWEST / 4
+    x[6] = -LOWEST                       # the same at the other end
+    x[7, 100:200] = -LOWEST
+    x[8, :] = LOWEST
+    x[8, 9:V - 9] = -np.inf              # both kinds of mask
+    x[9, 17:4500] = LOWEST
+    return x
+
+
+@pytest.mark.parametrize("rows", [10, MANY])
+@pytest.mark.parametrize("V,k", [(20000, 8), (20002, 64), (9001, 1)])
+def test_masks_of_the_lowest_value(rows, V, k):
+    """Finite logits whatever their size: masks of the type's lowest value on
+    some, most and all tokens of a row."""
+    x = masked_rows(V)
+    with np.errstate(all="ignore"):
+        ws, _, wt = best(candidates(x, np.zeros((10, 1), np.float32)), k, V)
+    s, _, t = run(many(x) if rows == MANY else x, np.zeros((rows, 1), np.float32), k)
+    ws, wt = np.resize(ws, s.shape), np.resize(wt, t.shape)
+    assert (t == wt).all()
+    fine = np.isfinite(ws)
+    assert (s[~fine] == ws[~fine]).all()
+    assert (np.abs(s[fine] - ws[fine]) <= 2.0 ** -16 + 2.0 ** -22 * np.abs(ws[fine])).all()
+
+
+def test_a_masked_beam_beside_others():
+    """A beam whose tokens are all masked alike has its 1 / vocab candidates
+    among the other beams'."""
+    V = 9000
+    x = np.random.default_rng(4).standard_normal((4, V)).astype(np.float32) * 4
+    x[2] = LOWEST
+    scores = np.array([[-9, -30, 0, -5]], np.float32)
+    s, p, t = run(x, scores, 12)
+    ws, wp, wt = best(candidates(x, scores), 12, V)
+    assert (p == wp).all() and (t == wt).all() and (wp == 2).any() and (wp != 2).any()
+    assert np.abs(s - ws).max() < 2.0 ** -16

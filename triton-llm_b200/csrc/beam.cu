@@ -2,8 +2,11 @@
 // vocabulary (tllm_beam_select) and the reordering of the beams' page tables
 // (tllm_beam_reorder).
 //
-// Selection: candidate (b, t) of a group scores s_b + (x_bt - L_b) with
-// L_b = max + log sum exp(x_bt - max). Within a beam the order is that of its
+// Selection: candidate (b, t) of a group scores
+//   s_b + ((x_bt - m_b) - log sum_t exp(x_bt - m_b)),   m_b = max_t x_bt,
+// where every logit is taken less the maximum before it is scaled, multiplied or
+// rounded: m_b itself may be of any size (a mask of the type's lowest value,
+// 1000 with its steps of 2^-14). Within a beam the order is that of its
 // logits, so a CTA that reads a part of one row needs to keep only the part's
 // max, its sum of exponentials and its k largest logits; the last CTA of a
 // group to finish joins them. Each logit is read once.
@@ -159,7 +162,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
   __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
   __shared__ int s_n, s_last;
-  __shared__ float s_base[kMaxBeams], s_lse[kMaxBeams];
+  __shared__ float s_base[kMaxBeams], s_max[kMaxBeams], s_log[kMaxBeams];
   __shared__ int s_done[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -198,11 +201,14 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
 #pragma unroll
       for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, v[i]);
       // (a NaN anywhere, or +inf, makes the sum NaN; -inf alone leaves it 0)
-      const float mn = fmaxf(m, top), zero = mn == -INFINITY ? 0.f : mn * kLog2e;
+      const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
       float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2(fmaf(v[i], kLog2e, -zero));
-      s = s * fast_exp2(fmaf(m, kLog2e, -zero)) + ((add[0] + add[1]) + (add[2] + add[3]));
+      for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2((v[i] - base) * kLog2e);
+      // (a factor of exactly 1 while the maximum stays: a rounding of it would
+      // compound over the steps)
+      if (mn != m) s *= fast_exp2((m - mn) * kLog2e);
+      s += (add[0] + add[1]) + (add[2] + add[3]);
       if (t0 == begin) {
         m = top;
         return;
@@ -388,7 +394,8 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     if (lane == 0) {
       s_done[b] = done;
       s_base[b] = base;
-      s_lse[b] = mm + logf(ss);
+      s_max[b] = mm;
+      s_log[b] = logf(ss);
     }
   }
   __syncthreads();
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       uint64_t made = 0;
       if (i < n) {
         const int b = i / per, c = i - b * per;
-        const float base = s_base[b], lse = s_lse[b];
+        const float base = s_base[b], top = s_max[b], log_sum = s_log[b];
         float score = -INFINITY;
         uint32_t token = c;
         bool is = true;
@@ -413,12 +420,13 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
           is = c < k;
           token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
           if (c == 0) score = base;
-        } else if (!(fabsf(lse) < INFINITY) || !(fabsf(base) < INFINITY)) {
+        } else if (!(fabsf(top) < INFINITY && fabsf(log_sum) < INFINITY &&
+                     fabsf(base) < INFINITY)) {
           is = c < k;   // the beam has no finite candidate
         } else {
           is = key[j] != 0;
           token = key_index(key[j]);
-          score = base + (key_value(key[j]) - lse);
+          score = base + ((key_value(key[j]) - top) - log_sum);
         }
         if (!(score == score)) score = -INFINITY;
         if (is) made = rank_key(score, (uint32_t)b * p.vocab + token);
