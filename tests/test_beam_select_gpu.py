@@ -174,3 +174,57 @@ def test_scores_that_all_collapse():
     s, p, t = run(x[1:2], scores[:, 1:2], 6)
     assert t[0].tolist() == [5, 50, 500, 0, 1, 2]
     assert (s[0, :3] == np.float32(-1e30)).all() and (s[0, 3:] == -np.inf).all()
+
+
+def crowded(V, lanes, kVec=True):
+    """Rows whose large values all lie in the shares of a few threads, in every
+    step of 4096 logits; the largest in the last ones."""
+    rng = np.random.default_rng(V + lanes)
+    at = np.arange(V)
+    warp, inner = at % 4096 // 512, at % 512
+    lane = inner % 128 // 4 if kVec else inner % 32
+    x = rng.standard_normal((6, V)).astype(np.float32)
+    for r in range(6):
+        mine = np.isin(warp * 32 + lane, rng.choice(256, lanes, replace=False))
+        n = int(mine.sum())
+        large = 10 + rng.permutation(n).astype(np.float32) / 1024
+        x[r, mine] = [np.sort(large), np.sort(large)[::-1], large, np.round(large * 4) / 4,
+                      np.full(n, 11, np.float32), large][r]
+    x[5, ::3] = -np.inf
+    return x
+
+
+@pytest.mark.parametrize("lanes", [1, 3, 20])
+@pytest.mark.parametrize("V,k", [(40000, 1), (40000, 8), (40001, 64), (24576, 64)])
+def test_values_crowded_into_few_threads(V, k, lanes):
+    """A thread's third and later steps hold the best values (they are read
+    again), and with 20 such threads more values pass the bound than the list
+    holds (k rounds over all of them)."""
+    x = crowded(V, lanes, V % 4 == 0)
+    zero = np.zeros((MANY, 1), np.float32)
+    s, _, t = run(many(x), zero, k)
+    # (equal logits are equal scores; unequal ones are 2^-10 apart)
+    ws, _, wt = best(candidates(x, zero[:6]), k, V)
+    assert (t == np.resize(wt, t.shape)).all()
+    assert np.abs(s - np.resize(ws, s.shape)).max() < 2.0 ** -16
+
+
+@pytest.mark.parametrize("V,ld", [(5000, 5004), (5000, 5001), (3, 8), (128256, 128300)])
+@pytest.mark.parametrize("G,W", [(1, 4), (3, 2), (75, 8)])
+def test_rows_wider_than_the_vocabulary(V, ld, G, W):
+    """Logits with a row stride above the vocabulary, whose rest is NaN."""
+    torch = pytest.importorskip("torch")
+    if G * W * ld > 1 << 25:
+        G, W = 4, 2
+    rng = np.random.default_rng(ld)
+    x = (rng.standard_normal((G * W, V)) * 3).astype(np.float32)
+    scores = (-rng.random((G, W)) * 30).astype(np.float32)
+    wide = torch.full((G * W, ld), float("nan"))
+    wide[:, :V] = torch.from_numpy(x)
+    wide = wide.cuda()
+    torch.cuda.synchronize()
+    k = min(V, 5)
+    s, p, t = run(wide[:, :V], scores, k)
+    ws, wp, wt = best(candidates(x, scores), k, V)
+    assert (p == wp).all() and (t == wt).all()
+    assert np.abs(s - ws).max() < 2.0 ** -16
