@@ -175,6 +175,41 @@ def memset(t: DeviceTensor, value: int = 0):
     _lib.call("tllm_memset", t.ptr, int(value), t.nbytes, None)
 
 
+class Scratch:
+    """``nbytes`` of device memory for kernels of any stream, its first ``zeros``
+    bytes (default: all) zero-filled when the constructor returns. It is no part
+    of the library stream's pool, which would give it out again in that stream's
+    order alone: releasing it waits for the device's work. Not made or released
+    within a graph capture."""
+
+    def __init__(self, nbytes: int, zeros: int | None = None):
+        _initialize()
+        self.nbytes = int(nbytes)
+        self.device = current_device()
+        self.ptr = ctypes.c_void_p()
+        _lib.call("tllm_malloc_static", ctypes.byref(self.ptr), max(self.nbytes, 1))
+        _lib.call("tllm_memset", self.ptr, 0, self.nbytes if zeros is None else int(zeros),
+                  None)
+        synchronize()
+
+    def data_ptr(self):
+        return self.ptr.value
+
+    def __del__(self):
+        if _lib is None or _lib._lib is None or not getattr(self, "ptr", None):
+            return
+        try:
+            lib = _lib._lib
+            cur = ctypes.c_int(0)
+            lib.tllm_get_device(ctypes.byref(cur))
+            lib.tllm_set_device(self.device)
+            lib.tllm_device_synchronize()
+            lib.tllm_free_static(self.ptr)
+            lib.tllm_set_device(cur.value)
+        except Exception:
+            pass
+
+
 def to_device(arr: np.ndarray):
     """Copy a numpy array to the GPU."""
     _initialize()

@@ -10,8 +10,6 @@ from __future__ import annotations
 import ctypes
 import math
 
-import numpy as np
-
 from triton_llm import gpu, _lib
 from ._common import device_of, dtype_code, on_device, require_gpu, strides
 from .paged import _workspace
@@ -19,13 +17,14 @@ from .paged import _workspace
 
 class BeamWorkspace:
     """Scratch of ``beam_select`` (allocated once; calls that overlap on the
-    GPU need one each)."""
+    GPU need one each). Ready for any stream when it has been made, and released
+    only after the device's work."""
 
     def __init__(self, groups, beams, vocab, k):
         n = ctypes.c_size_t()
         _lib.call("tllm_beam_workspace", int(groups), int(beams), int(vocab), int(k),
                   ctypes.byref(n))
-        self._buf = gpu.zeros((max(n.value // 4, 1),), np.int32)
+        self._buf = gpu.Scratch(n.value)
         self.ptr, self.nbytes = self._buf.data_ptr(), n.value
 
 

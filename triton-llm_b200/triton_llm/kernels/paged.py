@@ -19,8 +19,6 @@ from __future__ import annotations
 import ctypes
 import math
 
-import numpy as np
-
 from triton_llm import gpu, _lib
 from ._common import dtype_code, on_device, require_gpu, strides
 
@@ -81,17 +79,18 @@ class PagedKV:
 
 class PagedWorkspace:
     """Scratch of ``paged_attention`` for up to ``rows`` rows (allocated once;
-    calls that overlap on the GPU need one each)."""
+    calls that overlap on the GPU need one each). Ready for any stream when it has
+    been made, and released only after the device's work."""
 
     def __init__(self, rows, n_head, n_kv_head, head_dim):
         pb, cb = ctypes.c_size_t(), ctypes.c_size_t()
         _lib.call("tllm_paged_attention_workspace", int(rows), int(n_head),
                   int(n_kv_head), int(head_dim), ctypes.byref(pb), ctypes.byref(cb))
         self.key = (int(rows), int(n_head), int(n_kv_head), int(head_dim))
-        self._partial = gpu.allocate((max(pb.value // 4, 1),), np.float32)
-        self._counters = gpu.zeros((max(cb.value // 4, 1),), np.int32)
-        self.partial, self.partial_bytes = self._partial.data_ptr(), pb.value
-        self.counters, self.counter_bytes = self._counters.data_ptr(), cb.value
+        at = -(-cb.value // 256) * 256   # counters, then the partials
+        self._buf = gpu.Scratch(at + pb.value, zeros=at)
+        self.counters, self.counter_bytes = self._buf.data_ptr(), cb.value
+        self.partial, self.partial_bytes = self.counters + at, pb.value
 
 
 _workspaces: dict = {}
