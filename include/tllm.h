@@ -282,9 +282,10 @@ typedef struct {
  * right for any value. row_len above the table's capacity is clamped (bit 2 of the
  * device error word). bf16 and fp32 caches; head_dim up to 512 whose rows
  * are whole 16-byte units. Scratch: partial (tllm_paged_attention_workspace;
- * fewer bytes give fewer, longer splits) and counters, zero-filled once and
- * zero again after every call (but for one that set bit 1 of the device error
- * word: fill them again); a call that overlaps another on the GPU needs its
+ * for many rows 512 MB, or a few KB a row if that is more; fewer bytes give
+ * fewer, longer splits) and counters, zero-filled once and zero again after every
+ * call (but for one that set bit 1 of the device error word: fill them again); a
+ * call that overlaps another on the GPU needs its
  * own. No counterpart in the reference (its decode attention over the
  * preallocated cache: triton_llm/kernels/attention_gqa.py:149-269).
  */

@@ -58,6 +58,27 @@ def test_ready_for_any_stream(device, make):
     assert "tllm_device_synchronize" in log[at:log.index("tllm_free_static")]
 
 
+def test_attention_scratch_is_bounded():
+    """Calls of many rows (the prompt rows of a windowed prefill): their rows fill
+    the GPU, so that splits are few or none; the scratch stays within 512 MB. A
+    decode batch keeps its 8 splits and more."""
+    lib = _lib.load()
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+
+    def need(rows, heads, kv, dim):
+        assert lib.tllm_paged_attention_workspace(rows, heads, kv, dim, ctypes.byref(a),
+                                                  ctypes.byref(b)) == _lib.OK
+        return a.value
+    for rows, heads, kv, dim in [(16384, 24, 8, 128), (32768, 32, 8, 128), (131072, 9, 3, 64),
+                                 (1 << 20, 8, 1, 128)]:
+        # (two parts of a share for each of 296 CTAs and 512 rows, if that is more)
+        shares = rows // 512 * 296 * 2 * (heads // kv) * (dim + 2) * 4
+        assert need(rows, heads, kv, dim) <= max(1 << 29, shares)
+    for rows in (1, 64, 512):
+        row = 24 * 2 * (128 + 2) * 4
+        assert need(rows, 24, 8, 128) >= 8 * rows * row
+
+
 @pytest.mark.gpu
 def test_dropped_while_another_stream_works():
     """A workspace made for one call on another stream and dropped at once, with

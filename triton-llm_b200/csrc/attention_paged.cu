@@ -1422,6 +1422,8 @@ int launch_rows_t(const AttnParams &p, int lpr, int nv, dim3 grid, cudaStream_t 
 // 17 to 1003 keys: 13.1 us with 64, 10.6 with 128, 15.3 with 256).
 constexpr int kMinKeys = 128;
 
+constexpr size_t kMaxScratch = 512u << 20;   // of the splits, whatever the rows
+
 // Keys per split, a multiple of `tile`, for `pairs` (row, head group) pairs
 // of at most max_keys keys and about `keys` in all rows.
 int plan_chunk(int tile, long rows, int n_y, long keys, long max_keys, long slots) {
@@ -1484,7 +1486,8 @@ extern "C" int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_hea
   TLLM_CHECK_ARG(n_head % n_kv_head == 0, "n_head (%d) must be divisible by n_kv_head (%d)",
                  n_head, n_kv_head);
   // One token per row and split (heads of a KV head padded to a tile of 1, 2, 4
-  // or 8): splits that fill the GPU a few times over, at least 8. Or two parts
+  // or 8): splits that fill the GPU a few times over, at least 8 within 512 MB
+  // (64000 heads of 128 in all rows; so many fill it by themselves). Or two parts
   // of up to 16 heads per share of the tensor-core kernel.
   long splits = 8192 / ((long)(rows > 0 ? rows : 1) * n_kv_head);
   if (splits > kMaxSplits) splits = kMaxSplits;
@@ -1493,7 +1496,8 @@ extern "C" int tllm_paged_attention_workspace(int rows, int n_head, int n_kv_hea
   const size_t blocks = (size_t)(rows + kRowBlock - 1) / kRowBlock;
   const size_t ctas = (size_t)kMaxPerSm * sm_count();
   const int group = n_head / n_kv_head;
-  const size_t a = (size_t)rows * n_head * 2 * splits * row;
+  const size_t all = (size_t)rows * n_head * 2 * splits * row;
+  const size_t a = all < kMaxScratch ? all : kMaxScratch;
   const size_t b = blocks * ctas * 2 * (group < 16 ? group : 16) * row;
   *partial_bytes = a > b ? a : b;
   const size_t c = (size_t)rows * n_head;
