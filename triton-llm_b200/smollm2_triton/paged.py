@@ -92,6 +92,8 @@ class PagedSession(LlamaSession):
         self._capturing = False
         self.qkv = gpu.allocate((self.B, (w.H + 2 * w.Hkv) * w.D), np.float32)
         self.attn_ws = PagedWorkspace(self.B, w.H, w.Hkv, w.D)
+        self._prompt_ws = None                    # of windowed prompts, and its rows
+        self._prompt_ws_rows = 0
 
     def _upload(self):
         self.table.from_numpy(self._table)
@@ -248,10 +250,14 @@ class PagedSession(LlamaSession):
                             sinks=self.sinks, workspace=attn_ws)
         elif self.window:
             # prompt rows over their windows
+            if M > self._prompt_ws_rows:
+                self._prompt_ws = PagedWorkspace(M, w.H, w.Hkv, w.D)
+                self._prompt_ws_rows = M
             paged_attention(self.pages[i], gpu.sub_view(q, 0, (M, w.H, w.D)),
                             gpu.sub_view(row_len, 0, (M,)), attn,
                             row_seq=gpu.sub_view(row_seq, 0, (M,)), max_len=max_len,
-                            window=self.window, sinks=self.sinks)
+                            window=self.window, sinks=self.sinks,
+                            workspace=self._prompt_ws)
         else:
             super()._attend(i, M, q, attn, row_seq, lens, decode, attn_ws, row_len, max_len)
 
