@@ -44,3 +44,31 @@ def test_windowed_prefill_keeps_its_scratch_to_itself(weights):
     for n in (70, 290, 20):
         s.prefill([prompt(n)], slots=[1])
     assert set(paged._workspaces) == before
+
+
+def test_prompts_stage_their_own_rows(weights, monkeypatch):
+    """A prompt admitted into a session of many slots stages its own keys and
+    values, not places for every slot; results are the contiguous session's."""
+    from smollm2_triton.engine import LlamaSession
+    from smollm2_triton.paged import PagedSession
+    from triton_llm import gpu
+    prompts, slots = [prompt(33, 1), prompt(70, 2)], [9, 3]
+    want = LlamaSession(weights.dev, 12, 100).prefill(prompts, slots=slots)
+    for kw in (dict(), dict(window=80)):
+        s = PagedSession(weights.dev, 12, 100, page_size=16, **kw)
+        taken, allocate = [], gpu.allocate
+        monkeypatch.setattr(gpu, "allocate", lambda shape, *a: taken.append(shape)
+                            or allocate(shape, *a))
+        got = s.prefill(prompts, slots=slots)
+        monkeypatch.undo()
+        staged = [x for x in taken if len(x) == 4]
+        assert staged and all(x[0] == 2 for x in staged)
+        assert np.abs(got - want).max() < 1e-4 * np.abs(want).max()
+        # and the pages hold them: the next tokens agree too
+        c = LlamaSession(weights.dev, 12, 100)
+        c.prefill(prompts, slots=slots)
+        for _ in range(4):
+            s.step()
+            c.step()
+            a, b = s.logits.to_numpy()[slots], c.logits.to_numpy()[slots]
+            assert np.abs(a - b).max() < 1e-4 * np.abs(b).max()

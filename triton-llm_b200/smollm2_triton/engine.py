@@ -452,8 +452,10 @@ class LlamaSession:
             raise ValueError(f"prompt of {lens.max()} tokens exceeds max_seq {self.S}")
         return prompts, slots, lens, keep
 
-    def _prompt_rows(self, seq, pos):
-        """Called with the sequences and positions of a prefill's rows."""
+    def _prompt_seqs(self, slots, lens, pos):
+        """The sequences of ``kv`` that the prompts of these slots and lengths
+        are written to (pos: the positions of all their rows)."""
+        return slots
 
     def prefill(self, prompts, all_logits=False, slots=None):
         """Run the prompts through the model into cache sequences ``slots``
@@ -474,16 +476,16 @@ class LlamaSession:
         if M > self._prefill_rows:
             self._prefill_buffers(M, 256 << 20)
         ids = np.concatenate(prompts)
-        seq = np.repeat(slots, lens)
         pos = np.concatenate([np.arange(n, dtype=np.int32) for n in lens])
-        self._prompt_rows(seq, pos)
+        at = self._prompt_seqs(slots, lens, pos)
+        seq = np.repeat(at, lens)
         self.p_ids.from_numpy(np.pad(ids, (0, self._prefill_rows - M)))
         self.p_seq.from_numpy(np.pad(seq, (0, self._prefill_rows - M)))
         self.p_pos.from_numpy(np.pad(pos, (0, self._prefill_rows - M)))
         self.p_len.from_numpy(np.pad(pos + 1, (0, self._prefill_rows - M)))
         self._p_blocks, self._p_nblocks = None, 0
         if prefill_supported(self.kv[0][0]):
-            blocks = prefill_blocks(lens, slots)
+            blocks = prefill_blocks(lens, at)
             self._p_blocks = gpu.to_device(blocks)
             self._p_nblocks = len(blocks)
         h, x = self.p_h, self.p_x

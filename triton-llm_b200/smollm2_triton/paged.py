@@ -224,10 +224,13 @@ class PagedSession(LlamaSession):
         return len(src)
 
     # -- one layer ----------------------------------------------------------
-    def _prompt_rows(self, seq, pos):
-        k = self.kv[0][0]
-        self._p_src = gpu.to_device((seq.astype(np.int64) * k.shape[1] * k.shape[2]
-                                     + pos).astype(np.int32))
+    def _prompt_seqs(self, slots, lens, pos):
+        # one after another in the staging cache; their rows' slots for the pages
+        k, at = self.kv[0][0], np.arange(len(slots), dtype=np.int32)
+        self._p_slot = gpu.to_device(np.repeat(slots, lens).astype(np.int32))
+        self._p_src = gpu.to_device((np.repeat(at, lens).astype(np.int64) * k.shape[1]
+                                     * k.shape[2] + pos).astype(np.int32))
+        return at
 
     def _project_qkv(self, i, M, x, q, row_seq, row_pos, lens, ws, decode, fold_in):
         w = self.w
@@ -239,7 +242,7 @@ class PagedSession(LlamaSession):
         super()._project_qkv(i, M, x, q, row_seq, row_pos, lens, ws, decode, fold_in)
         k, v = self.kv[i]
         paged_write(self.pages[i], k, v, gpu.sub_view(row_pos, 0, (M,)),
-                    row_seq=gpu.sub_view(row_seq, 0, (M,)), row_src=self._p_src,
+                    row_seq=self._p_slot, row_src=self._p_src,
                     row_stride=w.D, head_stride=int(k.shape[2]) * w.D)
 
     def _attend(self, i, M, q, attn, row_seq, lens, decode, attn_ws, row_len, max_len):
@@ -255,9 +258,8 @@ class PagedSession(LlamaSession):
                 self._prompt_ws_rows = M
             paged_attention(self.pages[i], gpu.sub_view(q, 0, (M, w.H, w.D)),
                             gpu.sub_view(row_len, 0, (M,)), attn,
-                            row_seq=gpu.sub_view(row_seq, 0, (M,)), max_len=max_len,
-                            window=self.window, sinks=self.sinks,
-                            workspace=self._prompt_ws)
+                            row_seq=self._p_slot, max_len=max_len, window=self.window,
+                            sinks=self.sinks, workspace=self._prompt_ws)
         else:
             super()._attend(i, M, q, attn, row_seq, lens, decode, attn_ws, row_len, max_len)
 
@@ -271,7 +273,7 @@ class PagedSession(LlamaSession):
             self._idle(np.setdiff1d(np.arange(self.B), at))
         self._set_pages(at, lens)
         w = self.w
-        shape = (self.B, w.Hkv, int(lens.max()), w.D)
+        shape = (len(at), w.Hkv, int(lens.max()), w.D)
         dt = "bfloat16" if self.kv_bf16 else np.float32
         try:
             self.kv = [(gpu.allocate(shape, dt), gpu.allocate(shape, dt))] * w.L
@@ -280,7 +282,7 @@ class PagedSession(LlamaSession):
             self.release(at)
             raise
         finally:
-            self.kv, self._p_src = None, None
+            self.kv = self._p_src = self._p_slot = None
         self._pos[at] = lens
         for b, n in zip(at, lens):
             self._drop_outside(int(b), int(n) + 1)
