@@ -72,3 +72,16 @@ def test_prompts_stage_their_own_rows(weights, monkeypatch):
             c.step()
             a, b = s.logits.to_numpy()[slots], c.logits.to_numpy()[slots]
             assert np.abs(a - b).max() < 1e-4 * np.abs(b).max()
+
+
+def test_idle_slots_of_a_session_shorter_than_a_page(weights):
+    """An idle slot stays below max_seq (and the rotary tables' last position)
+    however long the others go on."""
+    from smollm2_triton.paged import PagedSession
+    s = PagedSession(weights.dev, 2, 20, page_size=64,
+                     rope_scaling={"type": "linear", "factor": 2.0})
+    for seed in range(4):
+        s.prefill([prompt(10, seed)], slots=[1])
+        for _ in range(10):
+            s.step()
+            assert s._pos[0] <= 20 and s.pos.to_numpy()[0] <= 20

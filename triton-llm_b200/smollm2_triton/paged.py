@@ -148,7 +148,8 @@ class PagedSession(LlamaSession):
         if self._fixed:
             self._pos += 1
             return
-        idle = ~self._live & (self._pos >= self.P)
+        # (idle slots stay within their page, and where sequences may be)
+        idle = ~self._live & (self._pos >= min(self.P, self.S))
         if (self._live & (self._pos >= self.S)).any():
             raise ValueError(f"a sequence has reached max_seq ({self.S})")
         if idle.any():
