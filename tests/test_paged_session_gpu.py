@@ -85,3 +85,23 @@ def test_idle_slots_of_a_session_shorter_than_a_page(weights):
         for _ in range(10):
             s.step()
             assert s._pos[0] <= 20 and s.pos.to_numpy()[0] <= 20
+
+
+def test_set_state_refusals_change_nothing(weights):
+    from smollm2_triton.paged import PagedSession
+    s = PagedSession(weights.dev, 3, 100, page_size=16)
+    p = prompt(40)
+    s.prefill([p], slots=[1])
+    alone = PagedSession(weights.dev, 3, 100, page_size=16)
+    alone.prefill([p], slots=[1])
+    for pos, ids in [([1, 101, 3], [0, 0, 0]), ([1, 2], [0, 0]), ([1, 2, 3, 4], [0] * 4),
+                     ([1, -2, 3], [0, 0, 0]), ([1, 2, 3], [0, 0])]:
+        with pytest.raises(ValueError, match="set_state"):
+            s.set_state(np.array(pos), np.array(ids))
+        assert s.pool.used == 3
+    for _ in range(10):
+        s.step()
+        alone.step()
+        assert (s.logits.to_numpy()[1] == alone.logits.to_numpy()[1]).all()
+    s.set_state(np.array([100, 0, 16]), np.zeros(3, np.int32))
+    assert s.pool.used == 7 + 1 + 1

@@ -293,6 +293,10 @@ class PagedSession(LlamaSession):
     def set_state(self, pos, ids):
         """Sequences of these lengths with whatever their pages hold."""
         pos = np.asarray(pos, np.int64)
+        if pos.shape != (self.B,) or np.shape(ids) != (self.B,) or (pos < 0).any() or \
+                (pos > self.S).any():
+            raise ValueError(f"set_state needs {self.B} lengths within max_seq ({self.S}) "
+                             f"and as many tokens, got {pos.tolist()}, {np.shape(ids)}")
         self._set_pages(range(len(pos)), pos)
         for b, n in enumerate(pos):
             self._drop_outside(b, int(n) + 1)
