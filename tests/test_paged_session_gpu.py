@@ -105,3 +105,22 @@ def test_set_state_refusals_change_nothing(weights):
         assert (s.logits.to_numpy()[1] == alone.logits.to_numpy()[1]).all()
     s.set_state(np.array([100, 0, 16]), np.zeros(3, np.int32))
     assert s.pool.used == 7 + 1 + 1
+
+
+def test_generate_paged_holds_what_its_sequences_need(weights, monkeypatch):
+    """One long prompt among short ones does not make every sequence's pages as
+    many as its own."""
+    from smollm2_triton import paged
+    made, init = [], paged.PagedSession._cache_buffers
+
+    def record(self):
+        made.append(self.n_pages)
+        init(self)
+    monkeypatch.setattr(paged.PagedSession, "_cache_buffers", record)
+    prompts = [prompt(n, n) for n in (90, 3, 16, 1)]
+    got = weights.generate_paged(prompts, max_new_tokens=17, page_size=16)
+    assert made == [7 + 2 + 3 + 2]           # of 107, 20, 33 and 18 tokens
+    want = weights.generate_batch(prompts, max_new_tokens=17)
+    assert [g.tolist() for g in got] == [w.tolist() for w in want]
+    weights.generate_paged(prompts, max_new_tokens=17, page_size=16, n_pages=20)
+    assert made[-1] == 20

@@ -295,15 +295,18 @@ class SmolLM2ForCausalLM:
     def generate_paged(self, prompts, max_new_tokens: int = 20,
                        eos_token_id: int | None = None, use_graph: bool = True, **session):
         """``generate_batch`` over a paged KV cache. ``session``: arguments of
-        ``PagedSession`` -- page_size, n_pages, window and sinks (a sliding
-        window with a few first tokens that stay visible), rope_scaling (contexts
-        past the model's own, ``scaled_cos_sin``)."""
+        ``PagedSession`` -- page_size, n_pages (default: what every sequence
+        needs at its own length), window and sinks (a sliding window with a few
+        first tokens that stay visible), rope_scaling (contexts past the model's
+        own, ``scaled_cos_sin``)."""
         from .paged import PagedSession
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
         longest = max(len(p) for p in prompts) + max_new_tokens
         if longest > self.config.max_position_embeddings and not session.get("rope_scaling"):
             raise ValueError(f"{longest} tokens exceed max_position_embeddings "
                              f"({self.config.max_position_embeddings})")
+        P = max(1, int(session.get("page_size", 64)))
+        session.setdefault("n_pages", sum(-(-(len(p) + max_new_tokens) // P) for p in prompts))
         self._init_gpu_weights()
         sess = PagedSession(self.dev, len(prompts), longest, kv_dtype=self._kv_dtype,
                             act_dtype=self._act_dtype, **session)
