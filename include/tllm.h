@@ -400,8 +400,8 @@ int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
  * as -inf. out_done (groups, k), may be NULL: 1 for a candidate whose beam is
  * done or whose token is eos_token (-1: none), else 0. 1 <= k <= 64,
  * k <= vocab, beams <= 32, at most 65535 rows. Scratch: tllm_beam_workspace
- * bytes, zero-filled once; a call that overlaps another on the GPU needs its
- * own. The reference selects greedily or by sampling
+ * bytes (enough for fewer rows, a smaller k and any vocabulary too), zero-filled
+ * once; a call that overlaps another on the GPU needs its own. The reference selects greedily or by sampling
  * (smollm2_triton/model.py:566-584).
  */
 int tllm_beam_workspace(int groups, int beams, int vocab, int k, size_t *bytes);

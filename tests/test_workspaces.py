@@ -8,7 +8,7 @@ import ctypes
 import pytest
 
 from triton_llm import _lib, gpu
-from triton_llm.kernels import BeamWorkspace, PagedWorkspace
+from triton_llm.kernels import BeamWorkspace, PagedWorkspace, beam_select
 
 
 class FakeDevice:
@@ -16,7 +16,8 @@ class FakeDevice:
 
     NAMES = ("tllm_malloc", "tllm_free", "tllm_malloc_static", "tllm_free_static",
              "tllm_memset", "tllm_synchronize", "tllm_stream_synchronize",
-             "tllm_device_synchronize", "tllm_get_device", "tllm_set_device")
+             "tllm_device_synchronize", "tllm_get_device", "tllm_set_device",
+             "tllm_beam_select")
 
     def __init__(self, real):
         self._real, self.log = real, []
@@ -27,6 +28,8 @@ class FakeDevice:
 
         def call(*args):
             self.log.append(name)
+            if name == "tllm_beam_select":
+                self.select = args[0]
             if name in ("tllm_malloc", "tllm_malloc_static"):
                 args[0]._obj.value = 1 << 20
             return 0
@@ -79,12 +82,55 @@ def test_attention_scratch_is_bounded():
         assert need(rows, 24, 8, 128) >= 8 * rows * row
 
 
+class Tensor:
+    """A described tensor, for calls that do not reach the device."""
+
+    def __init__(self, shape, dtype="float32"):
+        self.shape, self.dtype, self.is_cuda = tuple(shape), f"any.{dtype}", True
+
+    def data_ptr(self):
+        return 4096
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+
+def test_beam_scratch_of_ever_other_shapes(device, monkeypatch):
+    """The library stream's own workspaces stay few whatever numbers of requests,
+    beams, tokens and continuations come, and are large enough for each."""
+    from triton_llm.kernels import paged
+    kept = {}
+    monkeypatch.setattr(paged, "_workspaces", kept)
+    real, need = device._real, ctypes.c_size_t()
+    for groups in (1, 3, 5, 16, 37, 100, 1000):
+        for beams in (1, 2, 5, 8):
+            for vocab in (100, 5000, 32000, 128256):
+                for k in {1, 3, beams, 2 * beams, 64}:
+                    assert real.tllm_beam_workspace(groups, beams, vocab, k,
+                                                    ctypes.byref(need)) == _lib.OK
+                    beam_select(Tensor((groups * beams, vocab)), Tensor((groups, beams)),
+                                Tensor((groups, k)), Tensor((groups, k), "int32"),
+                                Tensor((groups, k), "int32"))
+                    used = packed(device.select)
+                    assert used >= need.value
+    assert len(kept) <= 14 * 7
+    assert sum(ws.nbytes for ws in kept.values()) < 64 << 20
+
+
+def packed(step):
+    """workspace_bytes of a packed tllm_beam_step."""
+    return _lib.BEAM_STEP.unpack(step)[8]
+
+
 @pytest.mark.gpu
 def test_dropped_while_another_stream_works():
     """A workspace made for one call on another stream and dropped at once, with
     the library stream writing over whatever memory it gets meanwhile."""
     import numpy as np
-    from triton_llm.kernels import PagedKV, beam_select, paged_attention
+    from triton_llm.kernels import PagedKV, paged_attention
     rng = np.random.default_rng(0)
     R, K, P, n = 8, 8, 64, 256
     kv = PagedKV(*[gpu.to_device_bf16(rng.standard_normal((n, K, P, 128), np.float32))

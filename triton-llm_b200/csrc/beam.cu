@@ -650,11 +650,11 @@ extern "C" int tllm_beam_workspace(int groups, int beams, int vocab, int k, size
   TLLM_CHECK_ARG(vocab >= 1 && vocab < (1 << 27), "vocab (%d) must be in [1, 2^27)", vocab);
   TLLM_CHECK_ARG(k >= 1 && k <= kMaxK && k <= vocab, "k (%d) must be in [1, %d] and <= vocab (%d)",
                  k, kMaxK, vocab);
-  const size_t rows = (size_t)groups * beams;
-  int chunk;
-  const size_t chunks = parts_of((int)rows, vocab, &chunk);
-  *bytes = kCounterBytes + align256(rows * chunks * sizeof(float4)) +
-           rows * chunks * k * sizeof(uint64_t);
+  // the parts of all rows are at most as many (parts_of), whatever the vocabulary
+  // and for fewer rows too
+  const size_t rows = (size_t)groups * beams, most = (size_t)kCtasPerSm * sm_count();
+  const size_t parts = rows > most ? rows : most;
+  *bytes = kCounterBytes + align256(parts * sizeof(float4)) + parts * k * sizeof(uint64_t);
   return TLLM_OK;
 }
 
