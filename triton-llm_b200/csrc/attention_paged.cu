@@ -1071,6 +1071,13 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     }
   };
   int it = 0, jobs = 0;
+  // whether the joining warp has the last job (until then s_job is not ours)
+  auto job_taken = [&]() {
+    if (jobs == 0 || wait_phase(job_empty, (jobs - 1) & 1, &s_fail)) return true;
+    if (!s_fail) atomicOr(p.err, DEV_ERR_WAIT_TIMEOUT);
+    s_fail = 1;
+    return false;
+  };
   Segment g;
   if (!next_segment(&g)) return;
   if (QB == 1 && g.row >= 0) load_q(g);
@@ -1301,8 +1308,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
       // warp, or at the end of the share all consumers
       bar_consumers(NCW * 32);
       if (next.row >= 0) {
-        if (tid == 0) {
-          if (jobs > 0 && !wait_phase(job_empty, (jobs - 1) & 1, &s_fail)) s_fail = 1;
+        if (tid == 0 && job_taken()) {
           s_job = Job{base + g.first, out_row, g.first, g.parts, G};
           arrive(job_full);
         }
@@ -1325,8 +1331,7 @@ __global__ void __launch_bounds__(Tile<D>::THREADS, QB == 1 || D == 64 ? 2 : 1)
     }
     g = next;
   }
-  if (tid == 0) {
-    if (jobs > 0 && !wait_phase(job_empty, (jobs - 1) & 1, &s_fail)) s_fail = 1;
+  if (tid == 0 && job_taken()) {
     s_job.parts = 0;
     arrive(job_full);
   }
