@@ -20,7 +20,7 @@
 // values) and the largest value outside them. The k-th largest of the threads'
 // own maxima is a key that the part's k largest reach; the few threads that
 // reach it read those steps again (from L2) and list what does. Bound by HBM
-// while it reads (9 us of 26 for 16 x 8 beams over 128256 tokens, 66 MB), then
+// while it reads (9 us of 25 for 16 x 8 beams over 128256 tokens, 66 MB), then
 // by the latency of a few dependent passes; a list of candidates kept up during
 // the reading took 31 us, k rounds of maxima over all values 121.
 #include <cmath>
@@ -170,9 +170,8 @@ struct GroupRows {
 
 // Puts the candidates that score the same as the last of top[k] in order where
 // the parts' lists left some out: the rows of those beams are read in order of
-// their tokens until enough are found. By all threads; rare. (Inlined: as a call
-// it costs every launch registers, 16 x 8 x 128256 0.4 us, 640 rows 2.3.)
-__device__ __forceinline__ void settle_ties(const BeamParams &p, const GroupRows &rows,
+// their tokens until enough are found. By all threads; rare.
+__device__ __noinline__ void settle_ties(const BeamParams &p, const GroupRows &rows,
                                          int group, uint64_t *top, uint64_t *list,
                                          int *s_warp) {
   constexpr int kDeep = 8;   // tokens of a thread on the way
@@ -236,8 +235,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
   __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
   __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
-  __shared__ uint32_t s_rest;
-  __shared__ int s_n, s_last;
+  __shared__ int s_n, s_last, s_skip;
   __shared__ GroupRows s_rows;
   __shared__ int s_count[kBeamWarps];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     const int per = warp_largest(mine, k, s_list + warp * 32);
     if (tid == 0) {
       s_bound = 0;
-      s_n = s_rest = 0;
+      s_n = s_skip = 0;
     }
     __syncthreads();
     // (four lanes a key, each against two warps' keys)
@@ -353,48 +351,42 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     __syncthreads();
     const uint64_t bound = s_bound;
     const float least = bound ? key_value(bound) : -INFINITY;
-    // list the values that reach it; a thread's other steps only if their
-    // largest value may (equal ones do not where the step starts past the
-    // bound's index). `rest`: what no value below the bound's exceeds
-    float rest = m;
-    if (any && m >= least) {
-      rest = -INFINITY;
+    // list the values that reach it, and for equal scores those just below (which
+    // covers scores of up to 2^14); a thread's other steps only if their largest
+    // value may be such
+    const float low = least - fmaf(fabsf(least), 0x1p-20f, 0x1p-8f);
+    if (any && m >= low) {
       auto list = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-          if (!(v[i] >= least)) {
-            rest = fmaxf(rest, v[i]);
-            continue;
-          }
-          if (t0 + at(i) >= end) continue;
+          if (!(v[i] >= low) || t0 + at(i) >= end) continue;
           const uint64_t key = rank_key(v[i], (uint32_t)(t0 + at(i)));
-          if (key < bound) continue;
+          if (key < bound && v[i] == least) continue;
           const int to = atomicAdd(&s_n, 1);
           if (to < kKeys) s_list[to] = key;
         }
       };
-      auto may = [&](float top, int t) {
-        if (!bound || top > least || (top == least && t <= (int)key_index(bound))) return true;
-        rest = fmaxf(rest, top);
-        return false;
+      // (many threads may have values equal to the bound's, past its index: what
+      // else lies in their other steps is not looked for)
+      auto may = [&](float top) {
+        const bool skip = top == least && mine < bound;
+        if (skip) s_skip = 1;
+        return top >= low && !skip;
       };
       list(best);
-      if (second != best && may(m2, second)) {
+      if (second != best && may(m2)) {
         load(second, v);
         list(second);
       }
-      if (may(other, begin)) {
+      if (may(other)) {
 #pragma unroll 1
         for (int t = begin; t < end; t += kStep) {
           if (t == best || t == second) continue;
-          if (!may(other, t)) break;
           load(t, v);
           list(t);
         }
       }
     }
-    const uint32_t most = __reduce_max_sync(~0u, (uint32_t)(rank_key(rest, 0) >> 32));
-    if (lane == 0) atomicMax(&s_rest, most);
     __syncthreads();
     const size_t part = (size_t)row * p.chunks + chunk;
     uint64_t *out = p.lists + part * k;
@@ -402,13 +394,13 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       if (rank < k)
         out[rank] = key;
       else
-        p.stats[part].z = key_value(key);
+        p.stats[part].z = s_skip ? fmaxf(least, key_value(key)) : key_value(key);
     };
     const int n = s_n;
     if (n <= kKeys) {
       rank_keys(s_list, n, k + 1, put);
       for (int i = n + tid; i < k; i += kBeamThreads) out[i] = 0;   // a short last part
-      if (tid == 0 && n <= k) p.stats[part].z = key_value((uint64_t)s_rest << 32);
+      if (tid == 0 && n <= k) p.stats[part].z = s_skip ? least : low;
     } else {
       // more values above the bound than the list holds (they all lie in the
       // same threads' shares): rounds of the largest below the last
