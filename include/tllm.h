@@ -392,17 +392,16 @@ int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
  * each (rows g * beams + b of logits (rows, vocab) f32, row stride ld, 0: vocab):
  *   candidate (b, t) = scores[g][b] + (logits[b][t] - logsumexp(logits[b]))
  * and the k best of each group's beams * vocab candidates, best first, equal
- * ones (as fp32 scores, whatever their logits) by the lower beam, then the lower
- * token: out_scores, out_parents (beam within the group) and out_tokens, all
- * (groups, k). Finite logits may be of any size. A beam with
+ * ones by the lower beam, then the lower token: out_scores, out_parents
+ * (beam within the group) and out_tokens, all (groups, k). A beam with
  * done[row] != 0 (done may be NULL) has one candidate, (pad_token,
  * scores[row]). NaN candidates, and all of a beam whose score is +inf, count
  * as -inf. out_done (groups, k), may be NULL: 1 for a candidate whose beam is
  * done or whose token is eos_token (-1: none), else 0. 1 <= k <= 64,
  * k <= vocab, beams <= 32, at most 65535 rows. Scratch: tllm_beam_workspace
  * bytes (enough for fewer rows, a smaller k and any vocabulary too), zero-filled
- * once; a call that overlaps another on the GPU needs its own. The reference selects greedily or by sampling
- * (smollm2_triton/model.py:566-584).
+ * once; a call that overlaps another on the GPU needs its own. The reference
+ * selects greedily or by sampling (smollm2_triton/model.py:566-584).
  */
 int tllm_beam_workspace(int groups, int beams, int vocab, int k, size_t *bytes);
 typedef struct {

@@ -123,59 +123,6 @@ def test_a_masked_beam_beside_others():
     assert np.abs(s - ws).max() < 2.0 ** -16
 
 
-def rounded(c):
-    """Candidates as the fp32 scores that they have, where these do not hang on
-    the last bits of the logarithm: every one is further than 2^-13 of a unit
-    from the middle of two."""
-    s = c.astype(np.float32)
-    unit = np.spacing(np.abs(s.max()))
-    off = np.abs(c / unit - np.floor(c / unit) - 0.5)
-    assert (off[np.isfinite(c)] > 2.0 ** -13).all()
-    return s.astype(np.float64)
-
-
-@pytest.mark.parametrize("rows", ["few", "many"])
-@pytest.mark.parametrize("V,W,k", [(20000, 1, 1), (20000, 1, 8), (5000, 4, 7), (12289, 3, 64),
-                                   (40000, 2, 33)])
-def test_equal_scores_of_unequal_logits(rows, V, W, k):
-    """Beams so unlikely that many logits give the same fp32 score: equal scores
-    go to the lower beam, then the lower token, among all candidates."""
-    rng = np.random.default_rng(V + k)
-    x = rng.standard_normal((W, V)).astype(np.float32)
-    x = np.round(x * 32) / 32
-    base = np.full((1, W), -2.0 ** 20, np.float32)       # scores in units of 1/8
-    base[0, W // 2] -= 1
-    c = rounded(candidates(x, base))
-    ws, wp, wt = best(c, k, V)
-    # (the larger logits are not what decides: some lose to lower tokens)
-    assert (best(candidates(x, base), k, V)[2] != wt).any()
-    G = 1 if rows == "few" else -(-MANY // W)
-    s, p, t = run(np.tile(x, (G, 1)), np.tile(base, (G, 1)), k)
-    assert (p == wp).all() and (t == wt).all() and (s == ws).all()
-
-
-def test_scores_that_all_collapse():
-    """All candidates of a beam equal (a score of -1e30): the first tokens, of
-    the lowest beams; finished beams and masked tokens in their places."""
-    V, k = 30000, 40
-    x = np.random.default_rng(8).standard_normal((4, V)).astype(np.float32)
-    x[1, :17] = -np.inf
-    x[1, 19:12000] = LOWEST
-    scores = np.array([[-2e30, -1e30, -1e30, -1e30]], np.float32)
-    s, p, t = run(x, scores, k)
-    assert (p[0] == 1).all() and (s == np.float32(-1e30)).all()
-    assert t[0].tolist() == [17, 18] + list(range(12000, 12000 + k - 2))
-    done = np.array([[0, 1, 0, 0]])
-    s, p, t = run(x, scores, k, done, V - 1)
-    assert p[0].tolist() == [1] + [2] * (k - 1)
-    assert t[0].tolist() == [V - 1] + list(range(k - 1))
-    x[1] = -np.inf                       # fewer than k candidates in all
-    x[1, [5, 50, 500]] = [1, 3, 2]
-    s, p, t = run(x[1:2], scores[:, 1:2], 6)
-    assert t[0].tolist() == [5, 50, 500, 0, 1, 2]
-    assert (s[0, :3] == np.float32(-1e30)).all() and (s[0, 3:] == -np.inf).all()
-
-
 def crowded(V, lanes, kVec=True):
     """Rows whose large values all lie in the shares of a few threads, in every
     step of 4096 logits; the largest in the last ones."""

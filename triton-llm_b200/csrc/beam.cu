@@ -9,10 +9,7 @@
 // 1000 with its steps of 2^-14). Within a beam the order is that of its
 // logits, so a CTA that reads a part of one row needs to keep only the part's
 // max, its sum of exponentials and its k largest logits; the last CTA of a
-// group to finish joins them. Each logit is read once. (Unequal logits may round
-// to equal scores, which go to the lower token. So a part also tells what no
-// logit below its k-th exceeds outside the list; where that scores as much as the
-// group's k-th, the group's CTA looks for such tokens in the whole row.)
+// group to finish joins them. Each logit is read once.
 //
 // Values carry their index in a 64-bit code, so all are distinct and ties are
 // in order. A thread reads its share of the part with the next 16 values on the
@@ -70,8 +67,7 @@ struct BeamParams {
   int *out_parents, *out_tokens, *out_done;
   int eos;
   int *counters;        // (groups)
-  float4 *stats;        // (rows, chunks): max, sum of exponentials, and what no
-                        // lower logit outside the part's list exceeds
+  float2 *stats;        // (rows, chunks): max, sum of exponentials
   uint64_t *lists;      // (rows, chunks, k)
 };
 
@@ -154,79 +150,9 @@ __device__ __forceinline__ void rank_keys(const uint64_t *list, int n, int k, F 
   }
 }
 
-// The rows of a group as its last CTA knows them, in shared memory.
-struct GroupRows {
-  float base[kMaxBeams], max[kMaxBeams], log[kMaxBeams];   // log: of the sum
-  float next[kMaxBeams];   // the most that tokens outside the lists may score (NaN: none)
-  int done[kMaxBeams];
-  __device__ __forceinline__ bool live(int b) const {
-    return !done[b] && fabsf(max[b]) < INFINITY && fabsf(log[b]) < INFINITY &&
-           fabsf(base[b]) < INFINITY;
-  }
-  __device__ __forceinline__ float score(int b, float x) const {
-    return base[b] + ((x - max[b]) - log[b]);
-  }
-};
-
-// Puts the candidates that score the same as the last of top[k] in order where
-// the parts' lists left some out: the rows of those beams are read in order of
-// their tokens until enough are found. By all threads; rare.
-__device__ __noinline__ void settle_ties(const BeamParams &p, const GroupRows &rows,
-                                         int group, uint64_t *top, uint64_t *list,
-                                         int *s_warp) {
-  constexpr int kDeep = 8;   // tokens of a thread on the way
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, k = p.k;
-  const float cut = key_value(top[k - 1]);
-  int above = 0;   // (the same in all threads)
-  while (key_value(top[above]) > cut) ++above;
-  const int need = k - above;
-  int found = 0;
-  for (int b = 0; b < p.beams && found < need; ++b) {
-    if (!(rows.next[b] >= cut)) continue;
-    const float *x = p.logits + ((size_t)group * p.beams + b) * p.ld;
-    for (int t0 = 0; t0 < p.vocab && found < need; t0 += kDeep * kBeamThreads) {
-      float v[kDeep];
-#pragma unroll
-      for (int i = 0; i < kDeep; ++i) {
-        const int t = t0 + i * kBeamThreads + tid;
-        v[i] = t < p.vocab ? __ldg(x + t) : 0.f;
-      }
-      uint32_t hits = 0;
-#pragma unroll
-      for (int i = 0; i < kDeep; ++i)
-        if (t0 + i * kBeamThreads + tid < p.vocab && rows.score(b, v[i]) == cut) hits |= 1u << i;
-      if (!__syncthreads_or(hits)) continue;
-      for (int i = 0; i < kDeep; ++i) {
-        const uint32_t mine = __ballot_sync(~0u, hits >> i & 1);
-        if (lane == 0) s_warp[warp] = __popc(mine);
-        __syncthreads();
-        int at = found;
-        for (int w = 0; w < kBeamWarps; ++w) {
-          if (w < warp) at += s_warp[w];
-          found += s_warp[w];
-        }
-        at += __popc(mine & ((1u << lane) - 1));
-        if ((hits >> i & 1) && at < need)
-          list[at] = rank_key(cut, (uint32_t)b * p.vocab + t0 + i * kBeamThreads + tid);
-        __syncthreads();
-      }
-    }
-  }
-  // beside those of the other beams, which were listed
-  int n = min(found, need);
-  for (int i = above; i < k; ++i)
-    if (!(rows.next[key_index(top[i]) / p.vocab] >= cut)) {
-      if (tid == 0) list[n] = top[i];
-      ++n;
-    }
-  __syncthreads();
-  rank_keys(list, n, need, [&](int rank, uint64_t key) { top[above + rank] = key; });
-  __syncthreads();
-}
-
 template <bool kVec>
 __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
-    beam_select_kernel(const __grid_constant__ BeamParams p) {
+    beam_select_kernel(const BeamParams p) {
   griddep_launch();
   griddep_wait();
   constexpr int kKeys = kBatch * kBeamThreads + kMaxK;
@@ -235,9 +161,9 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
   __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
   __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
-  __shared__ int s_n, s_last, s_skip;
-  __shared__ GroupRows s_rows;
-  __shared__ int s_count[kBeamWarps];
+  __shared__ int s_n, s_last;
+  __shared__ float s_base[kMaxBeams], s_max[kMaxBeams], s_log[kMaxBeams];
+  __shared__ int s_done[kMaxBeams];
   const int chunk = blockIdx.x, row = blockIdx.y, group = row / p.beams;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = p.k;
@@ -275,10 +201,10 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
 #pragma unroll
       for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, v[i]);
       // (a NaN anywhere, or +inf, makes the sum NaN; -inf alone leaves it 0)
-      const float mn = fmaxf(m, top), zero = mn == -INFINITY ? 0.f : mn;
+      const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
       float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2((v[i] - zero) * kLog2e);
+      for (int i = 0; i < kPerLane; ++i) add[i & 3] += fast_exp2((v[i] - base) * kLog2e);
       // (a factor of exactly 1 while the maximum stays: a rounding of it would
       // compound over the steps)
       if (mn != m) s *= fast_exp2((m - mn) * kLog2e);
@@ -332,7 +258,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     const int per = warp_largest(mine, k, s_list + warp * 32);
     if (tid == 0) {
       s_bound = 0;
-      s_n = s_skip = 0;
+      s_n = 0;
     }
     __syncthreads();
     // (four lanes a key, each against two warps' keys)
@@ -351,61 +277,49 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     __syncthreads();
     const uint64_t bound = s_bound;
     const float least = bound ? key_value(bound) : -INFINITY;
-    // list the values that reach it, and for equal scores those just below (which
-    // covers scores of up to 2^14); a thread's other steps only if their largest
-    // value may be such
-    const float low = least - fmaf(fabsf(least), 0x1p-20f, 0x1p-8f);
-    if (any && m >= low) {
+    // list the values that reach it; a thread's other steps only if their
+    // largest value may (equal ones do not where the step starts past the
+    // bound's index)
+    if (mine >= bound && any) {
       auto list = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-          if (!(v[i] >= low) || t0 + at(i) >= end) continue;
+          if (!(v[i] >= least) || t0 + at(i) >= end) continue;
           const uint64_t key = rank_key(v[i], (uint32_t)(t0 + at(i)));
-          if (key < bound && v[i] == least) continue;
+          if (key < bound) continue;
           const int to = atomicAdd(&s_n, 1);
           if (to < kKeys) s_list[to] = key;
         }
       };
-      // (many threads may have values equal to the bound's, past its index: what
-      // else lies in their other steps is not looked for)
-      auto may = [&](float top) {
-        const bool skip = top == least && mine < bound;
-        if (skip) s_skip = 1;
-        return top >= low && !skip;
+      auto may = [&](float top, int t) {
+        return !bound || top > least || (top == least && t <= (int)key_index(bound));
       };
       list(best);
-      if (second != best && may(m2)) {
+      if (second != best && may(m2, second)) {
         load(second, v);
         list(second);
       }
-      if (may(other)) {
+      if (may(other, begin)) {
 #pragma unroll 1
         for (int t = begin; t < end; t += kStep) {
           if (t == best || t == second) continue;
+          if (!may(other, t)) break;
           load(t, v);
           list(t);
         }
       }
     }
     __syncthreads();
-    const size_t part = (size_t)row * p.chunks + chunk;
-    uint64_t *out = p.lists + part * k;
-    auto put = [&](int rank, uint64_t key) {
-      if (rank < k)
-        out[rank] = key;
-      else
-        p.stats[part].z = s_skip ? fmaxf(least, key_value(key)) : key_value(key);
-    };
+    uint64_t *out = p.lists + ((size_t)row * p.chunks + chunk) * k;
     const int n = s_n;
     if (n <= kKeys) {
-      rank_keys(s_list, n, k + 1, put);
+      rank_keys(s_list, n, k, [&](int rank, uint64_t key) { out[rank] = key; });
       for (int i = n + tid; i < k; i += kBeamThreads) out[i] = 0;   // a short last part
-      if (tid == 0 && n <= k) p.stats[part].z = s_skip ? least : low;
     } else {
       // more values above the bound than the list holds (they all lie in the
-      // same threads' shares): rounds of the largest below the last
+      // same threads' shares): k rounds of the largest below the last
       uint64_t last = ~0ull;
-      for (int j = 0; j <= k; ++j) {
+      for (int j = 0; j < k; ++j) {
         uint64_t top = 0;
         for (int t = begin; t < end; t += kStep) {
           load(t, v);
@@ -421,7 +335,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
         last = 0;
 #pragma unroll
         for (int w = 0; w < kBeamWarps; ++w) last = s_warp[w] > last ? s_warp[w] : last;
-        if (tid == 0) put(j, last);
+        if (tid == 0) out[j] = last;
       }
     }
     if (tid == 0) {
@@ -431,8 +345,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
 #pragma unroll
       for (int w = 0; w < kBeamWarps; ++w)
         ss += s_m[w] == -INFINITY ? s_s[w] : s_s[w] * fast_exp2((s_m[w] - all) * kLog2e);
-      p.stats[part].x = all;
-      p.stats[part].y = ss;
+      p.stats[(size_t)row * p.chunks + chunk] = make_float2(all, ss);
     }
   }
   __threadfence();
@@ -464,34 +377,25 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     const int r = group * p.beams + b;
     const bool done = p.done && p.done[r];
     const float base = p.scores[r];
-    const float4 *stats = p.stats + (size_t)r * p.chunks;
-    const float4 own = !done && lane < p.chunks ? __ldcg(stats + lane)
-                                                : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-    float mm = own.x, ss = 0.f, next = own.z;
+    const float2 *stats = p.stats + (size_t)r * p.chunks;
+    const float2 own = !done && lane < p.chunks ? __ldcg(stats + lane)
+                                                : make_float2(-INFINITY, 0.f);
+    float mm = own.x, ss = 0.f;
     if (!done)
-      for (int c = lane + 32; c < p.chunks; c += 32) {
-        const float4 st = __ldcg(stats + c);
-        mm = fmaxf(mm, st.x);
-        next = fmaxf(next, st.z);
-      }
+      for (int c = lane + 32; c < p.chunks; c += 32) mm = fmaxf(mm, __ldcg(stats + c).x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
-      next = fmaxf(next, __shfl_xor_sync(~0u, next, o));
-    }
-    auto add = [&](float4 st) { ss += st.x == -INFINITY ? st.y : st.y * expf(st.x - mm); };
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+    auto add = [&](float2 st) { ss += st.x == -INFINITY ? st.y : st.y * expf(st.x - mm); };
     add(own);
     if (!done)
       for (int c = lane + 32; c < p.chunks; c += 32) add(__ldcg(stats + c));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
     if (lane == 0) {
-      s_rows.done[b] = done;
-      s_rows.base[b] = base;
-      s_rows.max[b] = mm;
-      s_rows.log[b] = logf(ss);
-      s_rows.next[b] =
-          s_rows.live(b) && next > -INFINITY ? s_rows.score(b, next) : nanf("");
+      s_done[b] = done;
+      s_base[b] = base;
+      s_max[b] = mm;
+      s_log[b] = logf(ss);
     }
   }
   __syncthreads();
@@ -507,20 +411,22 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       uint64_t made = 0;
       if (i < n) {
         const int b = i / per, c = i - b * per;
+        const float base = s_base[b], top = s_max[b], log_sum = s_log[b];
         float score = -INFINITY;
         uint32_t token = c;
         bool is = true;
-        if (s_rows.done[b]) {
+        if (s_done[b]) {
           // the pad token, then others at -inf in order
           is = c < k;
           token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
-          if (c == 0) score = s_rows.base[b];
-        } else if (!s_rows.live(b)) {
+          if (c == 0) score = base;
+        } else if (!(fabsf(top) < INFINITY && fabsf(log_sum) < INFINITY &&
+                     fabsf(base) < INFINITY)) {
           is = c < k;   // the beam has no finite candidate
         } else {
           is = key[j] != 0;
           token = key_index(key[j]);
-          score = s_rows.score(b, key_value(key[j]));
+          score = base + ((key_value(key[j]) - top) - log_sum);
         }
         if (!(score == score)) score = -INFINITY;
         if (is) made = rank_key(score, (uint32_t)b * p.vocab + token);
@@ -543,8 +449,6 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
       __syncthreads();
     }
   }
-  if (__any_sync(~0u, lane < p.beams && s_rows.next[lane] >= key_value(s_top[k - 1])))
-    settle_ties(p, s_rows, group, s_top, s_list, s_count);   // (all warps or none)
   if (tid < k) {
     const uint32_t at = key_index(s_top[tid]);
     p.out_scores[(size_t)group * k + tid] = key_value(s_top[tid]);
@@ -552,7 +456,7 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     p.out_tokens[(size_t)group * k + tid] = at % p.vocab;
     if (p.out_done)
       p.out_done[(size_t)group * k + tid] =
-          s_rows.done[at / p.vocab] || (int)(at % p.vocab) == p.eos;
+          s_done[at / p.vocab] || (int)(at % p.vocab) == p.eos;
   }
 }
 
@@ -654,7 +558,7 @@ extern "C" int tllm_beam_workspace(int groups, int beams, int vocab, int k, size
   // and for fewer rows too
   const size_t rows = (size_t)groups * beams, most = (size_t)kCtasPerSm * sm_count();
   const size_t parts = rows > most ? rows : most;
-  *bytes = kCounterBytes + align256(parts * sizeof(float4)) + parts * k * sizeof(uint64_t);
+  *bytes = kCounterBytes + align256(parts * sizeof(float2)) + parts * k * sizeof(uint64_t);
   return TLLM_OK;
 }
 
@@ -700,8 +604,8 @@ extern "C" int tllm_beam_select(const tllm_beam_step *step, tllm_stream_t stream
   char *w = static_cast<char *>(workspace);
   p.counters = reinterpret_cast<int *>(w);
   w += kCounterBytes;
-  p.stats = reinterpret_cast<float4 *>(w);
-  w += align256((size_t)groups * beams * p.chunks * sizeof(float4));
+  p.stats = reinterpret_cast<float2 *>(w);
+  w += align256((size_t)groups * beams * p.chunks * sizeof(float2));
   p.lists = reinterpret_cast<uint64_t *>(w);
   const bool vec = ((uintptr_t)logits & 15) == 0 && p.ld % 4 == 0;
   TLLM_CUDA(launch_pdl(vec ? beam_select_kernel<true> : beam_select_kernel<false>,
