@@ -391,9 +391,12 @@ int tllm_page_copy(void *arena, long plane_stride, int planes, long page_stride,
  * One selection step of beam search for `groups` requests of `beams` beams
  * each (rows g * beams + b of logits (rows, vocab) f32, row stride ld, 0: vocab):
  *   candidate (b, t) = scores[g][b] + (logits[b][t] - logsumexp(logits[b]))
- * and the k best of each group's beams * vocab candidates, best first, equal
- * ones by the lower beam, then the lower token: out_scores, out_parents
- * (beam within the group) and out_tokens, all (groups, k). A beam with
+ * and the k best of each group's beams * vocab candidates, best first:
+ * out_scores, out_parents (beam within the group) and out_tokens, all
+ * (groups, k). Equal scores go to the lower beam, and within a beam (where
+ * unequal logits may round to one score) to the larger logit, then the lower
+ * token; those of -inf, which are none, to the lower beam and token. Finite
+ * logits may be of any size. A beam with
  * done[row] != 0 (done may be NULL) has one candidate, (pad_token,
  * scores[row]). NaN candidates, and all of a beam whose score is +inf, count
  * as -inf. out_done (groups, k), may be NULL: 1 for a candidate whose beam is

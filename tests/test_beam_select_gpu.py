@@ -123,6 +123,68 @@ def test_a_masked_beam_beside_others():
     assert np.abs(s - ws).max() < 2.0 ** -16
 
 
+def rounded(c):
+    """Candidates as the fp32 scores that they have, where these do not hang on
+    the last bits of the logarithm: every one is further than 2^-13 of a unit
+    from the middle of two."""
+    s = c.astype(np.float32)
+    unit = np.spacing(np.abs(s.max()))
+    off = np.abs(c / unit - np.floor(c / unit) - 0.5)
+    assert (off[np.isfinite(c)] > 2.0 ** -13).all()
+    return s.astype(np.float64)
+
+
+def best_of_equal(s, logits, k, vocab):
+    """The k best by fp32 score, beam, logit and token, in this order."""
+    x = logits.astype(np.float64).reshape(s.shape)
+    n = np.arange(s.shape[1])
+    at = np.stack([np.lexsort((n, -x[g], n // vocab, -s[g])) for g in range(len(s))])[:, :k]
+    return np.take_along_axis(s, at, 1), at // vocab, at % vocab
+
+
+@pytest.mark.parametrize("rows", ["few", "many"])
+@pytest.mark.parametrize("V,W,k", [(20000, 1, 1), (20000, 1, 8), (5000, 4, 7), (12289, 3, 64),
+                                   (40000, 2, 33)])
+def test_equal_scores_of_unequal_logits(rows, V, W, k):
+    """Beams so unlikely that many logits give the same fp32 score: one order of
+    all candidates, by score, beam, logit and token, at the end of a part's list
+    as among the listed ones."""
+    rng = np.random.default_rng(V + k)
+    x = rng.standard_normal((W, V)).astype(np.float32)
+    x = np.round(x * 32) / 32
+    base = np.full((1, W), -2.0 ** 20, np.float32)       # scores in units of 1/8
+    base[0, W // 2] -= 1
+    ws, wp, wt = best_of_equal(rounded(candidates(x, base)), x, k, V)
+    assert (ws[0, 1:] == ws[0, :-1]).any() or k == 1
+    G = 1 if rows == "few" else -(-MANY // W)
+    s, p, t = run(np.tile(x, (G, 1)), np.tile(base, (G, 1)), k)
+    assert (p == wp).all() and (t == wt).all() and (s == ws).all()
+
+
+def test_scores_that_all_collapse():
+    """All candidates of a beam equal (a score of -1e30): its largest logits, of
+    the lowest beams; finished beams and masked tokens in their places."""
+    V, k = 30000, 40
+    x = np.random.default_rng(8).standard_normal((4, V)).astype(np.float32)
+    x[1, :17] = -np.inf
+    x[1, 19:] = LOWEST
+    scores = np.array([[-2e30, -1e30, -1e30, -1e30]], np.float32)
+    order = np.argsort(-x, axis=1, kind="stable")
+    s, p, t = run(x, scores, k)
+    # (two tokens at -1e30; LOWEST less the maximum is far below)
+    assert p[0].tolist() == [1, 1] + [2] * (k - 2) and (s == np.float32(-1e30)).all()
+    assert t[0].tolist() == order[1, :2].tolist() + order[2, :k - 2].tolist()
+    done = np.array([[0, 1, 0, 0]])
+    s, p, t = run(x, scores, k, done, V - 1)
+    assert p[0].tolist() == [1] + [2] * (k - 1)
+    assert t[0].tolist() == [V - 1] + order[2, :k - 1].tolist()
+    x[1] = -np.inf                       # fewer than k candidates in all
+    x[1, [5, 50, 500]] = [1, 3, 2]
+    s, p, t = run(x[1:2], scores[:, 1:2], 6)
+    assert t[0].tolist() == [50, 500, 5, 0, 1, 2]
+    assert (s[0, :3] == np.float32(-1e30)).all() and (s[0, 3:] == -np.inf).all()
+
+
 def crowded(V, lanes, kVec=True):
     """Rows whose large values all lie in the shares of a few threads, in every
     step of 4096 logits; the largest in the last ones."""

@@ -12,7 +12,10 @@
 // group to finish joins them. Each logit is read once.
 //
 // Values carry their index in a 64-bit code, so all are distinct and ties are
-// in order. A thread reads its share of the part with the next 16 values on the
+// in order. Unequal logits may round to equal scores (a beam at -1000 collapses
+// logits 6e-5 apart), so the group's order is by score, beam and then the same
+// code of logit and token: by score alone, the lower token would win among the
+// listed ones and the larger logit at the end of a part's list. A thread reads its share of the part with the next 16 values on the
 // way, keeps the maximum and the sum, and remembers its two best steps (of 16
 // values) and the largest value outside them. The k-th largest of the threads'
 // own maxima is a key that the part's k largest reach; the few threads that
@@ -134,10 +137,6 @@ __device__ __forceinline__ int warp_largest(uint64_t key, int k, uint64_t *out) 
   return k;
 }
 
-__device__ __forceinline__ void keep(uint64_t key, uint64_t *list, int *n) {
-  list[atomicAdd(n, 1)] = key;
-}
-
 // Calls put(rank, key) for the k largest of the n keys of a list in shared
 // memory; all threads, after a barrier.
 template <typename F>
@@ -157,8 +156,8 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
   griddep_wait();
   constexpr int kKeys = kBatch * kBeamThreads + kMaxK;
   static_assert(kBeamWarps * 32 <= kKeys, "the threads' keys use the same memory");
-  __shared__ uint64_t s_list[kKeys];
-  __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK];
+  __shared__ uint64_t s_list[kKeys], s_logit[kKeys];
+  __shared__ uint64_t s_warp[kBeamWarps], s_top[kMaxK], s_token[kMaxK];
   __shared__ unsigned long long s_bound;
   __shared__ float s_m[kBeamWarps], s_s[kBeamWarps];
   __shared__ int s_n, s_last;
@@ -399,49 +398,70 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     }
   }
   __syncthreads();
-  // candidates in batches of kBatch per thread beside the best of those before
+  // candidates in batches of kBatch per thread beside the best of those before:
+  // the code of score and beam, then that of logit and token.
   int kept = 0;
   for (int i0 = 0; i0 < n; i0 += kBatch * kBeamThreads) {
     if (i0 > 0) load(i0);
-    uint64_t best = tid < kept ? s_top[tid] : 0;
-    const uint64_t old = best;
+    const uint64_t old = tid < kept ? s_top[tid] : 0;
+    const uint64_t old_key = tid < kept ? s_token[tid] : 0;
+    uint64_t best = old, code[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int i = i0 + j * kBeamThreads + tid;
-      uint64_t made = 0;
+      code[j] = 0;
       if (i < n) {
         const int b = i / per, c = i - b * per;
         const float base = s_base[b], top = s_max[b], log_sum = s_log[b];
         float score = -INFINITY;
-        uint32_t token = c;
         bool is = true;
         if (s_done[b]) {
           // the pad token, then others at -inf in order
           is = c < k;
-          token = c == 0 ? p.pad : (c - 1 < p.pad ? c - 1 : c);
           if (c == 0) score = base;
+          key[j] = rank_key(-INFINITY, c == 0 ? p.pad : c - 1 < p.pad ? c - 1 : c);
         } else if (!(fabsf(top) < INFINITY && fabsf(log_sum) < INFINITY &&
                      fabsf(base) < INFINITY)) {
           is = c < k;   // the beam has no finite candidate
+          key[j] = rank_key(-INFINITY, c);
         } else {
           is = key[j] != 0;
-          token = key_index(key[j]);
           score = base + ((key_value(key[j]) - top) - log_sum);
         }
         if (!(score == score)) score = -INFINITY;
-        if (is) made = rank_key(score, (uint32_t)b * p.vocab + token);
+        // (impossible ones by beam and token)
+        const uint32_t low = score == -INFINITY ? (uint32_t)b * p.vocab + key_index(key[j]) : b;
+        if (is) code[j] = rank_key(score, low);
       }
-      key[j] = made;
-      best = made > best ? made : best;
+      best = code[j] > best ? code[j] : best;
     }
     const uint64_t bound = block_bound(best, k, s_warp);
-    if (old && old >= bound) keep(old, s_list, &s_n);
+    auto keep = [&](uint64_t c, uint64_t logit) {
+      if (c == 0 || c < bound) return;
+      const int to = atomicAdd(&s_n, 1);
+      s_list[to] = c;
+      s_logit[to] = logit;
+    };
+    keep(old, old_key);
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (key[j] && key[j] >= bound) keep(key[j], s_list, &s_n);
+    for (int j = 0; j < kBatch; ++j) keep(code[j], key[j]);
     __syncthreads();
     const int found = s_n;
-    rank_keys(s_list, found, k, [&](int rank, uint64_t code) { s_top[rank] = code; });
+    for (int i = tid; i < found; i += kBeamThreads) {
+      const uint64_t mine = s_list[i], logit = s_logit[i];
+      int rank = 0, equal = 0;
+      for (int j = 0; j < found; ++j) {
+        const uint64_t other = s_list[j];
+        rank += other > mine;
+        equal += other == mine;
+      }
+      if (equal > 1)   // (rare)
+        for (int j = 0; j < found; ++j) rank += s_list[j] == mine && s_logit[j] > logit;
+      if (rank < k) {
+        s_top[rank] = mine;
+        s_token[rank] = logit;
+      }
+    }
     kept = min(found, k);
     __syncthreads();
     if (i0 + kBatch * kBeamThreads < n) {
@@ -450,13 +470,14 @@ __global__ void __launch_bounds__(kBeamThreads, kCtasPerSm)
     }
   }
   if (tid < k) {
-    const uint32_t at = key_index(s_top[tid]);
-    p.out_scores[(size_t)group * k + tid] = key_value(s_top[tid]);
-    p.out_parents[(size_t)group * k + tid] = at / p.vocab;
-    p.out_tokens[(size_t)group * k + tid] = at % p.vocab;
+    const float score = key_value(s_top[tid]);
+    const uint32_t low = key_index(s_top[tid]);
+    const int b = score == -INFINITY ? low / p.vocab : low, token = key_index(s_token[tid]);
+    p.out_scores[(size_t)group * k + tid] = score;
+    p.out_parents[(size_t)group * k + tid] = b;
+    p.out_tokens[(size_t)group * k + tid] = token;
     if (p.out_done)
-      p.out_done[(size_t)group * k + tid] =
-          s_done[at / p.vocab] || (int)(at % p.vocab) == p.eos;
+      p.out_done[(size_t)group * k + tid] = s_done[b] || token == p.eos;
   }
 }
 

@@ -37,8 +37,8 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
     out_scores, out_parents, out_tokens
              (groups, k) float32 / int32 / int32, best first: the candidate's
              score ``scores[b] + log_softmax(logits[b])[t]``, its beam b within
-             the group and its token t; equal scores by the lower beam, then
-             the lower token; k <= 64
+             the group and its token t; equal scores by the lower beam, within
+             a beam by the larger logit, then the lower token; k <= 64
     done     (groups, beams) or (groups * beams,) int32 or None: a beam with a
              value != 0 has one candidate, ``pad_token`` at its own score
     out_done (groups, k) int32 or None: whether the candidate's beam is done or
