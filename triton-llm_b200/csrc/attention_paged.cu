@@ -209,6 +209,12 @@ __device__ void finish_split(const AttnParams &p, const RowSpan &x, int row, int
 // over 32 lanes cost 16 shuffles, not 80, and end in one lane each, which keeps
 // the running maximum and sum of its head. Each group of LPR lanes has its own
 // over its keys; they are joined at the end.
+//
+// Bound by instruction issue where several heads share the keys: 16 rows of
+// 24/8/128 fp32 with 1024 to 8192 keys take 139 us (0.67 of HBM's bandwidth; 65 % of
+// the issue slots of SMs that are active for 85 % of the time; 3 heads run as 4),
+// 64 rows of the same over bf16 pages of 20 slots 417 (0.45), 64 of 12/4/96 176 (0.40);
+// with one head per KV head by HBM: 32 rows of 32/32/64 fp32 96.5 (0.90).
 // --------------------------------------------------------------------------
 constexpr int kGenWarps = 8;
 
@@ -1423,8 +1429,11 @@ int launch_rows_t(const AttnParams &p, int lpr, int nv, dim3 grid, cudaStream_t 
   return TLLM_ERR_UNSUPPORTED;
 }
 
-// A split of fewer keys costs more than it saves (6 rows of 12 heads of 64 fp32,
-// 17 to 1003 keys: 13.1 us with 64, 10.6 with 128, 15.3 with 256).
+// A split of fewer keys costs more than it saves. With 64, 128 and 256: 6 rows of
+// 12 heads of 64 fp32 with 17 to 1003 keys 12.9, 10.2 and 14.0 us; one row of
+// 24/8/128 fp32 with 3000 keys 19.3, 14.8, 18.8; 4 rows of 9/3/64 fp32 with 100 to
+// 2000 keys 8.4, 9.2, 10.5; 16 rows of 6/2/96 bf16 with 100 to 4000 keys 23.3, 23.2,
+// 16.9. Larger calls take longer splits anyway.
 constexpr int kMinKeys = 128;
 
 constexpr size_t kMaxScratch = 512u << 20;   // of the splits, whatever the rows

@@ -15,12 +15,14 @@
 // in order. Unequal logits may round to equal scores (a beam at -1000 collapses
 // logits 6e-5 apart), so the group's order is by score, beam and then the same
 // code of logit and token: by score alone, the lower token would win among the
-// listed ones and the larger logit at the end of a part's list. A thread reads its share of the part with the next 16 values on the
+// listed ones and the larger logit at the end of a part's list.
+//
+// A thread reads its share of the part with the next 16 values on the
 // way, keeps the maximum and the sum, and remembers its two best steps (of 16
 // values) and the largest value outside them. The k-th largest of the threads'
 // own maxima is a key that the part's k largest reach; the few threads that
 // reach it read those steps again (from L2) and list what does. Bound by HBM
-// while it reads (9 us of 25 for 16 x 8 beams over 128256 tokens, 66 MB), then
+// while it reads (9 us of 26 for 16 x 8 beams over 128256 tokens, 66 MB), then
 // by the latency of a few dependent passes; a list of candidates kept up during
 // the reading took 31 us, k rounds of maxima over all values 121.
 #include <cmath>

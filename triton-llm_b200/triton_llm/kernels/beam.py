@@ -70,8 +70,8 @@ def beam_select(logits, scores, out_scores, out_parents, out_tokens, done=None,
         if stream is not None:
             raise ValueError("a call on another stream needs its own workspace")
         # (one of a larger call holds a smaller one's parts; k > 64 is refused)
-        rows = 1 << max(0, n - 1).bit_length()
-        most = 1 << max(0, k - 1).bit_length() if k <= 64 else k
+        rows = 1 << (n - 1).bit_length()
+        most = 1 << (k - 1).bit_length() if k <= 64 else k
         workspace = _workspace(lambda: BeamWorkspace(rows, 1, max(vocab, most), most),
                                "beam", device_of(logits), rows, most)
     _lib.call("tllm_beam_select", _lib.BEAM_STEP.pack(
