@@ -20,7 +20,7 @@ class FakeDevice:
              "tllm_beam_select")
 
     def __init__(self, real):
-        self._real, self.log = real, []
+        self._real, self.log, self.refuse = real, [], None
 
     def __getattr__(self, name):
         if name not in self.NAMES:
@@ -32,7 +32,7 @@ class FakeDevice:
                 self.select = args[0]
             if name in ("tllm_malloc", "tllm_malloc_static"):
                 args[0]._obj.value = 1 << 20
-            return 0
+            return _lib.ERR_CUDA if name == self.refuse else 0
         return call
 
 
@@ -59,6 +59,16 @@ def test_ready_for_any_stream(device, make):
     del ws
     assert log.count("tllm_free_static") == n and "tllm_free" not in log
     assert "tllm_device_synchronize" in log[at:log.index("tllm_free_static")]
+
+
+def test_kept_where_the_device_cannot_be_waited_for(device):
+    """Released in the middle of a graph capture, a workspace's memory stays: the
+    work that uses it may not be over."""
+    ws, free = PagedWorkspace(4, 24, 8, 128), len(device.log)
+    device.refuse = "tllm_device_synchronize"
+    del ws
+    assert "tllm_device_synchronize" in device.log[free:]
+    assert "tllm_free_static" not in device.log
 
 
 def test_attention_scratch_is_bounded():

@@ -203,8 +203,9 @@ class Scratch:
             cur = ctypes.c_int(0)
             lib.tllm_get_device(ctypes.byref(cur))
             lib.tllm_set_device(self.device)
-            lib.tllm_device_synchronize()
-            lib.tllm_free_static(self.ptr)
+            # (kept where that cannot be waited for, as during a graph capture)
+            if lib.tllm_device_synchronize() == 0:
+                lib.tllm_free_static(self.ptr)
             lib.tllm_set_device(cur.value)
         except Exception:
             pass
